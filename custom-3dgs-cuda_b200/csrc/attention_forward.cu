@@ -1,0 +1,465 @@
+// Cross attention forward on the tensor cores, for several queries.
+//
+// A CTA holds two tiles of 128 query rows of one head and walks over tiles of 128 keys. For each
+// pair of tiles S = q k^T is a product into tensor memory; a warpgroup with one thread for each
+// query row reads its row of S, keeps the running maximum and sum, writes P = exp(S - max) back
+// over S in 16 bits, and P v is added to the row's accumulator, also in tensor memory. Four
+// warps serve the first query tile, four the second, one warp issues the products, one the
+// copies. While one tile's softmax runs, the other tile's products do.
+//
+// The maximum that P is formed with may lag behind the true one by up to kLag powers of two: the
+// accumulator (128 rows x D numbers through registers) is rescaled only when a row's maximum has
+// grown by more, which after the first tiles is rare. P is at most 2^kLag then, far inside both
+// 16-bit types' range; its rounding to 16 bits (the products' operand type) is relative, so
+// nothing is lost. The row sum adds P before that rounding, in 32 bits.
+//
+// With few query tiles the keys are split over CTAs: each writes its normalised output in 32
+// bits and its lse, and combine_kernel joins them with weights exp(lse_split - lse).
+#include <algorithm>
+#include <cmath>
+
+#include "attention.cuh"
+#include "capi_internal.h"
+#include "tensor_core.cuh"
+
+namespace gs {
+
+constexpr int kTileQ = 128;   // query rows of one warpgroup
+constexpr int kTileK = 128;   // keys of one tile
+constexpr float kLag = 8.0f;  // powers of two
+constexpr int kFwdThreads = 320;
+
+struct ForwardParams {
+  AttentionParams a;
+  float scale_log2;  // |scale| log2 e, above 0
+  float lag;         // kLag in units of unscaled scores
+  int negate;        // scale < 0: scores change sign first
+  int splits;
+  int kb, kh, vb, vh, qb, qh;  // 0 where all batch items (heads) share the tensor, else 1
+  float* part_out;  // [splits, B, Hq, Lq, D] where splits > 1
+  float* part_lse;  // [splits, B, Hq, Lq]
+  int mask_packs;   // mask rows may be read 16 bytes at a time
+};
+
+template <int DP>
+struct ForwardShared {
+  static constexpr int kBoxes = DP / 64;
+  static constexpr int kTileBytes = kBoxes * 128 * 128;
+  static constexpr int kStages = DP == 128 ? 2 : 4;
+  static constexpr int kBytes = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + 256;
+};
+
+// Sets s = -inf at the keys that row i of batch item b, head h leaves out: past `n`, or 0 in the
+// mask. `j0`: first key of the 32 in s.
+template <int N>
+__device__ __forceinline__ void hide(const AttentionParams& p, int packs, const unsigned char* row,
+                                     int j0, int n, unsigned* s) {
+  constexpr unsigned kMinusInf = 0xff800000u;
+  if (j0 + N <= n && packs && row) {
+#pragma unroll
+    for (int c = 0; c < N; c += 16) {
+      const uint4 m = *reinterpret_cast<const uint4*>(row + j0 + c);
+      const unsigned w[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (!((w[k / 4] >> (8 * (k % 4))) & 0xffu)) s[c + k] = kMinusInf;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (j0 + k >= n || (row && !row[j0 + k])) s[k] = kMinusInf;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+    attention_forward_kernel(const __grid_constant__ ForwardParams p,
+                             const __grid_constant__ CUtensorMap map_q,
+                             const __grid_constant__ CUtensorMap map_k,
+                             const __grid_constant__ CUtensorMap map_v) {
+  using S = ForwardShared<DP>;
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t q_full, k_full[S::kStages], k_free[S::kStages], v_full[S::kStages],
+      v_free[S::kStages], s_full[2], p_ready[2], o_full[2];
+  __shared__ unsigned tmem_slot;
+  __shared__ volatile int gave_up;
+  const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
+  const unsigned sm_q = base, sm_k = base + 2 * S::kTileBytes,
+                 sm_v = sm_k + S::kStages * S::kTileBytes;
+  const int warp = threadIdx.x / 32;
+  const AttentionParams& a = p.a;
+  const int q_blocks = (a.Lq + 2 * kTileQ - 1) / (2 * kTileQ);
+  const int q0 = blockIdx.x % q_blocks * 2 * kTileQ, bh = blockIdx.x / q_blocks;
+  const int b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hkv);
+  const int n = key_count(a, b);
+  const int tiles = (n + kTileK - 1) / kTileK;
+  const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
+  const int t1 = (int)((long long)tiles * (blockIdx.y + 1) / p.splits);
+  const int count = t1 - t0;
+  const bool two = q0 + kTileQ < a.Lq;
+
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    mbar_init(&q_full, 1);
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_free[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_free[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 128);
+      mbar_init(&o_full[i], 1);
+    }
+  }
+  if (warp == 8) tc_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = tmem_slot;
+  const unsigned tm_s = tmem, tm_o = tmem + 256;
+
+  if (warp == 9) {
+    // ---- copies ----
+    if (threadIdx.x % 32 == 0 && count > 0) {
+      const int bq = b * p.qb, hq = h * p.qh;
+      mbar_arrive_expect_tx(&q_full, (two ? 2 : 1) * S::kTileBytes);
+      for (int t = 0; t < (two ? 2 : 1); ++t)
+        for (int x = 0; x < S::kBoxes; ++x)
+          tma_load_4d(sm_q + t * S::kTileBytes + x * 16384, &map_q, x * 64, q0 + t * kTileQ, hq, bq,
+                      &q_full);
+      for (int j = 0; j < count; ++j) {
+        const int st = j % S::kStages;
+        const unsigned phase = (j / S::kStages & 1) ^ 1;
+        const int key = (t0 + j) * kTileK;
+        if (!tc_wait(&k_free[st], phase)) { gave_up = 1; break; }
+        mbar_arrive_expect_tx(&k_full[st], S::kTileBytes);
+        for (int x = 0; x < S::kBoxes; ++x)
+          tma_load_4d(sm_k + st * S::kTileBytes + x * 16384, &map_k, x * 64, key, hk * p.kh,
+                      b * p.kb, &k_full[st]);
+        if (!tc_wait(&v_free[st], phase)) { gave_up = 1; break; }
+        mbar_arrive_expect_tx(&v_full[st], S::kTileBytes);
+        for (int x = 0; x < S::kBoxes; ++x)
+          tma_load_4d(sm_v + st * S::kTileBytes + x * 16384, &map_v, x * 64, key, hk * p.vh,
+                      b * p.vb, &v_full[st]);
+      }
+    }
+  } else if (warp == 8) {
+    // ---- products ----
+    const int lane = threadIdx.x % 32;
+    const int steps = (a.D + 15) / 16;
+    const unsigned idesc_s = tc_idesc<T>(kTileK, false);
+    const unsigned idesc_o = tc_idesc<T>(steps * 16, true);
+    const bool key_mask = a.mask && a.mask_h == 0 && a.mask_q == 0;
+    const auto scores = [&](int t, int st) {  // S_t = q_t k^T
+      for (int k = 0; k < steps; ++k) {
+        const unsigned off = (k / 4) * 16384 + (k % 4) * 32;
+        tc_mma_ss(tm_s + t * 128, tc_desc(sm_q + t * S::kTileBytes + off, 16),
+                  tc_desc(sm_k + st * S::kTileBytes + off, 16), idesc_s, k > 0);
+      }
+    };
+    const auto values = [&](int t, int st, bool add) {  // O_t += P_t v
+      for (int k = 0; k < kTileK / 16; ++k)
+        tc_mma_ts(tm_o + t * 128, tm_s + t * 128 + k * 8,
+                  tc_desc(sm_v + st * S::kTileBytes + k * 2048, 16384), idesc_o, add || k > 0);
+    };
+    bool ok = count > 0 && tc_wait_warp(&q_full, 0) && tc_wait_warp(&k_full[0], 0);
+    if (ok && lane == 0) {
+      scores(0, 0);
+      tc_commit(&s_full[0]);
+      if (two) {
+        scores(1, 0);
+        tc_commit(&s_full[1]);
+      }
+      tc_commit(&k_free[0]);
+    }
+    for (int j = 0; ok && j < count; ++j) {
+      const int st = j % S::kStages, next = (j + 1) % S::kStages;
+      ok = tc_wait_warp(&v_full[st], j / S::kStages & 1);
+      if (!ok) break;
+      // What v holds at keys that no query of the CTA keeps must not reach the product, which
+      // would make 0 times NaN of it: those rows are set to zero.
+      const int key = (t0 + j) * kTileK;
+      if (n - key < kTileK || key_mask)
+        clear_rows<S::kBoxes>(sm_v + st * S::kTileBytes, kTileK, n - key,
+                              key_mask ? a.mask + b * a.mask_b + key : nullptr);
+      if (j + 1 < count) ok = tc_wait_warp(&k_full[next], (j + 1) / S::kStages & 1);
+      if (!ok) break;
+      for (int t = 0; t < (two ? 2 : 1); ++t) {
+        ok = tc_wait_warp(&p_ready[t], j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          values(t, st, j > 0);
+          if (t == (two ? 1 : 0)) tc_commit(&v_free[st]);
+          if (j + 1 < count) {
+            scores(t, next);
+            tc_commit(&s_full[t]);
+            if (t == (two ? 1 : 0)) tc_commit(&k_free[next]);
+          } else {
+            tc_commit(&o_full[t]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && count > 0) gave_up = 1;
+  } else {
+    // ---- softmax: one thread for each query row ----
+    const int t = warp / 4;
+    const int i = q0 + t * kTileQ + threadIdx.x % 128;
+    if (t == 0 || two) {
+      const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
+      const unsigned my_s = tm_s + t * 128 + lanes, my_o = tm_o + t * 128 + lanes;
+      const unsigned char* mask_row =
+          a.mask ? a.mask + b * a.mask_b + h * a.mask_h + (long long)min(i, a.Lq - 1) * a.mask_q
+                 : nullptr;
+      float m = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int j = 0; j < count; ++j) {
+        const int key = (t0 + j) * kTileK;
+        ok = tc_wait_warp(&s_full[t], j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        unsigned s[kTileK];
+#pragma unroll
+        for (int c = 0; c < kTileK; c += 32) tc_ld32(my_s + c, s + c);
+        tc_wait_ld();
+        if (p.negate) {
+#pragma unroll
+          for (int k = 0; k < kTileK; ++k) s[k] ^= 0x80000000u;
+        }
+        if (mask_row || key + kTileK > n) {
+#pragma unroll
+          for (int c = 0; c < kTileK; c += 32)
+            hide<32>(a, p.mask_packs, mask_row, key + c, n, s + c);
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < kTileK; ++k) top[k % 4] = fmaxf(top[k % 4], __uint_as_float(s[k]));
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const bool grew = mx > m + p.lag;
+        if (__any_sync(~0u, grew)) {
+          const float f = grew ? fast_exp2((m - mx) * p.scale_log2) : 1.0f;
+          if (grew) m = mx;
+          l *= f;
+          if (j > 0) {
+            for (int c = 0; c < DP; c += 16) {
+              unsigned o[16];
+              tc_ld16(my_o + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tc_st16(my_o + c, o);
+            }
+          }
+        }
+        const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < kTileK; c += 32) {
+          unsigned packed[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float e0 = fast_exp2(fmaf(__uint_as_float(s[c + k]), p.scale_log2, -off));
+            const float e1 = fast_exp2(fmaf(__uint_as_float(s[c + k + 1]), p.scale_log2, -off));
+            sum[0] += e0;
+            sum[1] += e1;
+            packed[k / 2] = pack2<T>(e0, e1);
+          }
+          tc_st16(my_s + c / 2, packed);
+        }
+        l += sum[0] + sum[1];
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_ready[t]);
+      }
+      if (ok && count > 0) ok = tc_wait_warp(&o_full[t], 0);
+      if (!ok) gave_up = 1;
+      tc_fence_after();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float lse = l == 0.0f ? -INFINITY : m * p.scale_log2 * 0.6931471805599453f + logf(l);
+      const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
+      const long long rows = (long long)a.B * a.Hq * a.Lq;
+      for (int c = 0; c < DP; c += 16) {
+        if (c >= a.D) break;
+        unsigned o[16];
+        if (ok && count > 0) {
+          tc_ld16(my_o + c, o);
+          tc_wait_ld();
+        }
+        float f[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) f[k] = l == 0.0f ? 0.0f : __uint_as_float(o[k]) * inv;
+        if (i < a.Lq) {
+          if (p.splits == 1) {
+            T* out = a.out.at<T>(b, i, h) + c;
+#pragma unroll
+            for (int k = 0; k < 16; k += 8) {
+              if (c + k >= a.D) break;
+              uint4 w;
+              w.x = pack2<T>(f[k], f[k + 1]), w.y = pack2<T>(f[k + 2], f[k + 3]);
+              w.z = pack2<T>(f[k + 4], f[k + 5]), w.w = pack2<T>(f[k + 6], f[k + 7]);
+              *reinterpret_cast<uint4*>(out + k) = w;
+            }
+          } else {
+            float* out = p.part_out + (blockIdx.y * rows + row) * a.D + c;
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              if (c + k >= a.D) break;
+              *reinterpret_cast<float4*>(out + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
+            }
+          }
+        }
+      }
+      if (i < a.Lq) {
+        if (p.splits > 1)
+          p.part_lse[blockIdx.y * rows + row] = lse;
+        else if (a.lse)
+          a.lse[row] = lse;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (gave_up) {
+    // A wait ran out. Copies still in flight end before the CTA's memory is given up.
+    if (threadIdx.x == 0) {
+      raise_device_error(kErrMmaTimeout);
+      const unsigned long long t = tma_global_ns();
+      for (int k = 0; k < (1 << 20) && tma_global_ns() - t < 10000000ull; ++k) __nanosleep(1000);
+    }
+    __syncthreads();
+  }
+  if (warp == 8) {
+    tc_fence_after();
+    tc_free(tmem, 512);
+  }
+}
+
+// out = sum over splits of exp(lse_s - lse) out_s: one warp for each row.
+template <typename T>
+__global__ void __launch_bounds__(256) combine_kernel(AttentionParams a, int splits,
+                                                      const float* part_out,
+                                                      const float* part_lse) {
+  const int lane = threadIdx.x % 32;
+  const long long rows = (long long)a.B * a.Hq * a.Lq;
+  const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+  if (row >= rows) return;
+  const int i = (int)(row % a.Lq), h = (int)(row / a.Lq % a.Hq), b = (int)(row / a.Lq / a.Hq);
+  float top = -INFINITY;
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + row]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  float total = 0.0f;
+  if (top > -INFINITY)
+    for (int s = lane; s < splits; s += 32) total += expf(part_lse[s * rows + row] - top);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+  const float lse = top > -INFINITY ? top + logf(total) : -INFINITY;
+  const int d = lane * 4;
+  float acc[4] = {};
+  if (d < a.D && lse != -INFINITY)
+    for (int s = 0; s < splits; ++s) {
+      const float ls = part_lse[s * rows + row];
+      if (ls == -INFINITY) continue;
+      const float w = expf(ls - lse);
+      const float4 o = *reinterpret_cast<const float4*>(part_out + (s * rows + row) * a.D + d);
+      acc[0] = fmaf(w, o.x, acc[0]);
+      acc[1] = fmaf(w, o.y, acc[1]);
+      acc[2] = fmaf(w, o.z, acc[2]);
+      acc[3] = fmaf(w, o.w, acc[3]);
+    }
+  if (d < a.D) {
+    const uint2 w = make_uint2(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]));
+    *reinterpret_cast<uint2*>(a.out.at<T>(b, i, h) + d) = w;
+  }
+  if (a.lse && lane == 0) a.lse[row] = lse;
+}
+
+// Splits of the keys: as many as fill the card's SMs once, each with at least two tiles of keys.
+static int forward_splits(const gs_attention_args& a) {
+  const long long ctas =
+      (long long)a.B * a.Hq * ((a.Lq + 2 * kTileQ - 1) / (2 * kTileQ));
+  const long long tiles = (a.Lk + kTileK - 1) / kTileK;
+  return (int)std::max(1ll, std::min(kSms / std::max(1ll, ctas), tiles / 2));
+}
+
+size_t attention_forward_workspace(const gs_attention_args& a) {
+  const long long splits = forward_splits(a), rows = (long long)a.B * a.Hq * a.Lq;
+  return splits > 1 ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0;
+}
+
+template <typename T, int DP>
+static cudaError_t launch_forward(const ForwardParams& p, const CUtensorMap& q,
+                                  const CUtensorMap& k, const CUtensorMap& v,
+                                  cudaStream_t stream) {
+  const auto kernel = attention_forward_kernel<T, DP>;
+  const cudaError_t err = cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ForwardShared<DP>::kBytes);
+  if (err != cudaSuccess) return err;
+  const dim3 grid((p.a.Lq + 2 * kTileQ - 1) / (2 * kTileQ) * p.a.B * p.a.Hq, p.splits);
+  kernel<<<grid, kFwdThreads, ForwardShared<DP>::kBytes, stream>>>(p, q, k, v);
+  return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch_combine(const AttentionParams& a, int splits, const float* out,
+                                  const float* lse, cudaStream_t stream) {
+  const long long rows = (long long)a.B * a.Hq * a.Lq;
+  combine_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(a, splits, out, lse);
+  return cudaGetLastError();
+}
+
+cudaError_t attention_combine(const gs_attention_args& args, int splits, const float* out,
+                              const float* lse, cudaStream_t stream) {
+  const AttentionParams a = attention_params(args);
+  return args.dtype == GS_FP16 ? launch_combine<__half>(a, splits, out, lse, stream)
+                               : launch_combine<__nv_bfloat16>(a, splits, out, lse, stream);
+}
+
+int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t stream) {
+  ForwardParams p{};
+  p.a = attention_params(a);
+  const float magnitude = std::max(std::fabs(a.scale), 1e-30f);  // a scale of 0 weighs all alike
+  p.scale_log2 = magnitude * 1.4426950408889634f;
+  p.lag = std::min(kLag / p.scale_log2, 1e30f);
+  p.negate = a.scale < 0.0f;
+  p.splits = forward_splits(a);
+  p.part_out = static_cast<float*>(workspace);
+  const long long rows = (long long)a.B * a.Hq * a.Lq;
+  p.part_lse = p.part_out + p.splits * rows * a.D;
+  p.qb = a.B > 1 && a.q.batch_stride != 0, p.qh = a.Hq > 1;
+  p.kb = a.B > 1 && a.k.batch_stride != 0, p.kh = a.Hkv > 1;
+  p.vb = a.B > 1 && a.v.batch_stride != 0, p.vh = a.Hkv > 1;
+  p.mask_packs = a.mask && (reinterpret_cast<uintptr_t>(a.mask) | (uintptr_t)a.mask_batch_stride |
+                            (uintptr_t)a.mask_head_stride | (uintptr_t)a.mask_query_stride) % 16 == 0;
+  CUtensorMap q, k, v;
+  GS_REQUIRE(encode_tokens(&q, a.dtype, a.q.data, a.D, a.Lq, a.Hq, a.B, a.q.token_stride,
+                           a.q.head_stride, a.q.batch_stride, kTileQ),
+             "the driver refused to describe q");
+  k = v = q;  // without keys nothing is copied
+  if (a.Lk > 0) {
+    GS_REQUIRE(encode_tokens(&k, a.dtype, a.k.data, a.D, a.Lk, a.Hkv, a.B, a.k.token_stride,
+                             a.k.head_stride, a.k.batch_stride, kTileK),
+               "the driver refused to describe k");
+    GS_REQUIRE(encode_tokens(&v, a.dtype, a.v.data, a.D, a.Lk, a.Hkv, a.B, a.v.token_stride,
+                             a.v.head_stride, a.v.batch_stride, kTileK),
+               "the driver refused to describe v");
+  }
+  if (a.dtype == GS_FP16)
+    GS_CUDA(a.D <= 64 ? (launch_forward<__half, 64>(p, q, k, v, stream))
+                      : (launch_forward<__half, 128>(p, q, k, v, stream)));
+  else
+    GS_CUDA(a.D <= 64 ? (launch_forward<__nv_bfloat16, 64>(p, q, k, v, stream))
+                      : (launch_forward<__nv_bfloat16, 128>(p, q, k, v, stream)));
+  count_launches(1u);
+  if (p.splits > 1) {
+    GS_CUDA(attention_combine(a, p.splits, p.part_out, p.part_lse, stream));
+    count_launches(1u);
+  }
+  return GS_OK;
+}
+
+}  // namespace gs

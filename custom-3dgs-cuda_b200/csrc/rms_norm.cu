@@ -1,0 +1,500 @@
+// Root-mean-square norm with the residual's addition, its gradient, and its 8-bit output.
+//
+//   h = x + r (or x),  rstd = 1 / sqrt(mean(h^2) + eps),  y = h rstd w.
+// Statistics and products are in 32 bits; h is rounded once when it is written to the residual
+// stream, and y is formed from the unrounded h. With u = h rstd and g = dy w:
+//   dh_total = rstd (g - u mean(g u)) + dh,  dx = dr = dh_total,  dw = sum over rows of dy u.
+// The backward reads the h that the forward wrote and the forward's rstd.
+// 8 bits: for each row, or each group of `group` numbers of it, s = max|y| / 448 and
+// q = e4m3(y / s), so that y ~ q s (448 is e4m3's largest number); s = 0 where y is all zero.
+//
+// Bound by HBM: each input is read once and each output written once, the row staying in
+// registers between the sum of squares and the scaling. ROW threads hold one row, CHUNKS packs of
+// VEC elements each; the smallest of a warp, 4 warps and 32 warps that holds the row takes it.
+// dw is summed by a fixed set of CTAs over their own rows into partial rows, which a second
+// kernel adds in a fixed order: the same bits on every run.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "capi_internal.h"
+#include "gs_common.cuh"
+#include "token_types.cuh"
+
+namespace gs {
+
+constexpr float kE4m3Max = 448.0f;
+constexpr int kNormMaxWidth = 32768;
+constexpr int kNormMaxBlocks = 148 * 4;  // CTAs (and partial rows of dw) of the backward
+
+struct NormParams {
+  const void* x;
+  const void* r;
+  const void* w;
+  void* y;        // T, or e4m3 bytes
+  void* h;        // residual stream out, or null
+  float* rstd;    // [rows] or null
+  float* scales;  // [rows, width / group]
+  long long rows;
+  int width, group;
+  float eps;
+};
+
+template <int ROW>
+__device__ __forceinline__ float row_sum(float v, float* shared) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  if constexpr (ROW > 32) {
+    constexpr int W = ROW / 32;
+    __syncthreads();  // the previous use of `shared` is over
+    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v += shared[i];
+  }
+  return v;
+}
+
+// The larger of two, NaN where either is: a row with a NaN says so in its scale.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+
+template <int ROW>
+__device__ __forceinline__ float row_max(float v, float* shared) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+  if constexpr (ROW > 32) {
+    constexpr int W = ROW / 32;
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = shared[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v = max_nan(v, shared[i]);
+  }
+  return v;
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_e4m3(unsigned char* p, const float (&v)[VEC]) {
+  Pack<unsigned char, VEC> a;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    a.v[i] = (unsigned char)__nv_cvt_float_to_fp8(v[i], __NV_SATFINITE, __NV_E4M3);
+  *reinterpret_cast<Pack<unsigned char, VEC>*>(p) = a;
+}
+
+// CTAs of max(ROW, 128) threads. Each row's threads take packs at stride ROW, so a warp's accesses
+// are consecutive.
+template <typename T, int VEC, int CHUNKS, int ROW, bool E4M3>
+__global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_kernel(NormParams p) {
+  constexpr int kThreads = ROW < 128 ? 128 : ROW;
+  __shared__ float shared[32];
+  const int lane = threadIdx.x % ROW;
+  const long long row = (long long)blockIdx.x * (kThreads / ROW) + threadIdx.x / ROW;
+  if (row >= p.rows) return;  // whole warps, and whole CTAs where ROW > 32
+  const T* x = reinterpret_cast<const T*>(p.x) + row * p.width;
+  const T* r = p.r ? reinterpret_cast<const T*>(p.r) + row * p.width : nullptr;
+  const T* w = reinterpret_cast<const T*>(p.w);
+  float h[CHUNKS][VEC];
+  float sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int i = (c * ROW + lane) * VEC;
+    if (i < p.width) {
+      load_pack<T, VEC>(x + i, h[c]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[c][k] = 0.0f;
+    }
+  }
+  if (r) {
+    float a[CHUNKS][VEC];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = (c * ROW + lane) * VEC;
+      if (i < p.width) load_pack<T, VEC>(r + i, a[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = (c * ROW + lane) * VEC;
+      if (i < p.width) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h[c][k] += a[c][k];
+        if (p.h) store_pack<T, VEC>(reinterpret_cast<T*>(p.h) + row * p.width + i, h[c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sum = fmaf(h[c][k], h[c][k], sum);
+  sum = row_sum<ROW>(sum, shared);
+  const float rstd = rsqrtf(sum / (float)p.width + p.eps);
+  if (p.rstd && lane == 0) p.rstd[row] = rstd;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int i = (c * ROW + lane) * VEC;
+    if (i < p.width) {
+      float wv[VEC];
+      load_pack<T, VEC>(w + i, wv);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[c][k] = h[c][k] * rstd * wv[k];
+      if constexpr (!E4M3) store_pack<T, VEC>(reinterpret_cast<T*>(p.y) + row * p.width + i, h[c]);
+    }
+  }
+  if constexpr (E4M3) {
+    unsigned char* q = reinterpret_cast<unsigned char*>(p.y) + row * p.width;
+    if (p.group == p.width) {
+      float top = 0.0f;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) top = max_nan(top, fabsf(h[c][k]));
+      top = row_max<ROW>(top, shared);
+      const float s = top / kE4m3Max;
+      const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+      if (lane == 0) p.scales[row] = s;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int i = (c * ROW + lane) * VEC;
+        if (i < p.width) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) h[c][k] *= inv;
+          store_e4m3<VEC>(q + i, h[c]);
+        }
+      }
+    } else {
+      // groups of 128 are 128 / VEC neighbouring lanes (VEC is 4 or 8 here): half a warp or one
+      if constexpr (VEC >= 4) {
+        const int groups = p.width / 128;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int i = (c * ROW + lane) * VEC;
+          float top = 0.0f;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) top = max_nan(top, fabsf(h[c][k]));
+#pragma unroll
+          for (int o = 64 / VEC; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
+          const float s = top / kE4m3Max;
+          const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+          if (i < p.width) {
+            if (i % 128 == 0) p.scales[row * groups + i / 128] = s;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) h[c][k] *= inv;
+            store_e4m3<VEC>(q + i, h[c]);
+          }
+        }
+      }
+    }
+  }
+}
+
+struct NormBackwardParams {
+  const void* dy;
+  const void* dh;  // or null
+  const void* h;
+  const void* w;
+  const float* rstd;
+  void* dx;
+  float* partial;  // [gridDim.x, width]
+  long long rows;
+  int width;
+};
+
+template <typename T, int VEC, int CHUNKS, int ROW>
+__global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_backward_kernel(
+    NormBackwardParams p) {
+  constexpr int kThreads = ROW < 128 ? 128 : ROW;
+  constexpr int kRows = kThreads / ROW;
+  __shared__ float shared[32];
+  // the CTA's rows of dw meet here, CHUNKS * VEC * ROW floats for each of kRows - 1 rows
+  extern __shared__ float meet[];
+  const int lane = threadIdx.x % ROW, slot = threadIdx.x / ROW;
+  const T* w = reinterpret_cast<const T*>(p.w);
+  float dw[CHUNKS][VEC];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) dw[c][k] = 0.0f;
+  for (long long row = (long long)blockIdx.x * kRows + slot; row < p.rows;
+       row += (long long)gridDim.x * kRows) {
+    const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.width;
+    const T* h = reinterpret_cast<const T*>(p.h) + row * p.width;
+    const T* dh = p.dh ? reinterpret_cast<const T*>(p.dh) + row * p.width : nullptr;
+    T* dx = reinterpret_cast<T*>(p.dx) + row * p.width;
+    const float rstd = p.rstd[row];
+    Pack<T, VEC> g[CHUNKS], u[CHUNKS], add[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = (c * ROW + lane) * VEC;
+      if (i < p.width) {
+        g[c] = *reinterpret_cast<const Pack<T, VEC>*>(dy + i);
+        u[c] = *reinterpret_cast<const Pack<T, VEC>*>(h + i);
+        if (dh) add[c] = *reinterpret_cast<const Pack<T, VEC>*>(dh + i);
+      }
+    }
+    float dot = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = (c * ROW + lane) * VEC;
+      if (i < p.width) {
+        float wv[VEC];
+        load_pack<T, VEC>(w + i, wv);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float a = to_f32<T>(g[c].v[k]), b = to_f32<T>(u[c].v[k]) * rstd;
+          dw[c][k] = fmaf(a, b, dw[c][k]);
+          dot = fmaf(a * wv[k], b, dot);
+        }
+      }
+    }
+    dot = row_sum<ROW>(dot, shared) / (float)p.width;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = (c * ROW + lane) * VEC;
+      if (i < p.width) {
+        float wv[VEC], o[VEC];
+        load_pack<T, VEC>(w + i, wv);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float a = to_f32<T>(g[c].v[k]) * wv[k], b = to_f32<T>(u[c].v[k]) * rstd;
+          o[k] = rstd * (a - b * dot);
+          if (dh) o[k] += to_f32<T>(add[c].v[k]);
+        }
+        store_pack<T, VEC>(dx + i, o);
+      }
+    }
+  }
+  if constexpr (kRows > 1) {
+    constexpr int kPer = CHUNKS * VEC * ROW;
+    if (slot) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          meet[(slot - 1) * kPer + (c * VEC + k) * ROW + lane] = dw[c][k];
+    }
+    __syncthreads();
+    if (slot) return;
+#pragma unroll
+    for (int s = 0; s < kRows - 1; ++s)
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dw[c][k] += meet[s * kPer + (c * VEC + k) * ROW + lane];
+  }
+  float* out = p.partial + (long long)blockIdx.x * p.width;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int i = (c * ROW + lane) * VEC;
+    if (i < p.width) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) out[i + k] = dw[c][k];
+    }
+  }
+}
+
+// dw = the sum of the partial rows: a warp's lanes take 32 neighbouring columns, the CTA's 8 warps
+// every eighth partial row, and the 8 sums meet in shared memory in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_dw_kernel(const float* partial, int parts, int width,
+                                                      void* dw) {
+  __shared__ float meet[8][32];
+  const int col = blockIdx.x * 32 + threadIdx.x % 32, first = threadIdx.x / 32;
+  float s = 0.0f;
+  if (col < width)
+    for (int i = first; i < parts; i += 8) s += partial[(long long)i * width + col];
+  meet[first][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (first == 0 && col < width) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += meet[i][threadIdx.x];
+    reinterpret_cast<T*>(dw)[col] = from_f32<T>(s);
+  }
+}
+
+// Calls f with the (VEC, CHUNKS, ROW) that holds a row: 16-byte packs where width and pointers
+// allow them, else single elements.
+template <typename T, typename F>
+static void with_row_shape(int width, bool packed, F&& f) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (packed) {
+    if (width <= 32 * 4 * V)
+      f.template operator()<V, 4, 32>();
+    else if (width <= 128 * 4 * V)
+      f.template operator()<V, 4, 128>();
+    else
+      f.template operator()<V, 32 / V, 1024>();
+  } else {
+    if (width <= 32 * 32)
+      f.template operator()<1, 32, 32>();
+    else
+      f.template operator()<1, 32, 1024>();
+  }
+}
+
+template <typename F>
+static void with_type(int dtype, F&& f) {
+  if (dtype == GS_FP32)
+    f.template operator()<float>();
+  else if (dtype == GS_FP16)
+    f.template operator()<__half>();
+  else
+    f.template operator()<__nv_bfloat16>();
+}
+
+static bool packs(int dtype, int width, std::initializer_list<const void*> pointers) {
+  const size_t size = element_size(dtype);
+  if (width * size % 16) return false;
+  for (const void* q : pointers)
+    if (reinterpret_cast<uintptr_t>(q) % 16) return false;
+  return true;
+}
+
+template <typename T, bool E4M3>
+struct NormLaunch {
+  const NormParams& p;
+  cudaStream_t stream;
+  template <int VEC, int CHUNKS, int ROW>
+  void operator()() const {
+    constexpr int threads = ROW < 128 ? 128 : ROW;
+    const long long blocks = (p.rows + threads / ROW - 1) / (threads / ROW);
+    rms_norm_kernel<T, VEC, CHUNKS, ROW, E4M3><<<(unsigned)blocks, threads, 0, stream>>>(p);
+  }
+};
+
+template <bool E4M3>
+struct NormByType {
+  const NormParams& p;
+  bool packed;
+  cudaStream_t stream;
+  template <typename T>
+  void operator()() const {
+    with_row_shape<T>(p.width, packed, NormLaunch<T, E4M3>{p, stream});
+  }
+};
+
+static int norm_blocks(long long rows, int width) {
+  // a row takes a warp up to 512 (fp32) or 1024 elements; the count only has to be a bound
+  (void)width;
+  return (int)std::max(1ll, std::min(rows, (long long)kNormMaxBlocks));
+}
+
+template <typename T>
+struct NormBackwardLaunch {
+  const NormBackwardParams& p;
+  int blocks;
+  cudaStream_t stream;
+  cudaError_t* err;
+  template <int VEC, int CHUNKS, int ROW>
+  void operator()() const {
+    constexpr int threads = ROW < 128 ? 128 : ROW;
+    constexpr size_t meet = (size_t)(threads / ROW - 1) * CHUNKS * VEC * ROW * sizeof(float);
+    static_assert(meet <= 48 * 1024, "the rows of dw meet in shared memory");
+    rms_norm_backward_kernel<T, VEC, CHUNKS, ROW><<<blocks, threads, meet, stream>>>(p);
+    *err = cudaGetLastError();
+  }
+};
+
+struct NormBackwardByType {
+  const NormBackwardParams& p;
+  bool packed;
+  int blocks;
+  void* dw;
+  cudaStream_t stream;
+  cudaError_t* err;
+  template <typename T>
+  void operator()() const {
+    with_row_shape<T>(p.width, packed, NormBackwardLaunch<T>{p, blocks, stream, err});
+    if (*err != cudaSuccess) return;
+    norm_dw_kernel<T><<<(p.width + 31) / 32, 256, 0, stream>>>(p.partial, blocks, p.width, dw);
+    *err = cudaGetLastError();
+  }
+};
+
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int gs_rms_norm_forward(int dtype, long long rows, int width, const void* x,
+                                   const void* residual, const void* weight, float eps, void* y,
+                                   void* h, float* rstd, void* stream) {
+  GS_API_BEGIN();
+  GS_REQUIRE(known_type(dtype), "dtype must be GS_FP32, GS_FP16 or GS_BF16");
+  GS_REQUIRE(rows >= 0 && rows < (1ll << 31), "rows must be in [0, 2^31)");
+  GS_REQUIRE(width >= 1 && width <= kNormMaxWidth, "width must be in [1, 32768]");
+  GS_REQUIRE(eps >= 0.0f, "eps must be non-negative");
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(x && weight && y, "null pointer");
+  GS_REQUIRE(!h || residual, "the residual stream is written only where a residual is added");
+  const NormParams p{x, residual, weight, y, h, rstd, nullptr, rows, width, width, eps};
+  const bool packed = packs(dtype, width, {x, residual, weight, y, h});
+  with_type(dtype, NormByType<false>{p, packed, (cudaStream_t)stream});
+  GS_CHECK_LAUNCH();
+  return GS_OK;
+  GS_API_END();
+}
+
+extern "C" int gs_rms_norm_e4m3(int dtype, long long rows, int width, int group, const void* x,
+                                const void* residual, const void* weight, float eps, void* q,
+                                float* scales, void* h, void* stream) {
+  GS_API_BEGIN();
+  GS_REQUIRE(known_type(dtype), "dtype must be GS_FP32, GS_FP16 or GS_BF16");
+  GS_REQUIRE(rows >= 0 && rows < (1ll << 31), "rows must be in [0, 2^31)");
+  GS_REQUIRE(width >= 1 && width <= kNormMaxWidth, "width must be in [1, 32768]");
+  GS_REQUIRE(eps >= 0.0f, "eps must be non-negative");
+  GS_REQUIRE(group == 0 || (group == 128 && width % 128 == 0),
+             "group must be 0 (one scale a row) or 128, dividing the width");
+  if (rows == 0) return GS_OK;
+  GS_REQUIRE(x && weight && q && scales, "null pointer");
+  GS_REQUIRE(!h || residual, "the residual stream is written only where a residual is added");
+  const bool packed = packs(dtype, width, {x, residual, weight, q, h});
+  GS_REQUIRE(group == 0 || packed, "with groups, every buffer must start on a 16-byte boundary");
+  const NormParams p{x, residual, weight, q, h, nullptr, scales, rows, width,
+                     group ? group : width, eps};
+  // a group as wide as the row is a row
+  with_type(dtype, NormByType<true>{p, packed, (cudaStream_t)stream});
+  GS_CHECK_LAUNCH();
+  return GS_OK;
+  GS_API_END();
+}
+
+extern "C" size_t gs_rms_norm_backward_workspace_size(long long rows, int width) {
+  if (rows <= 0 || width <= 0 || width > kNormMaxWidth) return 0;
+  return (size_t)norm_blocks(rows, width) * width * sizeof(float);
+}
+
+extern "C" int gs_rms_norm_backward(int dtype, long long rows, int width, const void* dy,
+                                    const void* dh, const void* h, const void* weight,
+                                    const float* rstd, void* dx, void* dw, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  GS_API_BEGIN();
+  GS_REQUIRE(known_type(dtype), "dtype must be GS_FP32, GS_FP16 or GS_BF16");
+  GS_REQUIRE(rows >= 0 && rows < (1ll << 31), "rows must be in [0, 2^31)");
+  GS_REQUIRE(width >= 1 && width <= kNormMaxWidth, "width must be in [1, 32768]");
+  GS_REQUIRE(dw, "null pointer");
+  if (rows == 0) {
+    GS_CUDA(cudaMemsetAsync(dw, 0, element_size(dtype) * width, (cudaStream_t)stream));
+    return GS_OK;
+  }
+  GS_REQUIRE(dy && h && weight && rstd && dx && workspace, "null pointer");
+  GS_REQUIRE(workspace_bytes >= gs_rms_norm_backward_workspace_size(rows, width),
+             "workspace too small");
+  GS_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "misaligned workspace");
+  const NormBackwardParams p{dy, dh, h, weight, rstd, dx, static_cast<float*>(workspace), rows,
+                             width};
+  const bool packed = packs(dtype, width, {dy, dh, h, weight, dx});
+  cudaError_t err = cudaSuccess;
+  with_type(dtype, NormBackwardByType{p, packed, norm_blocks(rows, width), dw,
+                                      (cudaStream_t)stream, &err});
+  GS_CUDA(err);
+  gs::count_launches(2u);
+  return GS_OK;
+  GS_API_END();
+}

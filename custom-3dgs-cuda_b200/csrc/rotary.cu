@@ -1,0 +1,245 @@
+// Rotary positions with several axes.
+//
+// Axis a owns d_a consecutive numbers of every head (d_a even); pair j < d_a / 2 of that block is
+// turned by the angle p_a * base_a^(-2 j / d_a):
+//   (u, v) -> (u cos - v sin, u sin + v cos),
+// with (u, v) at (j, j + d_a / 2) of the block, or at (2 j, 2 j + 1) when interleaved. Numbers
+// past the last block are copied. The gradient is the rotation by the negative angle (inverse).
+//
+// The angle is formed in turns, not radians: p * (f / 2 pi) with the frequency split into two
+// floats (made in double on the host) and the product's rounding error recovered by one fused
+// multiply-add, so the whole turns drop out exactly and a coordinate of a few thousand costs no
+// accuracy. Coordinates are float32, or int32 converted to float32 (exact up to 2^24).
+//
+// Bound by HBM: every element is read once and written once. The angles depend on the token and
+// the pair but not on the head, so a thread keeps VEC pairs' sines and cosines and walks over
+// heads, issuing the loads of kHeadsInFlight heads before it turns the first.
+#include <cmath>
+
+#include "capi_internal.h"
+#include "gs_common.cuh"
+#include "token_types.cuh"
+
+namespace gs {
+
+constexpr int kRotaryMaxAxes = 4;
+constexpr int kRotaryMaxPairs = 128;
+constexpr int kRotaryThreads = 256;
+constexpr int kHeadsInFlight = 4;
+
+struct RotaryParams {
+  const void* x;
+  void* y;
+  long long xb, xl, xh, yb, yl, yh;  // strides in elements
+  const void* pos;
+  long long pos_b, pos_l;
+  long long tokens;  // B * L
+  int L, H;
+  int n_axes;
+  int pairs, turned;      // pairs a head, and how many of them are turned
+  int items;              // pairs / VEC
+  int head_lanes;         // threads that share a token's item, each walking over its own heads
+  int tokens_per_block;
+  int interleaved;
+  float sign;
+  int axis_start[kRotaryMaxAxes + 1];  // first pair of each axis; [n_axes] = turned
+  float freq_hi[kRotaryMaxPairs], freq_lo[kRotaryMaxPairs];  // turns per unit of position
+};
+
+template <typename T, int VEC, bool INTERLEAVED, typename P>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__
+                                                                RotaryParams p) {
+  __shared__ float s_hi[kRotaryMaxPairs], s_lo[kRotaryMaxPairs];
+  for (int i = threadIdx.x; i < p.turned; i += blockDim.x) {
+    s_hi[i] = p.freq_hi[i];
+    s_lo[i] = p.freq_lo[i];
+  }
+  __syncthreads();
+  const int per_token = p.items * p.head_lanes;
+  const int slot = threadIdx.x / per_token;
+  if (slot >= p.tokens_per_block) return;
+  const int in_token = threadIdx.x - slot * per_token;
+  const int lane_h = in_token / p.items;
+  const int pair = (in_token - lane_h * p.items) * VEC;
+  const long long token = (long long)blockIdx.x * p.tokens_per_block + slot;
+  if (token >= p.tokens) return;
+  const long long b = token / p.L, l = token - b * p.L;
+
+  float c[VEC], s[VEC];
+  const bool turned = pair < p.turned;
+  int axis = 0, off_u, off_v;
+  if (turned) {
+#pragma unroll
+    for (int a = 1; a < kRotaryMaxAxes; ++a)
+      if (a < p.n_axes && pair >= p.axis_start[a]) axis = a;
+    const P raw = reinterpret_cast<const P*>(p.pos)[b * p.pos_b + l * p.pos_l + axis];
+    const float x = p.sign * (float)raw;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float hi = s_hi[pair + i];
+      const float r = x * hi;
+      const float err = fmaf(x, hi, -r) + x * s_lo[pair + i];
+      sincospif(2.0f * ((r - rintf(r)) + err), &s[i], &c[i]);
+    }
+  }
+  const int first = turned ? p.axis_start[axis] : p.turned;
+  const int end = turned ? p.axis_start[axis + 1] : p.pairs;
+  if (INTERLEAVED) {
+    off_u = 2 * pair;
+    off_v = off_u + VEC;  // the second half of 2 VEC consecutive numbers
+  } else {
+    off_u = first + pair;  // block start 2 * first, then pair - first
+    off_v = off_u + (end - first);
+  }
+  const T* x = reinterpret_cast<const T*>(p.x) + b * p.xb + l * p.xl;
+  T* y = reinterpret_cast<T*>(p.y) + b * p.yb + l * p.yl;
+  for (int h0 = lane_h; h0 < p.H; h0 += kHeadsInFlight * p.head_lanes) {
+    float u[kHeadsInFlight][VEC], v[kHeadsInFlight][VEC];
+#pragma unroll
+    for (int k = 0; k < kHeadsInFlight; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      if (h < p.H) {
+        load_pack<T, VEC>(x + h * p.xh + off_u, u[k]);
+        load_pack<T, VEC>(x + h * p.xh + off_v, v[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kHeadsInFlight; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      if (h >= p.H) break;
+      if (turned) {
+        if (INTERLEAVED) {
+          // u, v hold 2 VEC consecutive numbers: pair i is (z[2 i], z[2 i + 1])
+          float z[2 * VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) z[i] = u[k][i], z[VEC + i] = v[k][i];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float a = z[2 * i], d = z[2 * i + 1];
+            z[2 * i] = a * c[i] - d * s[i];
+            z[2 * i + 1] = a * s[i] + d * c[i];
+          }
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) u[k][i] = z[i], v[k][i] = z[VEC + i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float a = u[k][i], d = v[k][i];
+            u[k][i] = a * c[i] - d * s[i];
+            v[k][i] = a * s[i] + d * c[i];
+          }
+        }
+      }
+      store_pack<T, VEC>(y + h * p.yh + off_u, u[k]);
+      store_pack<T, VEC>(y + h * p.yh + off_v, v[k]);
+    }
+  }
+}
+
+template <typename T, int VEC, bool INTERLEAVED>
+static void launch_rotary(const RotaryParams& p, int position_type, unsigned blocks,
+                          cudaStream_t stream) {
+  if (position_type == GS_FP32)
+    rotary_kernel<T, VEC, INTERLEAVED, float><<<blocks, kRotaryThreads, 0, stream>>>(p);
+  else
+    rotary_kernel<T, VEC, INTERLEAVED, int><<<blocks, kRotaryThreads, 0, stream>>>(p);
+}
+
+template <typename T, int VEC>
+static void launch_rotary(const RotaryParams& p, int position_type, unsigned blocks,
+                          cudaStream_t stream) {
+  if (p.interleaved)
+    launch_rotary<T, VEC, true>(p, position_type, blocks, stream);
+  else
+    launch_rotary<T, VEC, false>(p, position_type, blocks, stream);
+}
+
+template <typename T>
+static void launch_rotary(const RotaryParams& p, int vec, int position_type, unsigned blocks,
+                          cudaStream_t stream) {
+  if (vec == 4)
+    launch_rotary<T, 4>(p, position_type, blocks, stream);
+  else if (vec == 2)
+    launch_rotary<T, 2>(p, position_type, blocks, stream);
+  else
+    launch_rotary<T, 1>(p, position_type, blocks, stream);
+}
+
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int gs_rotary_axes(int dtype, int B, int L, int H, int D, const gs_token_view* x,
+                              const gs_token_view* y, const void* positions, int position_type,
+                              long long position_batch_stride, long long position_token_stride,
+                              int n_axes, const int* axis_dims, const double* bases,
+                              int interleaved, int inverse, void* stream) {
+  GS_API_BEGIN();
+  GS_REQUIRE(known_type(dtype), "dtype must be GS_FP32, GS_FP16 or GS_BF16");
+  GS_REQUIRE(position_type == GS_FP32 || position_type == GS_INT32,
+             "positions must be GS_FP32 or GS_INT32");
+  GS_REQUIRE(B >= 0 && L >= 0 && H >= 0, "sizes must be non-negative");
+  GS_REQUIRE(D >= 2 && D <= 2 * kRotaryMaxPairs && D % 2 == 0,
+             "the head size must be even, between 2 and 256");
+  GS_REQUIRE(n_axes >= 1 && n_axes <= kRotaryMaxAxes, "between 1 and 4 axes");
+  GS_REQUIRE(x && y && axis_dims && bases, "null pointer");
+  int sum = 0;
+  RotaryParams p{};
+  for (int a = 0; a < n_axes; ++a) {
+    GS_REQUIRE(axis_dims[a] >= 2 && axis_dims[a] % 2 == 0 && axis_dims[a] <= D,
+               "each axis must own an even number of at least 2 of the head's numbers");
+    GS_REQUIRE(bases[a] > 0.0 && std::isfinite(bases[a]), "bases must be positive");
+    p.axis_start[a] = sum / 2;
+    for (int j = 0; j < axis_dims[a] / 2 && sum + 2 * j < D; ++j) {
+      const double turns = std::pow(bases[a], -2.0 * j / axis_dims[a]) / (2.0 * M_PI);
+      p.freq_hi[sum / 2 + j] = (float)turns;
+      p.freq_lo[sum / 2 + j] = (float)(turns - (double)p.freq_hi[sum / 2 + j]);
+    }
+    sum += axis_dims[a];
+    GS_REQUIRE(sum <= D, "the axes own more numbers than a head has");
+  }
+  p.axis_start[n_axes] = sum / 2;
+  if (B == 0 || L == 0 || H == 0) return GS_OK;
+  GS_REQUIRE(x->data && y->data && positions, "null pointer");
+  p.x = x->data;
+  p.y = y->data;
+  p.xb = x->batch_stride, p.xl = x->token_stride, p.xh = x->head_stride;
+  p.yb = y->batch_stride, p.yl = y->token_stride, p.yh = y->head_stride;
+  p.pos = positions;
+  p.pos_b = position_batch_stride, p.pos_l = position_token_stride;
+  p.tokens = (long long)B * L;
+  p.L = L, p.H = H, p.n_axes = n_axes;
+  p.pairs = D / 2, p.turned = sum / 2;
+  p.interleaved = interleaved != 0;
+  p.sign = inverse ? -1.0f : 1.0f;
+  // pairs a thread: the largest of 4, 2, 1 that divides every block of pairs, with every access
+  // (VEC elements, so 16 bytes at most) aligned
+  const size_t size = element_size(dtype);
+  int vec = 4;
+  const auto fits = [&](int n) {
+    for (int a = 0; a < n_axes; ++a)
+      if (axis_dims[a] / 2 % n) return false;
+    if ((p.pairs - p.turned) % n) return false;
+    for (const long long s : {p.xb, p.xl, p.xh, p.yb, p.yl, p.yh})
+      if (s % n) return false;
+    return (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y)) % (n * size) == 0;
+  };
+  while (vec > 1 && !fits(vec)) vec /= 2;
+  p.items = p.pairs / vec;
+  GS_REQUIRE(p.items <= kRotaryThreads, "head size");
+  p.head_lanes = (H + kHeadsInFlight - 1) / kHeadsInFlight;
+  while (p.head_lanes > 1 && p.items * p.head_lanes > kRotaryThreads)
+    p.head_lanes = (p.head_lanes + 1) / 2;
+  p.tokens_per_block = kRotaryThreads / (p.items * p.head_lanes);
+  const long long blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+  GS_REQUIRE(blocks < (1ll << 31), "too many tokens");
+  if (dtype == GS_FP32)
+    launch_rotary<float>(p, vec, position_type, (unsigned)blocks, (cudaStream_t)stream);
+  else if (dtype == GS_FP16)
+    launch_rotary<__half>(p, vec, position_type, (unsigned)blocks, (cudaStream_t)stream);
+  else
+    launch_rotary<__nv_bfloat16>(p, vec, position_type, (unsigned)blocks, (cudaStream_t)stream);
+  GS_CHECK_LAUNCH();
+  return GS_OK;
+  GS_API_END();
+}

@@ -1,0 +1,221 @@
+// Fifth-generation tensor-core matrix products (tcgen05) with accumulators in tensor memory, and
+// the copies and barriers that feed them.
+//
+// Conventions of the callers: operand tiles lie in shared memory as the 128-byte-swizzled boxes
+// that the copy engine writes, rows of 64 16-bit numbers (128 bytes), 8 rows to a 1,024-byte
+// group, tiles starting on 1,024-byte boundaries. A tile read along its rows (contraction over
+// the 64 numbers) is "K-major"; the same tile read across (contraction over the rows) is
+// "MN-major". Wider rows are several such boxes one after another. Accumulator row r is lane r
+// of tensor memory, column j of the product its column j.
+#pragma once
+
+#include "tma.cuh"
+#include "token_types.cuh"
+
+namespace gs {
+
+// Limit of a wait inside the attention kernels; a wait that runs out ends the kernel with
+// kErrMmaTimeout.
+constexpr unsigned long long kTcWaitNs = 2000000000ull;
+
+// Waits for phase `parity` of the barrier; false if the limit ran out. The clock is read once in
+// 64 polls, each of which may suspend the thread for a time that the hardware sets.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, unsigned parity) {
+  const unsigned addr = smem_u32(bar);
+  unsigned long long t0 = 0;
+  for (unsigned k = 0; k < (1u << 28); ++k) {
+    unsigned done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (k % 64 == 63) {
+      const unsigned long long t = tma_global_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kTcWaitNs) return false;
+    }
+  }
+  return false;
+}
+
+// The same for a whole warp: false for every lane where it is for one.
+__device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, unsigned parity) {
+  return __all_sync(~0u, tc_wait(bar, parity));
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Box at (x, y, z, w), innermost first, into swizzled shared memory, completing on `bar`.
+__device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap* map, int x, int y,
+                                            int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_alloc(unsigned* slot, unsigned columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   smem_u32(slot)),
+               "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tc_free(unsigned base, unsigned columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// Shared-memory writes of this thread become visible to the copy and matrix engines.
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Arrives on `bar` when every matrix product issued by this thread so far has completed.
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+
+// D[tmem] (+)= A[shared] B[shared]^T, one step of 16 along the contraction.
+__device__ __forceinline__ void tc_mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc,
+                                          unsigned accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in tensor memory: 8 columns of two 16-bit numbers each.
+__device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, uint64_t b, unsigned idesc,
+                                          unsigned accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: 32-bit accumulators, A and B both half (0) or both bfloat16 (1), M = 128
+// rows, N columns (a multiple of 16), B K-major or MN-major, A K-major.
+template <typename T>
+struct TcFormat;
+template <>
+struct TcFormat<__half> {
+  static constexpr unsigned kId = 0;
+};
+template <>
+struct TcFormat<__nv_bfloat16> {
+  static constexpr unsigned kId = 1;
+};
+template <typename T>
+__device__ __forceinline__ unsigned tc_idesc(unsigned n, bool b_mn_major) {
+  return (1u << 4) | (TcFormat<T>::kId << 7) | (TcFormat<T>::kId << 10) |
+         ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// Shared-memory operand descriptor of a 128-byte-swizzled tile. `group_bytes`: distance of
+// neighbouring 64-number boxes (MN-major operands wider than 64 only).
+__device__ __forceinline__ uint64_t tc_desc(unsigned addr, unsigned group_bytes) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(group_bytes >> 4) << 16) |
+         ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+#define GS_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), \
+                    "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define GS_I8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), \
+                    "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+
+// 32 consecutive columns of the thread's lane (asynchronous: tc_wait_ld before use).
+__device__ __forceinline__ void tc_ld32(unsigned addr, unsigned* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19,"
+      " %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : GS_R8(r, 0), GS_R8(r, 8), GS_R8(r, 16), GS_R8(r, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_ld16(unsigned addr, unsigned* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : GS_R8(r, 0), GS_R8(r, 8)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st16(unsigned addr, const unsigned* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::GS_I8(r, 0),
+      GS_I8(r, 8), "r"(addr)
+      : "memory");
+}
+
+// Two floats rounded to two 16-bit numbers, `lo` in the low half.
+template <typename T>
+__device__ __forceinline__ unsigned pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ unsigned pack2<__half>(float lo, float hi) {
+  unsigned r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <>
+__device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float lo, float hi) {
+  unsigned r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// 2^x by the special-function unit: relative error below 2^-22, 0 for -inf, results below 2^-126
+// are flushed to 0.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Host: describes a [B, L, H, D] tensor of 16-bit numbers as (D, L, H, B), innermost first, copied
+// in boxes of 64 numbers x `rows` tokens of one head, 128-byte-swizzled; what lies past D or L
+// reads as zero. Axes of one element, and a batch stride of 0 (all items alike), are encoded as
+// one element: the caller passes coordinate 0 there.
+inline bool encode_tokens(CUtensorMap* map, int dtype, const void* base, int D, int L, int H,
+                          int B, long long stride_l, long long stride_h, long long stride_b,
+                          unsigned rows) {
+  const EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const auto one = [](long long n, long long stride) { return n <= 1 || stride == 0; };
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)(one(L, stride_l) ? 1 : L),
+                              (cuuint64_t)(one(H, stride_h) ? 1 : H),
+                              (cuuint64_t)(one(B, stride_b) ? 1 : B)};
+  const cuuint64_t row = (cuuint64_t)(D * 2 + 15) / 16 * 16;
+  const cuuint64_t strides[3] = {one(L, stride_l) ? row : (cuuint64_t)stride_l * 2,
+                                 one(H, stride_h) ? row : (cuuint64_t)stride_h * 2,
+                                 one(B, stride_b) ? row : (cuuint64_t)stride_b * 2};
+  const cuuint32_t box[4] = {64, rows, 1, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  return fn(map,
+            dtype == GS_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            4, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace gs

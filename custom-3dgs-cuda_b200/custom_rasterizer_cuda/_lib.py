@@ -66,6 +66,17 @@ SIGNATURES = {
                             c_int, c_int, P, c_size_t, P, P, P]),
     "gs_adc_apply": (c_int, [c_int, P, c_size_t, P, P, P, P, P, c_int, P, P, P, P]),
     "gs_densify_stats": (c_int, [c_int, P, c_int, c_float, c_float, P, P, P, P]),
+    "gs_rotary_axes": (c_int, [c_int, c_int, c_int, c_int, c_int, P, P, P, c_int, c_longlong,
+                               c_longlong, c_int, P, P, c_int, c_int, P]),
+    "gs_rms_norm_forward": (c_int, [c_int, c_longlong, c_int, P, P, P, c_float, P, P, P, P]),
+    "gs_rms_norm_e4m3": (c_int, [c_int, c_longlong, c_int, c_int, P, P, P, c_float, P, P, P, P]),
+    "gs_rms_norm_backward_workspace_size": (c_size_t, [c_longlong, c_int]),
+    "gs_rms_norm_backward": (c_int, [c_int, c_longlong, c_int, P, P, P, P, P, P, P, P, c_size_t,
+                                     P]),
+    "gs_cross_attention_workspace_size": (c_size_t, [P]),
+    "gs_cross_attention_forward": (c_int, [P, P, c_size_t, P]),
+    "gs_cross_attention_backward_workspace_size": (c_size_t, [P]),
+    "gs_cross_attention_backward": (c_int, [P, P, P, P, P, P, c_size_t, P]),
     "gs_event_create": (c_int, [POINTER(c_void_p)]),
     "gs_event_synchronize": (c_int, [P]),
     "gs_event_destroy": (c_int, [P]),
@@ -89,6 +100,31 @@ class ViewSums(ctypes.Structure):
                 ("t", c_void_p), ("cam_pos", c_void_p),
                 ("fx", c_float), ("fy", c_float), ("cx", c_float), ("cy", c_float),
                 ("stat_scale_x", c_float), ("stat_scale_y", c_float)]
+
+
+# element types of the token operators (GS_FP32, GS_FP16, GS_BF16, GS_INT32)
+GS_FP32 = 0
+GS_FP16 = 1
+GS_BF16 = 2
+GS_INT32 = 3
+
+
+class TokenView(ctypes.Structure):
+    """Mirror of gs_token_view: a [batch, token, head, D] tensor, strides in elements."""
+
+    _fields_ = [("data", c_void_p), ("batch_stride", c_longlong), ("token_stride", c_longlong),
+                ("head_stride", c_longlong)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """Mirror of gs_attention_args."""
+
+    _fields_ = [("dtype", c_int), ("B", c_int), ("Lq", c_int), ("Lk", c_int), ("Hq", c_int),
+                ("Hkv", c_int), ("D", c_int), ("scale", c_float), ("q", TokenView),
+                ("k", TokenView), ("v", TokenView), ("out", TokenView), ("lengths", c_void_p),
+                ("mask", c_void_p), ("mask_batch_stride", c_longlong),
+                ("mask_head_stride", c_longlong), ("mask_query_stride", c_longlong),
+                ("lse", c_void_p)]
 
 
 def load(path: Path = LIB_PATH) -> ctypes.CDLL:

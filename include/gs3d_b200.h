@@ -369,6 +369,97 @@ GS_API int gs_densify_stats(int N, const float* mean2d_grad, int grad_stride, fl
                             void* stream);
 
 /*
+ * Token operators: what a decoder that predicts Gaussians from images needs between its matrix
+ * products (no counterpart in the reference). Tensors of float32, half or bfloat16; sums,
+ * statistics and products in 32 bits, one rounding when a result is written.
+ */
+#define GS_FP32 0
+#define GS_FP16 1
+#define GS_BF16 2
+#define GS_INT32 3 /* positions only */
+
+/* A [batch, token, head, D] tensor: strides in elements, the D numbers of a head contiguous. */
+typedef struct gs_token_view {
+  void* data;
+  long long batch_stride, token_stride, head_stride;
+} gs_token_view;
+
+/*
+ * Rotary positions with up to 4 axes (view, row, column, ...): axis a owns axis_dims[a]
+ * consecutive numbers of every head (even; together at most D, the rest is copied), and pair
+ * j < axis_dims[a] / 2 of them is turned by positions[b, l, a] * bases[a]^(-2 j / axis_dims[a]):
+ * (u, v) -> (u cos - v sin, u sin + v cos), with (u, v) the numbers (j, j + axis_dims[a] / 2) of
+ * the block, or (2 j, 2 j + 1) when `interleaved`. `inverse` turns the other way: the gradient.
+ * x and y: [B, L, H, D] of `dtype`, D even and at most 256; y may be x itself, else they must not
+ * overlap. positions: float32 or int32 (exact up to 2^24), the n_axes coordinates of a token
+ * contiguous; a batch stride of 0 gives every batch item the same positions. axis_dims and bases
+ * are host arrays.
+ */
+GS_API int gs_rotary_axes(int dtype, int B, int L, int H, int D, const gs_token_view* x,
+                          const gs_token_view* y, const void* positions, int position_type,
+                          long long position_batch_stride, long long position_token_stride,
+                          int n_axes, const int* axis_dims, const double* bases, int interleaved,
+                          int inverse, void* stream);
+
+/*
+ * Root-mean-square norm of contiguous [rows, width] tensors (width at most 32768):
+ * h = x + residual (x where residual is NULL), y = h * rstd * weight with
+ * rstd = 1 / sqrt(mean(h^2) + eps). y, and h where it is given (only with a residual), have
+ * x's type; rstd[rows] may be NULL.
+ * gs_rms_norm_e4m3 writes y as 8-bit e4m3 numbers q with scales, y ~ q * scale and
+ * scale = max|y| / 448: one for each row (group 0, scales[rows]) or for each 128 numbers of it
+ * (group 128, scales[rows, width / 128], buffers on 16-byte boundaries). A row or group of zeros
+ * has scale 0.
+ * gs_rms_norm_backward: dx (the gradient of x and of the residual alike) and dw of type dtype,
+ * from dy, dh (the gradient of h as an output, or NULL), the forward's h (x without a residual)
+ * and its rstd. The same bits on every run.
+ */
+GS_API int gs_rms_norm_forward(int dtype, long long rows, int width, const void* x,
+                               const void* residual, const void* weight, float eps, void* y,
+                               void* h, float* rstd, void* stream);
+GS_API int gs_rms_norm_e4m3(int dtype, long long rows, int width, int group, const void* x,
+                            const void* residual, const void* weight, float eps, void* q,
+                            float* scales, void* h, void* stream);
+GS_API size_t gs_rms_norm_backward_workspace_size(long long rows, int width);
+GS_API int gs_rms_norm_backward(int dtype, long long rows, int width, const void* dy,
+                                const void* dh, const void* h, const void* weight,
+                                const float* rstd, void* dx, void* dw, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/*
+ * Cross attention of queries to an encoder's states of another length:
+ * out = softmax(scale q k^T) v for each query head, Hq / Hkv query heads sharing a key head.
+ * q, out: [B, Lq, Hq, D]; k, v: [B, Lk, Hkv, D], half or bfloat16, D a multiple of 8 up to 128;
+ * every view starts on a 16-byte boundary with strides of multiples of 8 elements.
+ * lengths[B] (device, or NULL): the keys of each batch item, held to [0, Lk]; what lies past them
+ * is not looked at. mask (device bytes, or NULL): 0 leaves a key out for a query; strides for
+ * batch item, head and query (0 where they share), keys contiguous. What k and v hold at a key
+ * that all queries of a batch item leave out (head and query stride 0) never reaches a result,
+ * NaN included; under a mask that differs between queries, v must be finite.
+ * A query that keeps no key has out = 0, lse = -inf and no gradient.
+ * lse[B, Hq, Lq] (or NULL; the backward needs it): log sum exp of the scaled scores.
+ * gs_cross_attention_backward: gradients in the layouts of q, k and v, from the same arguments,
+ * the forward's out and lse. Sums run in a fixed order: the same bits on every run.
+ */
+typedef struct gs_attention_args {
+  int dtype, B, Lq, Lk, Hq, Hkv, D;
+  float scale;
+  gs_token_view q, k, v, out;
+  const int* lengths;
+  const unsigned char* mask;
+  long long mask_batch_stride, mask_head_stride, mask_query_stride;
+  float* lse;
+} gs_attention_args;
+GS_API size_t gs_cross_attention_workspace_size(const gs_attention_args* args);
+GS_API int gs_cross_attention_forward(const gs_attention_args* args, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+GS_API size_t gs_cross_attention_backward_workspace_size(const gs_attention_args* args);
+GS_API int gs_cross_attention_backward(const gs_attention_args* args, const gs_token_view* dout,
+                                       const gs_token_view* dq, const gs_token_view* dk,
+                                       const gs_token_view* dv, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/*
  * CUDA event helpers for m_ready_event (cudaEvent_t values passed as void*): create an event
  * with timing disabled, block the calling thread until it completes, destroy it.
  */
@@ -398,7 +489,8 @@ GS_API unsigned long long gs_kernel_launches(void);
  * Device-side error bits recorded by the kernels of earlier calls on this device since
  * the last gs_clear_device_errors() (1 = a look-back wait gave up, 2 = pair capacity
  * exceeded, 4 = an index out of range, 8 = a cross-GPU barrier wait of gs_sharded_adam_step
- * gave up, 16 = a wait for a tile copy of the tensor memory accelerator gave up).
+ * gave up, 16 = a wait for a tile copy of the tensor memory accelerator gave up, 32 = a wait
+ * inside an attention kernel gave up).
  * Synchronises the device.
  */
 GS_API int gs_device_error_bits(unsigned* bits);
