@@ -159,7 +159,7 @@ using namespace gs;
 
 extern "C" size_t gs_cross_attention_workspace_size(const gs_attention_args* a) {
   if (!a || *attention_fault(*a) || a->B == 0 || a->Hq == 0 || a->Lq == 0) return 0;
-  return attention_forward_workspace(*a);
+  return attention_is_single(*a) ? attention_single_workspace(*a) : attention_forward_workspace(*a);
 }
 
 extern "C" int gs_cross_attention_forward(const gs_attention_args* a, void* workspace,
@@ -176,7 +176,8 @@ extern "C" int gs_cross_attention_forward(const gs_attention_args* a, void* work
   }
   GS_REQUIRE(workspace_bytes >= gs_cross_attention_workspace_size(a), "workspace too small");
   GS_REQUIRE(workspace || !gs_cross_attention_workspace_size(a), "null pointer");
-  return attention_forward(*a, workspace, (cudaStream_t)stream);
+  return attention_is_single(*a) ? attention_single(*a, workspace, (cudaStream_t)stream)
+                                 : attention_forward(*a, workspace, (cudaStream_t)stream);
   GS_API_END();
 }
 

@@ -69,5 +69,11 @@ constexpr long long kSms = 148;  // streaming multiprocessors of a B200
 AttentionParams attention_params(const gs_attention_args& a);
 size_t attention_forward_workspace(const gs_attention_args& a);
 int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t stream);
+cudaError_t attention_combine(const gs_attention_args& args, int splits, const float* out,
+                              const float* lse, cudaStream_t stream);
+// Few rows for each key head: the kernel that reads k and v straight into registers.
+bool attention_is_single(const gs_attention_args& a);
+size_t attention_single_workspace(const gs_attention_args& a);
+int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t stream);
 
 }  // namespace gs
