@@ -27,8 +27,7 @@ struct AttentionParams {
   const int* lengths;         // [B] or null
   const unsigned char* mask;  // keys contiguous; 0 leaves a key out; or null
   long long mask_b, mask_h, mask_q;
-  float* lse;    // [B, Hq, Lq]
-  float* delta;  // [B, Hq, Lq]
+  float* lse;  // [B, Hq, Lq] or null
 };
 
 // Keys of batch item b: its length, held to [0, Lk].
@@ -36,8 +35,26 @@ __device__ __forceinline__ int key_count(const AttentionParams& p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.Lk) : p.Lk;
 }
 
-__device__ __forceinline__ bool keeps(const AttentionParams& p, int b, int h, int i, int j) {
-  return !p.mask || p.mask[b * p.mask_b + h * p.mask_h + i * p.mask_q + j];
+// Sets s = -inf at the keys that a query leaves out: past `n`, or 0 in its row of the mask (or
+// null). `j0`: the first of the N keys in s.
+template <int N>
+__device__ __forceinline__ void hide(int packs, const unsigned char* row, int j0, int n,
+                                     unsigned* s) {
+  constexpr unsigned kMinusInf = 0xff800000u;
+  if (j0 + N <= n && packs && row) {
+#pragma unroll
+    for (int c = 0; c < N; c += 16) {
+      const uint4 m = *reinterpret_cast<const uint4*>(row + j0 + c);
+      const unsigned w[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (!((w[k / 4] >> (8 * (k % 4))) & 0xffu)) s[c + k] = kMinusInf;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (j0 + k >= n || (row && !row[j0 + k])) s[k] = kMinusInf;
 }
 
 // Zeroes, in a swizzled tile of `rows` keys (BOXES boxes of 128 bytes a row) at shared address
@@ -66,6 +83,7 @@ __device__ __forceinline__ void clear_rows(unsigned tile, int rows, int left,
 
 constexpr long long kSms = 148;  // streaming multiprocessors of a B200
 
+int attention_mask_packs(const gs_attention_args& a);
 AttentionParams attention_params(const gs_attention_args& a);
 size_t attention_forward_workspace(const gs_attention_args& a);
 int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t stream);
@@ -75,5 +93,10 @@ cudaError_t attention_combine(const gs_attention_args& args, int splits, const f
 bool attention_is_single(const gs_attention_args& a);
 size_t attention_single_workspace(const gs_attention_args& a);
 int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t stream);
+
+size_t attention_backward_workspace(const gs_attention_args& a);
+int attention_backward(const gs_attention_args& a, const gs_token_view& dout,
+                       const gs_token_view& dq, const gs_token_view& dk, const gs_token_view& dv,
+                       void* workspace, cudaStream_t stream);
 
 }  // namespace gs

@@ -1,0 +1,532 @@
+// Cross attention backward on the tensor cores.
+//
+//   P = exp(scale q k^T - lse),  dP = dO v^T,  dS = P o (dP - delta),  delta = rowsum(dO o O),
+//   dv = P^T dO,  dk = scale dS^T q,  dq = scale dS k.
+// Three kernels, none of which adds to memory that another CTA adds to, so that the sums have a
+// fixed order: delta and lse of every row (prepare_kernel), then one kernel that owns tiles of
+// 128 keys and walks over the queries of every head that shares them (dk, dv), and one that owns
+// tiles of 128 queries and walks over the keys (dq). Both recompute S and dP: 7 products for
+// each pair of tiles instead of the 5 that one kernel with shared sums would need.
+//
+// Both are the same kernel, with KEYS telling which side is owned. The owned ("outer") tiles stay
+// in shared memory, the others ("inner", 64 rows) stream through. S and dP, outer rows x inner
+// rows, are products into tensor memory; a thread for each outer row turns them into P and dS in
+// 16 bits, in place; those are the next products' left operands, read from tensor memory, with
+// the same inner tiles read across as right operands. S and dP exist twice: two warpgroups take
+// inner tiles in turn, one works on a tile while the other's products run.
+//
+// P and dS are rounded to the products' 16-bit type, a relative error for bfloat16 down to 2^-126,
+// where the exponential's results and the products' operands end. Both are formed 2^32 times
+// larger and the sums scaled back, so that probabilities down to 2^-158 still count. Half has few
+// exponents: P is formed 2^15 times larger there, and dS as it is, since it has no bound: half's
+// gradients lose bits where dS is below 2^-14 unless the loss is scaled.
+#include <algorithm>
+#include <cmath>
+
+#include "attention.cuh"
+#include "capi_internal.h"
+#include "tensor_core.cuh"
+
+namespace gs {
+
+constexpr int kOuter = 128, kInner = 64;
+constexpr int kBwdThreads = 320;
+
+struct BackwardParams {
+  AttentionParams a;
+  float scale_log2;
+  const float2* stats;  // [B, Hq, lq_pad]: lse log2 e - kLog2 (+inf: no probability), delta
+  int lq_pad;           // Lq rounded up to kInner
+  int splits;           // of the inner tiles
+  int x1b, x1h, x2b, x2h, y1b, y1h, y2b, y2h;  // 0 where items or heads share the tensor, else 1
+  float* part1;  // [splits, outer rows, D] where splits > 1: dq or dk
+  float* part2;  // dv
+  int mask_packs;
+};
+
+template <int DP>
+struct BackwardShared {
+  static constexpr int kBoxes = DP / 64;
+  static constexpr int kOuterBytes = kBoxes * kOuter * 128;
+  static constexpr int kInnerBytes = kBoxes * kInner * 128;
+  static constexpr int kStages = DP == 128 ? 4 : 6;
+  static constexpr int kBytes =
+      1024 + 2 * kOuterBytes + kStages * (2 * kInnerBytes + kInner * 8);
+};
+
+// P is formed 2^kLog2 times larger; kDs brings dS back where its type cannot hold that, kAcc1 and
+// kAcc2 the accumulators of dS and P.
+template <typename T>
+struct ProbabilityScale {
+  static constexpr float kLog2 = 32.0f, kDs = 1.0f;
+  static constexpr float kAcc1 = 1.0f / 4294967296.0f, kAcc2 = kAcc1;
+};
+template <>
+struct ProbabilityScale<__half> {
+  static constexpr float kLog2 = 15.0f, kDs = 1.0f / 32768.0f;
+  static constexpr float kAcc1 = 1.0f, kAcc2 = kDs;
+};
+
+// delta and lse in powers of two of every query row, 8 lanes a row; the rows, padded to a multiple
+// of 64 for each head, fill the grid exactly.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams a, int lq_pad,
+                                                                float2* stats) {
+  const int sub = threadIdx.x % 8;
+  const long long at = (long long)blockIdx.x * 32 + threadIdx.x / 8;
+  const int i = (int)(at % lq_pad), h = (int)(at / lq_pad % a.Hq), b = (int)(at / lq_pad / a.Hq);
+  float delta = 0.0f, lse = INFINITY;
+  if (i < a.Lq) {
+    const T* o = a.out.at<T>(b, i, h);
+    const T* g = a.dout.at<T>(b, i, h);
+    for (int d = sub * 8; d < a.D; d += 64) {
+      float x[8], y[8];
+      load_pack<T, 8>(o + d, x);
+      load_pack<T, 8>(g + d, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) delta = fmaf(x[k], y[k], delta);
+    }
+    lse = a.lse[((long long)b * a.Hq + h) * a.Lq + i];
+    lse = lse == -INFINITY ? INFINITY
+                           : fmaf(lse, 1.4426950408889634f, -ProbabilityScale<T>::kLog2);
+  }
+#pragma unroll
+  for (int w = 4; w; w >>= 1) delta += __shfl_xor_sync(~0u, delta, w);
+  if (sub == 0) stats[at] = make_float2(lse, delta);
+}
+
+__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    attention_backward_kernel(const __grid_constant__ BackwardParams p,
+                              const __grid_constant__ CUtensorMap map_x1,
+                              const __grid_constant__ CUtensorMap map_x2,
+                              const __grid_constant__ CUtensorMap map_y1,
+                              const __grid_constant__ CUtensorMap map_y2) {
+  using S = BackwardShared<DP>;
+  using PS = ProbabilityScale<T>;
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t x_full, y_full[S::kStages], y_free[S::kStages], sp_full[2], ready[2], acc_full;
+  __shared__ unsigned tmem_slot;
+  __shared__ volatile int gave_up;
+  const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
+  const unsigned sm_x1 = base, sm_x2 = sm_x1 + S::kOuterBytes, sm_y = sm_x2 + S::kOuterBytes,
+                 sm_stats = sm_y + S::kStages * 2 * S::kInnerBytes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const AttentionParams& a = p.a;
+  const int shared_heads = a.Hq / a.Hkv;
+  const int outer_rows = KEYS ? a.Lk : a.Lq, outer_heads = KEYS ? a.Hkv : a.Hq;
+  const int outer_tiles = (outer_rows + kOuter - 1) / kOuter;
+  const int x0 = blockIdx.x % outer_tiles * kOuter, bh = blockIdx.x / outer_tiles;
+  const int b = bh / outer_heads, ho = bh % outer_heads;
+  const int n = key_count(a, b);
+  const int q_tiles = p.lq_pad / kInner;
+  const int tiles = KEYS ? (x0 < n ? q_tiles * shared_heads : 0) : (n + kInner - 1) / kInner;
+  const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
+  const int count = (int)((long long)tiles * (blockIdx.y + 1) / p.splits) - t0;
+  const bool key_mask = a.mask && a.mask_h == 0 && a.mask_q == 0;
+
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    mbar_init(&x_full, 1);
+    mbar_init(&acc_full, 1);
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&y_full[i], 1);
+      mbar_init(&y_free[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sp_full[i], 1);
+      mbar_init(&ready[i], 128);
+    }
+  }
+  if (warp == 8) tc_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = tmem_slot;
+  const unsigned tm_s = tmem, tm_dp = tmem + 128, tm_acc1 = tmem + 256, tm_acc2 = tmem + 384;
+
+  if (warp == 9) {
+    // ---- copies ----
+    if (lane == 0 && count > 0) {
+      mbar_arrive_expect_tx(&x_full, 2 * S::kOuterBytes);
+      for (int x = 0; x < S::kBoxes; ++x) {
+        tma_load_4d(sm_x1 + x * kOuter * 128, &map_x1, x * 64, x0, ho * p.x1h, b * p.x1b, &x_full);
+        tma_load_4d(sm_x2 + x * kOuter * 128, &map_x2, x * 64, x0, ho * p.x2h, b * p.x2b, &x_full);
+      }
+      for (int j = 0; j < count; ++j) {
+        const int st = j % S::kStages;
+        if (!tc_wait(&y_free[st], (j / S::kStages & 1) ^ 1)) { gave_up = 1; break; }
+        const int t = t0 + j;
+        const int head = KEYS ? ho * shared_heads + t / q_tiles : ho / shared_heads;
+        const int row = (KEYS ? t % q_tiles : t) * kInner;
+        const unsigned dst = sm_y + st * 2 * S::kInnerBytes;
+        mbar_arrive_expect_tx(&y_full[st], 2 * S::kInnerBytes + (KEYS ? kInner * 8 : 0));
+        for (int x = 0; x < S::kBoxes; ++x) {
+          tma_load_4d(dst + x * kInner * 128, &map_y1, x * 64, row, head * p.y1h, b * p.y1b,
+                      &y_full[st]);
+          tma_load_4d(dst + S::kInnerBytes + x * kInner * 128, &map_y2, x * 64, row, head * p.y2h,
+                      b * p.y2b, &y_full[st]);
+        }
+        if (KEYS)
+          bulk_load(sm_stats + st * kInner * 8,
+                    p.stats + ((long long)b * a.Hq + head) * p.lq_pad + row, kInner * 8,
+                    &y_full[st]);
+      }
+    }
+  } else if (warp == 8) {
+    // ---- products ----
+    const int steps = (a.D + 15) / 16;
+    const unsigned idesc_s = tc_idesc<T>(kInner, false);
+    const unsigned idesc_acc = tc_idesc<T>(steps * 16, true);
+    bool ok = count > 0 && tc_wait_warp(&x_full, 0);
+    const auto scores = [&](int j) {  // S and dP of inner tile j
+      const int st = j % S::kStages, buf = j & 1;
+      if (!tc_wait_warp(&y_full[st], j / S::kStages & 1)) return false;
+      const unsigned y1 = sm_y + st * 2 * S::kInnerBytes, y2 = y1 + S::kInnerBytes;
+      if (!KEYS) {
+        // keys that all queries leave out: what they hold must not reach dq, where 0 times NaN
+        // would be added
+        const int key = (t0 + j) * kInner;
+        if (n - key < kInner || key_mask)
+          clear_rows<S::kBoxes>(y1, kInner, n - key,
+                                key_mask ? a.mask + b * a.mask_b + key : nullptr);
+      }
+      if (lane == 0) {
+        for (int k = 0; k < steps; ++k) {
+          const unsigned ox = (k / 4) * kOuter * 128 + (k % 4) * 32,
+                         oy = (k / 4) * kInner * 128 + (k % 4) * 32;
+          tc_mma_ss(tm_s + buf * 64, tc_desc(sm_x1 + ox, 16), tc_desc(y1 + oy, 16), idesc_s, k > 0);
+        }
+        for (int k = 0; k < steps; ++k) {
+          const unsigned ox = (k / 4) * kOuter * 128 + (k % 4) * 32,
+                         oy = (k / 4) * kInner * 128 + (k % 4) * 32;
+          tc_mma_ss(tm_dp + buf * 64, tc_desc(sm_x2 + ox, 16), tc_desc(y2 + oy, 16), idesc_s,
+                    k > 0);
+        }
+        tc_commit(&sp_full[buf]);
+      }
+      __syncwarp();
+      return true;
+    };
+    ok = ok && scores(0) && (count < 2 || scores(1));
+    for (int j = 0; ok && j < count; ++j) {
+      const int st = j % S::kStages, buf = j & 1;
+      ok = tc_wait_warp(&ready[buf], j / 2 & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        const unsigned y1 = sm_y + st * 2 * S::kInnerBytes, y2 = y1 + S::kInnerBytes;
+        if (KEYS)
+          for (int k = 0; k < kInner / 16; ++k)
+            tc_mma_ts(tm_acc2, tm_s + buf * 64 + k * 8, tc_desc(y2 + k * 2048, kInner * 128),
+                      idesc_acc, j > 0 || k > 0);
+        for (int k = 0; k < kInner / 16; ++k)
+          tc_mma_ts(tm_acc1, tm_dp + buf * 64 + k * 8, tc_desc(y1 + k * 2048, kInner * 128),
+                    idesc_acc, j > 0 || k > 0);
+        tc_commit(&y_free[st]);
+        if (j + 1 == count) tc_commit(&acc_full);
+      }
+      __syncwarp();
+      if (j + 2 < count) ok = scores(j + 2);
+    }
+    if (!ok && count > 0) gave_up = 1;
+  } else {
+    // ---- P and dS: one thread for each outer row ----
+    const int wg = warp / 4, row = threadIdx.x % 128, x = x0 + row;
+    const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
+    const float c = p.scale_log2;
+    float2 mine = make_float2(INFINITY, 0.0f);
+    const unsigned char* mask_row = nullptr;
+    bool dead = false;  // KEYS: a key that no query keeps
+    if (KEYS) {
+      dead = x >= n || (key_mask && !a.mask[b * a.mask_b + x]);
+    } else {
+      if (x < a.Lq) mine = p.stats[((long long)b * a.Hq + ho) * p.lq_pad + x];
+      if (a.mask)
+        mask_row = a.mask + b * a.mask_b + ho * a.mask_h + (long long)min(x, a.Lq - 1) * a.mask_q;
+    }
+    bool ok = true;
+    for (int j = wg; j < count; j += 2) {
+      const int st = j % S::kStages, t = t0 + j;
+      ok = tc_wait_warp(&sp_full[wg], j / 2 & 1);
+      if (!ok) break;
+      // the statistics came by the copy engine: their own barrier makes them visible
+      if (KEYS) ok = tc_wait_warp(&y_full[st], j / S::kStages & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const int y0 = (KEYS ? t % q_tiles : t) * kInner;
+      const bool hidden = KEYS ? (a.mask || x0 + kOuter > n) : (a.mask || y0 + kInner > n);
+#pragma unroll
+      for (int h = 0; h < kInner; h += 32) {
+        unsigned s[32], dp[32], pp[16], ds[16];
+        tc_ld32(tm_s + wg * 64 + lanes + h, s);
+        tc_ld32(tm_dp + wg * 64 + lanes + h, dp);
+        tc_wait_ld();
+        if (hidden) {
+          constexpr unsigned kMinusInf = 0xff800000u;
+          if (KEYS) {
+            const int head = ho * shared_heads + t / q_tiles;
+            const unsigned char* m =
+                a.mask && !key_mask ? a.mask + b * a.mask_b + head * a.mask_h + x : nullptr;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int i = min(y0 + h + k, a.Lq - 1);
+              if (dead || (m && !m[(long long)i * a.mask_q])) s[k] = kMinusInf;
+            }
+          } else {
+            hide<32>(p.mask_packs, mask_row, y0 + h, n, s);
+          }
+          // 0 times what the value product holds there, NaN included, is 0
+          const unsigned fill = __float_as_uint(0.0f);
+          const bool negative = c < 0.0f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (s[k] == kMinusInf) {
+              dp[k] = fill;
+              if (negative) s[k] = 0x7f800000u;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          float4 st2;  // lse and delta of inner rows h + k, h + k + 1
+          if (KEYS)
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(st2.x), "=f"(st2.y), "=f"(st2.z), "=f"(st2.w)
+                         : "r"(sm_stats + st * kInner * 8 + (h + k) * 8));
+          else
+            st2 = make_float4(mine.x, mine.y, mine.x, mine.y);
+          const float p0 = fast_exp2(fmaf(__uint_as_float(s[k]), c, -st2.x));
+          const float p1 = fast_exp2(fmaf(__uint_as_float(s[k + 1]), c, -st2.z));
+          const float d0 = p0 * ((__uint_as_float(dp[k]) - st2.y) * PS::kDs);
+          const float d1 = p1 * ((__uint_as_float(dp[k + 1]) - st2.w) * PS::kDs);
+          if (KEYS) pp[k / 2] = pack2<T>(p0, p1);
+          ds[k / 2] = pack2<T>(d0, d1);
+        }
+        if (KEYS) tc_st16(tm_s + wg * 64 + lanes + h / 2, pp);
+        tc_st16(tm_dp + wg * 64 + lanes + h / 2, ds);
+      }
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ready[wg]);
+    }
+    if (ok && count > 0) ok = tc_wait_warp(&acc_full, 0);
+    if (!ok) gave_up = 1;
+    tc_fence_after();
+    // KEYS: the first warpgroup writes dk, the second dv; else they take half of dq's columns each
+    const bool first = !KEYS || wg == 0;
+    const float factor = first ? a.scale * PS::kAcc1 : PS::kAcc2;
+    const TokenView& view = KEYS ? (first ? a.dk : a.dv) : a.dq;
+    const long long rows = (long long)a.B * outer_heads * outer_rows;
+    float* part = first ? p.part1 : p.part2;
+    for (int d = KEYS ? 0 : wg * (DP / 2); d < (KEYS ? DP : (wg + 1) * (DP / 2)); d += 16) {
+      if (d >= a.D) break;
+      unsigned o[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o[k] = 0u;
+      if (ok && count > 0) {
+        tc_ld16((first ? tm_acc1 : tm_acc2) + lanes + d, o);
+        tc_wait_ld();
+      }
+      if (x >= outer_rows) continue;
+      float f[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(o[k]) * factor;
+      if (p.splits == 1) {
+        T* out = view.at<T>(b, x, ho) + d;
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+          if (d + k >= a.D) break;
+          uint4 w;
+          w.x = pack2<T>(f[k], f[k + 1]), w.y = pack2<T>(f[k + 2], f[k + 3]);
+          w.z = pack2<T>(f[k + 4], f[k + 5]), w.w = pack2<T>(f[k + 6], f[k + 7]);
+          *reinterpret_cast<uint4*>(out + k) = w;
+        }
+      } else {
+        float* out = part + (blockIdx.y * rows + (long long)bh * outer_rows + x) * a.D + d;
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+          if (d + k >= a.D) break;
+          *reinterpret_cast<float4*>(out + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (gave_up) {
+    // A wait ran out. Copies still in flight end before the CTA's memory is given up.
+    if (threadIdx.x == 0) {
+      raise_device_error(kErrMmaTimeout);
+      const unsigned long long t = tma_global_ns();
+      for (int k = 0; k < (1 << 20) && tma_global_ns() - t < 10000000ull; ++k) __nanosleep(1000);
+    }
+    __syncthreads();
+  }
+  if (warp == 8) {
+    tc_fence_after();
+    tc_free(tmem, 512);
+  }
+}
+
+// out[b, row, h] = the sum of the splits' parts, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float* part, int splits,
+                                                        TokenView out, int rows_a_head, int heads,
+                                                        long long rows, int D) {
+  const int per_row = D / 4;
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= rows * per_row) return;
+  const long long row = at / per_row;
+  const int d = (int)(at % per_row) * 4;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int k = 0; k < splits; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(part + (k * rows + row) * D + d);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const int x = (int)(row % rows_a_head), bh = (int)(row / rows_a_head);
+  T* o = out.at<T>(bh / heads, x, bh % heads) + d;
+  *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+}
+
+struct BackwardPlan {
+  int key_splits = 1, query_splits = 1;
+  long long lq_pad = 0, key_floats = 0, query_floats = 0;
+  size_t bytes = 0;
+};
+
+// The inner tiles are split where the outer tiles leave SMs idle, each split with at least four.
+static BackwardPlan backward_plan(const gs_attention_args& a) {
+  BackwardPlan plan;
+  const auto tiles = [](long long rows, long long tile) { return (rows + tile - 1) / tile; };
+  const auto splits = [](long long ctas, long long inner) {
+    return (int)std::max(1ll, std::min(kSms / std::max(1ll, ctas), inner / 4));
+  };
+  plan.lq_pad = tiles(a.Lq, kInner) * kInner;
+  if (a.Hkv > 0)
+    plan.key_splits = splits(a.B * a.Hkv * tiles(a.Lk, kOuter),
+                             tiles(a.Lq, kInner) * (a.Hq / a.Hkv));
+  plan.query_splits = splits(a.B * a.Hq * tiles(a.Lq, kOuter), tiles(a.Lk, kInner));
+  if (plan.key_splits > 1)
+    plan.key_floats = (long long)plan.key_splits * a.B * a.Hkv * a.Lk * a.D;
+  if (plan.query_splits > 1)
+    plan.query_floats = (long long)plan.query_splits * a.B * a.Hq * a.Lq * a.D;
+  // dk, dv and dq in turn use the same parts
+  plan.bytes = (size_t)(a.B * a.Hq * plan.lq_pad) * sizeof(float2) +
+               (size_t)std::max(2 * plan.key_floats, plan.query_floats) * sizeof(float);
+  return plan;
+}
+
+size_t attention_backward_workspace(const gs_attention_args& a) { return backward_plan(a).bytes; }
+
+template <typename T, int DP, bool KEYS>
+static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&m)[4],
+                                   cudaStream_t stream) {
+  const auto kernel = attention_backward_kernel<T, DP, KEYS>;
+  const cudaError_t err = cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BackwardShared<DP>::kBytes);
+  if (err != cudaSuccess) return err;
+  const int rows = KEYS ? p.a.Lk : p.a.Lq, heads = KEYS ? p.a.Hkv : p.a.Hq;
+  const dim3 grid((rows + kOuter - 1) / kOuter * p.a.B * heads, p.splits);
+  kernel<<<grid, kBwdThreads, BackwardShared<DP>::kBytes, stream>>>(p, m[0], m[1], m[2], m[3]);
+  return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch_add(const float* part, int splits, const TokenView& out, int rows_a_head,
+                              int heads, int B, int D, cudaStream_t stream) {
+  const long long rows = (long long)B * heads * rows_a_head;
+  add_parts_kernel<T><<<(unsigned)((rows * (D / 4) + 255) / 256), 256, 0, stream>>>(
+      part, splits, out, rows_a_head, heads, rows, D);
+  return cudaGetLastError();
+}
+
+template <typename T>
+static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
+                        const gs_token_view& dq, const gs_token_view& dk, const gs_token_view& dv,
+                        void* workspace, cudaStream_t stream) {
+  const BackwardPlan plan = backward_plan(a);
+  BackwardParams p{};
+  p.a = attention_params(a);
+  p.a.dout = TokenView(dout), p.a.dq = TokenView(dq), p.a.dk = TokenView(dk),
+  p.a.dv = TokenView(dv);
+  // a scale of 0 weighs all keys alike; -inf, where a key is left out, has to stay what it is
+  p.scale_log2 = (a.scale == 0.0f ? 1e-30f : a.scale) * 1.4426950408889634f;
+  p.lq_pad = (int)plan.lq_pad;
+  float2* stats = static_cast<float2*>(workspace);
+  p.stats = stats;
+  const long long stat_rows = a.B * a.Hq * plan.lq_pad;
+  float* parts = reinterpret_cast<float*>(stats + stat_rows);
+  p.mask_packs = attention_mask_packs(a);
+  if (stat_rows) {
+    attention_prepare_kernel<T>
+        <<<(unsigned)(stat_rows / 32), 256, 0, stream>>>(p.a, p.lq_pad, stats);
+    GS_CHECK_LAUNCH();
+  }
+  const auto describe = [&](CUtensorMap* map, const gs_token_view& v, int L, int H, unsigned rows) {
+    return encode_tokens(map, a.dtype, v.data, a.D, L, H, a.B, v.token_stride, v.head_stride,
+                         v.batch_stride, rows);
+  };
+  const auto items = [&](const gs_token_view& v) { return a.B > 1 && v.batch_stride != 0; };
+  CUtensorMap m[4];
+  if (a.Lk > 0) {
+    GS_REQUIRE(describe(&m[0], a.k, a.Lk, a.Hkv, kOuter) &&
+                   describe(&m[1], a.v, a.Lk, a.Hkv, kOuter),
+               "the driver refused to describe a tensor");
+    m[2] = m[3] = m[0];  // without queries nothing is copied
+    if (stat_rows)
+      GS_REQUIRE(describe(&m[2], a.q, a.Lq, a.Hq, kInner) &&
+                     describe(&m[3], dout, a.Lq, a.Hq, kInner),
+                 "the driver refused to describe a tensor");
+    p.x1b = items(a.k), p.x2b = items(a.v), p.y1b = items(a.q), p.y2b = items(dout);
+    p.x1h = p.x2h = a.Hkv > 1, p.y1h = p.y2h = a.Hq > 1;
+    p.splits = plan.key_splits;
+    p.part1 = parts, p.part2 = parts + plan.key_floats;
+    GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, true>(p, m, stream))
+                      : (launch_backward<T, 128, true>(p, m, stream)));
+    count_launches(1u);
+    if (p.splits > 1) {
+      GS_CUDA(launch_add<T>(p.part1, p.splits, p.a.dk, a.Lk, a.Hkv, a.B, a.D, stream));
+      GS_CUDA(launch_add<T>(p.part2, p.splits, p.a.dv, a.Lk, a.Hkv, a.B, a.D, stream));
+      count_launches(2u);
+    }
+  }
+  if (!stat_rows) return GS_OK;
+  GS_REQUIRE(describe(&m[0], a.q, a.Lq, a.Hq, kOuter) && describe(&m[1], dout, a.Lq, a.Hq, kOuter),
+             "the driver refused to describe a tensor");
+  m[2] = m[3] = m[0];  // without keys nothing is copied
+  if (a.Lk > 0)
+    GS_REQUIRE(describe(&m[2], a.k, a.Lk, a.Hkv, kInner) &&
+                   describe(&m[3], a.v, a.Lk, a.Hkv, kInner),
+               "the driver refused to describe a tensor");
+  p.x1b = items(a.q), p.x2b = items(dout), p.y1b = items(a.k), p.y2b = items(a.v);
+  p.x1h = p.x2h = a.Hq > 1, p.y1h = p.y2h = a.Hkv > 1;
+  p.splits = plan.query_splits;
+  p.part1 = parts, p.part2 = nullptr;
+  GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, false>(p, m, stream))
+                    : (launch_backward<T, 128, false>(p, m, stream)));
+  count_launches(1u);
+  if (p.splits > 1) {
+    GS_CUDA(launch_add<T>(p.part1, p.splits, p.a.dq, a.Lq, a.Hq, a.B, a.D, stream));
+    count_launches(1u);
+  }
+  return GS_OK;
+}
+
+int attention_backward(const gs_attention_args& a, const gs_token_view& dout,
+                       const gs_token_view& dq, const gs_token_view& dk, const gs_token_view& dv,
+                       void* workspace, cudaStream_t stream) {
+  return a.dtype == GS_FP16
+             ? run_backward<__half>(a, dout, dq, dk, dv, workspace, stream)
+             : run_backward<__nv_bfloat16>(a, dout, dq, dk, dv, workspace, stream);
+}
+
+}  // namespace gs

@@ -49,28 +49,6 @@ struct ForwardShared {
   static constexpr int kBytes = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + 256;
 };
 
-// Sets s = -inf at the keys that row i of batch item b, head h leaves out: past `n`, or 0 in the
-// mask. `j0`: first key of the 32 in s.
-template <int N>
-__device__ __forceinline__ void hide(const AttentionParams& p, int packs, const unsigned char* row,
-                                     int j0, int n, unsigned* s) {
-  constexpr unsigned kMinusInf = 0xff800000u;
-  if (j0 + N <= n && packs && row) {
-#pragma unroll
-    for (int c = 0; c < N; c += 16) {
-      const uint4 m = *reinterpret_cast<const uint4*>(row + j0 + c);
-      const unsigned w[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (!((w[k / 4] >> (8 * (k % 4))) & 0xffu)) s[c + k] = kMinusInf;
-    }
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    if (j0 + k >= n || (row && !row[j0 + k])) s[k] = kMinusInf;
-}
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1)
     attention_forward_kernel(const __grid_constant__ ForwardParams p,
@@ -233,7 +211,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (mask_row || key + kTileK > n) {
 #pragma unroll
           for (int c = 0; c < kTileK; c += 32)
-            hide<32>(a, p.mask_packs, mask_row, key + c, n, s + c);
+            hide<32>(p.mask_packs, mask_row, key + c, n, s + c);
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -433,8 +411,7 @@ int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t 
   p.qb = a.B > 1 && a.q.batch_stride != 0, p.qh = a.Hq > 1;
   p.kb = a.B > 1 && a.k.batch_stride != 0, p.kh = a.Hkv > 1;
   p.vb = a.B > 1 && a.v.batch_stride != 0, p.vh = a.Hkv > 1;
-  p.mask_packs = a.mask && (reinterpret_cast<uintptr_t>(a.mask) | (uintptr_t)a.mask_batch_stride |
-                            (uintptr_t)a.mask_head_stride | (uintptr_t)a.mask_query_stride) % 16 == 0;
+  p.mask_packs = attention_mask_packs(a);
   CUtensorMap q, k, v;
   GS_REQUIRE(encode_tokens(&q, a.dtype, a.q.data, a.D, a.Lq, a.Hq, a.B, a.q.token_stride,
                            a.q.head_stride, a.q.batch_stride, kTileQ),
