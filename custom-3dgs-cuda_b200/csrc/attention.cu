@@ -45,12 +45,6 @@ AttentionParams attention_params(const gs_attention_args& a) {
   return p;
 }
 
-// Whether rows of the mask may be read 16 bytes at a time.
-int attention_mask_packs(const gs_attention_args& a) {
-  return a.mask && (reinterpret_cast<uintptr_t>(a.mask) | (uintptr_t)a.mask_batch_stride |
-                    (uintptr_t)a.mask_head_stride | (uintptr_t)a.mask_query_stride) % 16 == 0;
-}
-
 }  // namespace gs
 
 using namespace gs;

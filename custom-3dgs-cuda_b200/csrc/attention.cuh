@@ -27,6 +27,9 @@ struct AttentionParams {
   const int* lengths;         // [B] or null
   const unsigned char* mask;  // keys contiguous; 0 leaves a key out; or null
   long long mask_b, mask_h, mask_q;
+  // the mask as bits, rows of 4 words for each 128 keys; strides in words, 0 where shared; or null
+  const unsigned* bits;
+  long long bits_b, bits_h, bits_q;
   float* lse;  // [B, Hq, Lq] or null
 };
 
@@ -35,40 +38,32 @@ __device__ __forceinline__ int key_count(const AttentionParams& p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.Lk) : p.Lk;
 }
 
-// Sets s = -inf at the keys that a query leaves out: past `n`, or 0 in its row of the mask (or
-// null). `j0`: the first of the N keys in s.
-template <int N>
-__device__ __forceinline__ void hide(int packs, const unsigned char* row, int j0, int n,
-                                     unsigned* s) {
-  constexpr unsigned kMinusInf = 0xff800000u;
-  if (j0 + N <= n && packs && row) {
+// The bits of keys 32 w .. 32 w + 31 that lie below `left`.
+__device__ __forceinline__ unsigned below(int left, int w) {
+  const int k = left - 32 * w;
+  return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u;
+}
+
+constexpr unsigned kMinusInf = 0xff800000u;
+
+// Sets the scores s of 32 keys to -inf where their bit in `keep` is 0.
+__device__ __forceinline__ void hide32(unsigned keep, unsigned* s) {
 #pragma unroll
-    for (int c = 0; c < N; c += 16) {
-      const uint4 m = *reinterpret_cast<const uint4*>(row + j0 + c);
-      const unsigned w[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (!((w[k / 4] >> (8 * (k % 4))) & 0xffu)) s[c + k] = kMinusInf;
-    }
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    if (j0 + k >= n || (row && !row[j0 + k])) s[k] = kMinusInf;
+  for (int k = 0; k < 32; ++k)
+    if (!(keep >> k & 1u)) s[k] = kMinusInf;
 }
 
 // Zeroes, in a swizzled tile of `rows` keys (BOXES boxes of 128 bytes a row) at shared address
-// `tile`, the rows from `left` on and those whose byte in `mask` is 0 (or null): whole rows, so
+// `tile`, the rows from `left` on and those whose bit in `bits` is 0 (or null): whole rows, so
 // the swizzle inside them does not matter. One warp; the matrix engine sees it afterwards.
 template <int BOXES>
 __device__ __forceinline__ void clear_rows(unsigned tile, int rows, int left,
-                                           const unsigned char* mask) {
+                                           const unsigned* bits) {
   const int lane = threadIdx.x % 32;
-  for (int r0 = 0; r0 < rows; r0 += 32) {
-    const int r = r0 + lane;
-    unsigned out = __ballot_sync(~0u, r >= left || (mask && !mask[r]));
+  for (int w = 0; w < rows / 32; ++w) {
+    unsigned out = ~(below(left, w) & (bits ? bits[w] : ~0u));
     while (out) {
-      const int k = r0 + __ffs(out) - 1;
+      const int k = w * 32 + __ffs(out) - 1;
       out &= out - 1;
 #pragma unroll
       for (int x = 0; x < BOXES; ++x)
@@ -83,7 +78,10 @@ __device__ __forceinline__ void clear_rows(unsigned tile, int rows, int left,
 
 constexpr long long kSms = 148;  // streaming multiprocessors of a B200
 
-int attention_mask_packs(const gs_attention_args& a);
+// The mask's bits in `workspace` (16-byte aligned, attention_mask_bytes long).
+size_t attention_mask_bytes(const gs_attention_args& a);
+int attention_pack_mask(const gs_attention_args& a, AttentionParams& p, void* workspace,
+                        cudaStream_t stream);
 AttentionParams attention_params(const gs_attention_args& a);
 size_t attention_forward_workspace(const gs_attention_args& a);
 int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t stream);

@@ -41,7 +41,6 @@ struct BackwardParams {
   int x1b, x1h, x2b, x2h, y1b, y1h, y2b, y2h;  // 0 where items or heads share the tensor, else 1
   float* part1;  // [splits, outer rows, D] where splits > 1: dq or dk
   float* part2;  // dv
-  int mask_packs;
 };
 
 template <int DP>
@@ -132,7 +131,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int tiles = KEYS ? (x0 < n ? q_tiles * shared_heads : 0) : (n + kInner - 1) / kInner;
   const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
   const int count = (int)((long long)tiles * (blockIdx.y + 1) / p.splits) - t0;
-  const bool key_mask = a.mask && a.mask_h == 0 && a.mask_q == 0;
+  const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
 
   if (threadIdx.x == 0) {
     gave_up = 0;
@@ -198,7 +197,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int key = (t0 + j) * kInner;
         if (n - key < kInner || key_mask)
           clear_rows<S::kBoxes>(y1, kInner, n - key,
-                                key_mask ? a.mask + b * a.mask_b + key : nullptr);
+                                key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
       }
       if (lane == 0) {
         for (int k = 0; k < steps; ++k) {
@@ -245,14 +244,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
     const float c = p.scale_log2;
     float2 mine = make_float2(INFINITY, 0.0f);
-    const unsigned char* mask_row = nullptr;
-    bool dead = false;  // KEYS: a key that no query keeps
+    const unsigned* keep_row = nullptr;
+    // KEYS: the warp's 32 keys that are below the length, and that a key mask leaves
+    unsigned alive = 0;
     if (KEYS) {
-      dead = x >= n || (key_mask && !a.mask[b * a.mask_b + x]);
+      alive = below(n - x0, warp % 4);
+      if (key_mask) alive &= a.bits[b * a.bits_b + x0 / 32 + warp % 4];
     } else {
       if (x < a.Lq) mine = p.stats[((long long)b * a.Hq + ho) * p.lq_pad + x];
-      if (a.mask)
-        mask_row = a.mask + b * a.mask_b + ho * a.mask_h + (long long)min(x, a.Lq - 1) * a.mask_q;
+      if (a.bits)
+        keep_row = a.bits + b * a.bits_b + ho * a.bits_h + (long long)min(x, a.Lq - 1) * a.bits_q;
     }
     bool ok = true;
     for (int j = wg; j < count; j += 2) {
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const int y0 = (KEYS ? t % q_tiles : t) * kInner;
-      const bool hidden = KEYS ? (a.mask || x0 + kOuter > n) : (a.mask || y0 + kInner > n);
+      const bool hidden = a.bits || (KEYS ? x0 + kOuter > n : y0 + kInner > n);
 #pragma unroll
       for (int h = 0; h < kInner; h += 32) {
         unsigned s[32], dp[32], pp[16], ds[16];
@@ -272,28 +273,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_ld32(tm_dp + wg * 64 + lanes + h, dp);
         tc_wait_ld();
         if (hidden) {
-          constexpr unsigned kMinusInf = 0xff800000u;
+          unsigned keep;  // of the thread's 32 scores
           if (KEYS) {
-            const int head = ho * shared_heads + t / q_tiles;
-            const unsigned char* m =
-                a.mask && !key_mask ? a.mask + b * a.mask_b + head * a.mask_h + x : nullptr;
+            keep = alive >> lane & 1u ? ~0u : 0u;
+            if (a.bits && !key_mask) {
+              // lane k has the word of query y0 + h + k for the warp's 32 keys; each lane gathers
+              // its own key's bit of all 32
+              const int head = ho * shared_heads + t / q_tiles;
+              const unsigned word =
+                  a.bits[b * a.bits_b + head * a.bits_h +
+                         (long long)min(y0 + h + lane, a.Lq - 1) * a.bits_q + x0 / 32 + warp % 4];
+              unsigned mine = 0;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int i = min(y0 + h + k, a.Lq - 1);
-              if (dead || (m && !m[(long long)i * a.mask_q])) s[k] = kMinusInf;
+              for (int k = 0; k < 32; ++k)
+                mine |= (__shfl_sync(~0u, word, k) >> lane & 1u) << k;
+              keep &= mine;
             }
           } else {
-            hide<32>(p.mask_packs, mask_row, y0 + h, n, s);
+            keep = below(n - y0, h / 32);
+            if (keep_row) keep &= keep_row[(y0 + h) / 32];
           }
-          // 0 times what the value product holds there, NaN included, is 0
-          const unsigned fill = __float_as_uint(0.0f);
-          const bool negative = c < 0.0f;
+          // no probability, and 0 times what the value product holds there, NaN included, is 0
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            if (s[k] == kMinusInf) {
-              dp[k] = fill;
-              if (negative) s[k] = 0x7f800000u;
-            }
+            if (!(keep >> k & 1u)) s[k] = c < 0.0f ? 0x7f800000u : kMinusInf, dp[k] = 0u;
         }
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
@@ -425,7 +428,9 @@ static BackwardPlan backward_plan(const gs_attention_args& a) {
   return plan;
 }
 
-size_t attention_backward_workspace(const gs_attention_args& a) { return backward_plan(a).bytes; }
+size_t attention_backward_workspace(const gs_attention_args& a) {
+  return attention_mask_bytes(a) + backward_plan(a).bytes;
+}
 
 template <typename T, int DP, bool KEYS>
 static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&m)[4],
@@ -461,11 +466,12 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   // a scale of 0 weighs all keys alike; -inf, where a key is left out, has to stay what it is
   p.scale_log2 = (a.scale == 0.0f ? 1e-30f : a.scale) * 1.4426950408889634f;
   p.lq_pad = (int)plan.lq_pad;
-  float2* stats = static_cast<float2*>(workspace);
+  const size_t mask_bytes = attention_mask_bytes(a);
+  if (const int status = attention_pack_mask(a, p.a, workspace, stream)) return status;
+  float2* stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + mask_bytes);
   p.stats = stats;
   const long long stat_rows = a.B * a.Hq * plan.lq_pad;
   float* parts = reinterpret_cast<float*>(stats + stat_rows);
-  p.mask_packs = attention_mask_packs(a);
   if (stat_rows) {
     attention_prepare_kernel<T>
         <<<(unsigned)(stat_rows / 32), 256, 0, stream>>>(p.a, p.lq_pad, stats);

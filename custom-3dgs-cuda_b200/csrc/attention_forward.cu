@@ -38,7 +38,6 @@ struct ForwardParams {
   int kb, kh, vb, vh, qb, qh;  // 0 where all batch items (heads) share the tensor, else 1
   float* part_out;  // [splits, B, Hq, Lq, D] where splits > 1
   float* part_lse;  // [splits, B, Hq, Lq]
-  int mask_packs;   // mask rows may be read 16 bytes at a time
 };
 
 template <int DP>
@@ -129,7 +128,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const int steps = (a.D + 15) / 16;
     const unsigned idesc_s = tc_idesc<T>(kTileK, false);
     const unsigned idesc_o = tc_idesc<T>(steps * 16, true);
-    const bool key_mask = a.mask && a.mask_h == 0 && a.mask_q == 0;
+    const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
     const auto scores = [&](int t, int st) {  // S_t = q_t k^T
       for (int k = 0; k < steps; ++k) {
         const unsigned off = (k / 4) * 16384 + (k % 4) * 32;
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       const int key = (t0 + j) * kTileK;
       if (n - key < kTileK || key_mask)
         clear_rows<S::kBoxes>(sm_v + st * S::kTileBytes, kTileK, n - key,
-                              key_mask ? a.mask + b * a.mask_b + key : nullptr);
+                              key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
       if (j + 1 < count) ok = tc_wait_warp(&k_full[next], (j + 1) / S::kStages & 1);
       if (!ok) break;
       for (int t = 0; t < (two ? 2 : 1); ++t) {
@@ -190,13 +189,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     if (t == 0 || two) {
       const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
       const unsigned my_s = tm_s + t * 128 + lanes, my_o = tm_o + t * 128 + lanes;
-      const unsigned char* mask_row =
-          a.mask ? a.mask + b * a.mask_b + h * a.mask_h + (long long)min(i, a.Lq - 1) * a.mask_q
+      const uint4* keep_row =
+          a.bits ? reinterpret_cast<const uint4*>(a.bits + b * a.bits_b + h * a.bits_h +
+                                                  (long long)min(i, a.Lq - 1) * a.bits_q)
                  : nullptr;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
       for (int j = 0; j < count; ++j) {
         const int key = (t0 + j) * kTileK;
+        uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (keep_row) keep = keep_row[t0 + j];
         ok = tc_wait_warp(&s_full[t], j & 1);
         if (!ok) break;
         tc_fence_after();
@@ -208,10 +210,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
           for (int k = 0; k < kTileK; ++k) s[k] ^= 0x80000000u;
         }
-        if (mask_row || key + kTileK > n) {
-#pragma unroll
-          for (int c = 0; c < kTileK; c += 32)
-            hide<32>(p.mask_packs, mask_row, key + c, n, s + c);
+        if (keep_row || key + kTileK > n) {
+          hide32(keep.x & below(n - key, 0), s);
+          hide32(keep.y & below(n - key, 1), s + 32);
+          hide32(keep.z & below(n - key, 2), s + 64);
+          hide32(keep.w & below(n - key, 3), s + 96);
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -366,7 +369,8 @@ static int forward_splits(const gs_attention_args& a) {
 
 size_t attention_forward_workspace(const gs_attention_args& a) {
   const long long splits = forward_splits(a), rows = (long long)a.B * a.Hq * a.Lq;
-  return splits > 1 ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0;
+  return attention_mask_bytes(a) +
+         (splits > 1 ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0);
 }
 
 template <typename T, int DP>
@@ -405,13 +409,14 @@ int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t 
   p.lag = std::min(kLag / p.scale_log2, 1e30f);
   p.negate = a.scale < 0.0f;
   p.splits = forward_splits(a);
-  p.part_out = static_cast<float*>(workspace);
+  const size_t mask_bytes = attention_mask_bytes(a);
+  if (const int status = attention_pack_mask(a, p.a, workspace, stream)) return status;
+  p.part_out = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);
   const long long rows = (long long)a.B * a.Hq * a.Lq;
   p.part_lse = p.part_out + p.splits * rows * a.D;
   p.qb = a.B > 1 && a.q.batch_stride != 0, p.qh = a.Hq > 1;
   p.kb = a.B > 1 && a.k.batch_stride != 0, p.kh = a.Hkv > 1;
   p.vb = a.B > 1 && a.v.batch_stride != 0, p.vh = a.Hkv > 1;
-  p.mask_packs = attention_mask_packs(a);
   CUtensorMap q, k, v;
   GS_REQUIRE(encode_tokens(&q, a.dtype, a.q.data, a.D, a.Lq, a.Hq, a.B, a.q.token_stride,
                            a.q.head_stride, a.q.batch_stride, kTileQ),

@@ -65,73 +65,67 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
   if (token >= p.tokens) return;
   const long long b = token / p.L, l = token - b * p.L;
 
-  float c[VEC], s[VEC];
   const bool turned = pair < p.turned;
-  int axis = 0, off_u, off_v;
-  if (turned) {
+  int axis = 0;
 #pragma unroll
-    for (int a = 1; a < kRotaryMaxAxes; ++a)
-      if (a < p.n_axes && pair >= p.axis_start[a]) axis = a;
-    const P raw = reinterpret_cast<const P*>(p.pos)[b * p.pos_b + l * p.pos_l + axis];
-    const float x = p.sign * (float)raw;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float hi = s_hi[pair + i];
-      const float r = x * hi;
-      const float err = fmaf(x, hi, -r) + x * s_lo[pair + i];
-      sincospif(2.0f * ((r - rintf(r)) + err), &s[i], &c[i]);
-    }
-  }
+  for (int a = 1; a < kRotaryMaxAxes; ++a)
+    if (a < p.n_axes && pair >= p.axis_start[a]) axis = a;
   const int first = turned ? p.axis_start[axis] : p.turned;
   const int end = turned ? p.axis_start[axis + 1] : p.pairs;
-  if (INTERLEAVED) {
-    off_u = 2 * pair;
-    off_v = off_u + VEC;  // the second half of 2 VEC consecutive numbers
-  } else {
-    off_u = first + pair;  // block start 2 * first, then pair - first
-    off_v = off_u + (end - first);
-  }
+  // the block starts at 2 * first and its pair k is (k, k + half), or (2 k, 2 k + 1), whose second
+  // VEC numbers follow the first
+  const int off_u = INTERLEAVED ? 2 * pair : first + pair;
+  const int off_v = INTERLEAVED ? off_u + VEC : off_u + (end - first);
   const T* x = reinterpret_cast<const T*>(p.x) + b * p.xb + l * p.xl;
   T* y = reinterpret_cast<T*>(p.y) + b * p.yb + l * p.yl;
-  for (int h0 = lane_h; h0 < p.H; h0 += kHeadsInFlight * p.head_lanes) {
-    float u[kHeadsInFlight][VEC], v[kHeadsInFlight][VEC];
+  Pack<T, VEC> u[kHeadsInFlight], v[kHeadsInFlight];
+  const auto load = [&](int h0) {
 #pragma unroll
     for (int k = 0; k < kHeadsInFlight; ++k) {
       const int h = h0 + k * p.head_lanes;
       if (h < p.H) {
-        load_pack<T, VEC>(x + h * p.xh + off_u, u[k]);
-        load_pack<T, VEC>(x + h * p.xh + off_v, v[k]);
+        u[k] = *reinterpret_cast<const Pack<T, VEC>*>(x + h * p.xh + off_u);
+        v[k] = *reinterpret_cast<const Pack<T, VEC>*>(x + h * p.xh + off_v);
       }
     }
+  };
+  load(lane_h);  // in flight while the angles are formed
+
+  float c[VEC], s[VEC];
+  if (turned) {
+    const P raw = reinterpret_cast<const P*>(p.pos)[b * p.pos_b + l * p.pos_l + axis];
+    const float at = p.sign * (float)raw;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float hi = s_hi[pair + i];
+      const float r = at * hi;
+      const float err = fmaf(at, hi, -r) + at * s_lo[pair + i];
+      sincospif(2.0f * ((r - rintf(r)) + err), &s[i], &c[i]);
+    }
+  }
+  for (int h0 = lane_h; h0 < p.H; h0 += kHeadsInFlight * p.head_lanes) {
+    if (h0 != lane_h) load(h0);
 #pragma unroll
     for (int k = 0; k < kHeadsInFlight; ++k) {
       const int h = h0 + k * p.head_lanes;
       if (h >= p.H) break;
       if (turned) {
-        if (INTERLEAVED) {
-          // u, v hold 2 VEC consecutive numbers: pair i is (z[2 i], z[2 i + 1])
-          float z[2 * VEC];
+        float z[2 * VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) z[i] = u[k][i], z[VEC + i] = v[k][i];
+        for (int i = 0; i < VEC; ++i) z[i] = to_f32<T>(u[k].v[i]), z[VEC + i] = to_f32<T>(v[k].v[i]);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float a = z[2 * i], d = z[2 * i + 1];
-            z[2 * i] = a * c[i] - d * s[i];
-            z[2 * i + 1] = a * s[i] + d * c[i];
-          }
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) u[k][i] = z[i], v[k][i] = z[VEC + i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float a = u[k][i], d = v[k][i];
-            u[k][i] = a * c[i] - d * s[i];
-            v[k][i] = a * s[i] + d * c[i];
-          }
+        for (int i = 0; i < VEC; ++i) {
+          const int iu = INTERLEAVED ? 2 * i : i, iv = INTERLEAVED ? 2 * i + 1 : VEC + i;
+          const float a = z[iu], d = z[iv];
+          z[iu] = a * c[i] - d * s[i];
+          z[iv] = a * s[i] + d * c[i];
         }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          u[k].v[i] = from_f32<T>(z[i]), v[k].v[i] = from_f32<T>(z[VEC + i]);
       }
-      store_pack<T, VEC>(y + h * p.yh + off_u, u[k]);
-      store_pack<T, VEC>(y + h * p.yh + off_v, v[k]);
+      *reinterpret_cast<Pack<T, VEC>*>(y + h * p.yh + off_u) = u[k];
+      *reinterpret_cast<Pack<T, VEC>*>(y + h * p.yh + off_v) = v[k];
     }
   }
 }
