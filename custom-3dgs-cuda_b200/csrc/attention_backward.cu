@@ -186,31 +186,34 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int steps = (a.D + 15) / 16;
     const unsigned idesc_s = tc_idesc<T>(kInner, false);
     const unsigned idesc_acc = tc_idesc<T>(steps * 16, true);
+    // descriptor units are 16 bytes; y is read along its rows and across them
+    const uint64_t desc_x1 = tc_desc(sm_x1, 16), desc_x2 = tc_desc(sm_x2, 16),
+                   desc_y = tc_desc(sm_y, 16), desc_yt = tc_desc(sm_y, kInner * 128);
     bool ok = count > 0 && tc_wait_warp(&x_full, 0);
     const auto scores = [&](int j) {  // S and dP of inner tile j
       const int st = j % S::kStages, buf = j & 1;
       if (!tc_wait_warp(&y_full[st], j / S::kStages & 1)) return false;
-      const unsigned y1 = sm_y + st * 2 * S::kInnerBytes, y2 = y1 + S::kInnerBytes;
       if (!KEYS) {
         // keys that all queries leave out: what they hold must not reach dq, where 0 times NaN
         // would be added
         const int key = (t0 + j) * kInner;
         if (n - key < kInner || key_mask)
-          clear_rows<S::kBoxes>(y1, kInner, n - key,
+          clear_rows<S::kBoxes>(sm_y + st * 2 * S::kInnerBytes, kInner, n - key,
                                 key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
       }
-      if (lane == 0) {
-        for (int k = 0; k < steps; ++k) {
-          const unsigned ox = (k / 4) * kOuter * 128 + (k % 4) * 32,
-                         oy = (k / 4) * kInner * 128 + (k % 4) * 32;
-          tc_mma_ss(tm_s + buf * 64, tc_desc(sm_x1 + ox, 16), tc_desc(y1 + oy, 16), idesc_s, k > 0);
-        }
-        for (int k = 0; k < steps; ++k) {
-          const unsigned ox = (k / 4) * kOuter * 128 + (k % 4) * 32,
-                         oy = (k / 4) * kInner * 128 + (k % 4) * 32;
-          tc_mma_ss(tm_dp + buf * 64, tc_desc(sm_x2 + ox, 16), tc_desc(y2 + oy, 16), idesc_s,
-                    k > 0);
-        }
+      if (elect_one()) {
+        const uint64_t in1 = desc_y + st * (2 * S::kInnerBytes / 16),
+                       in2 = in1 + S::kInnerBytes / 16;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+          if (k < steps)
+            tc_mma_ss(tm_s + buf * 64, desc_x1 + (k / 4) * (kOuter * 8) + (k % 4) * 2,
+                      in1 + (k / 4) * (kInner * 8) + (k % 4) * 2, idesc_s, k > 0);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+          if (k < steps)
+            tc_mma_ss(tm_dp + buf * 64, desc_x2 + (k / 4) * (kOuter * 8) + (k % 4) * 2,
+                      in2 + (k / 4) * (kInner * 8) + (k % 4) * 2, idesc_s, k > 0);
         tc_commit(&sp_full[buf]);
       }
       __syncwarp();
@@ -222,15 +225,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       ok = tc_wait_warp(&ready[buf], j / 2 & 1);
       if (!ok) break;
       tc_fence_after();
-      if (lane == 0) {
-        const unsigned y1 = sm_y + st * 2 * S::kInnerBytes, y2 = y1 + S::kInnerBytes;
-        if (KEYS)
+      if (elect_one()) {
+        const uint64_t in1 = desc_yt + st * (2 * S::kInnerBytes / 16),
+                       in2 = in1 + S::kInnerBytes / 16;
+        if (KEYS) {
+#pragma unroll
           for (int k = 0; k < kInner / 16; ++k)
-            tc_mma_ts(tm_acc2, tm_s + buf * 64 + k * 8, tc_desc(y2 + k * 2048, kInner * 128),
-                      idesc_acc, j > 0 || k > 0);
+            tc_mma_ts(tm_acc2, tm_s + buf * 64 + k * 8, in2 + k * 128, idesc_acc, j > 0 || k > 0);
+        }
+#pragma unroll
         for (int k = 0; k < kInner / 16; ++k)
-          tc_mma_ts(tm_acc1, tm_dp + buf * 64 + k * 8, tc_desc(y1 + k * 2048, kInner * 128),
-                    idesc_acc, j > 0 || k > 0);
+          tc_mma_ts(tm_acc1, tm_dp + buf * 64 + k * 8, in1 + k * 128, idesc_acc, j > 0 || k > 0);
         tc_commit(&y_free[st]);
         if (j + 1 == count) tc_commit(&acc_full);
       }

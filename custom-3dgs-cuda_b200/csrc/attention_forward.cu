@@ -124,25 +124,30 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     }
   } else if (warp == 8) {
     // ---- products ----
-    const int lane = threadIdx.x % 32;
     const int steps = (a.D + 15) / 16;
     const unsigned idesc_s = tc_idesc<T>(kTileK, false);
     const unsigned idesc_o = tc_idesc<T>(steps * 16, true);
     const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
+    const uint64_t desc_q = tc_desc(sm_q, 16), desc_k = tc_desc(sm_k, 16),
+                   desc_v = tc_desc(sm_v, 16384);
+    // descriptor units are 16 bytes
     const auto scores = [&](int t, int st) {  // S_t = q_t k^T
-      for (int k = 0; k < steps; ++k) {
-        const unsigned off = (k / 4) * 16384 + (k % 4) * 32;
-        tc_mma_ss(tm_s + t * 128, tc_desc(sm_q + t * S::kTileBytes + off, 16),
-                  tc_desc(sm_k + st * S::kTileBytes + off, 16), idesc_s, k > 0);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const unsigned off = ((k / 4) * 16384 + (k % 4) * 32) / 16;
+        if (k < steps)
+          tc_mma_ss(tm_s + t * 128, desc_q + t * (S::kTileBytes / 16) + off,
+                    desc_k + st * (S::kTileBytes / 16) + off, idesc_s, k > 0);
       }
     };
     const auto values = [&](int t, int st, bool add) {  // O_t += P_t v
+#pragma unroll
       for (int k = 0; k < kTileK / 16; ++k)
         tc_mma_ts(tm_o + t * 128, tm_s + t * 128 + k * 8,
-                  tc_desc(sm_v + st * S::kTileBytes + k * 2048, 16384), idesc_o, add || k > 0);
+                  desc_v + st * (S::kTileBytes / 16) + k * 128, idesc_o, add || k > 0);
     };
     bool ok = count > 0 && tc_wait_warp(&q_full, 0) && tc_wait_warp(&k_full[0], 0);
-    if (ok && lane == 0) {
+    if (ok && elect_one()) {
       scores(0, 0);
       tc_commit(&s_full[0]);
       if (two) {
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         ok = tc_wait_warp(&p_ready[t], j & 1);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
           values(t, st, j > 0);
           if (t == (two ? 1 : 0)) tc_commit(&v_free[st]);
           if (j + 1 < count) {

@@ -46,6 +46,17 @@ __device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, unsigned parity) {
   return __all_sync(~0u, tc_wait(bar, parity));
 }
 
+// True in one lane of the (converged) warp. The products and commits below are issued under it
+// rather than under `lane == 0`: the compiler then knows that one thread runs them and keeps their
+// descriptors in uniform registers (105 -> 25 clocks a product).
+__device__ __forceinline__ bool elect_one() {
+  unsigned is;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(is));
+  return is != 0;
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
