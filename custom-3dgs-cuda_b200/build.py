@@ -28,13 +28,17 @@ NVCC_FLAGS = ARCH_FLAGS + [
     "-O3",
     "-lineinfo",
     "-std=c++17",
-    "-rdc=true",
     "-Xcompiler",
     "-fPIC,-fvisibility=hidden",
     "-Xptxas",
     "-warn-spills",
     "--expt-relaxed-constexpr",
 ]
+
+# Files whose kernels are compiled as whole programs: they move registers between warps
+# (setmaxnreg), which ptxas ignores in relocatable code. They take the address of the device error
+# word as an argument instead of naming it.
+WHOLE_PROGRAM = ("attention_forward.cu", "attention_backward.cu")
 
 
 def nvcc() -> str:
@@ -50,7 +54,8 @@ def _newest_header() -> float:
 
 
 def _compile(src: Path, obj: Path, verbose: bool, extra: list[str]) -> None:
-    cmd = [nvcc(), *NVCC_FLAGS, *extra, "-I", str(CSRC), "-I", str(INCLUDE), "-c", str(src),
+    unit = [] if src.name in WHOLE_PROGRAM else ["-rdc=true"]
+    cmd = [nvcc(), *NVCC_FLAGS, *unit, *extra, "-I", str(CSRC), "-I", str(INCLUDE), "-c", str(src),
            "-o", str(obj)]
     if verbose:
         print(" ".join(cmd), flush=True)

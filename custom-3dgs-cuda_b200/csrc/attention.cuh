@@ -1,7 +1,7 @@
 // What the cross-attention kernels share: the operands' description, lengths and masks.
 #pragma once
 
-#include "gs_common.cuh"
+#include "device_errors.h"
 #include "token_types.cuh"
 
 namespace gs {

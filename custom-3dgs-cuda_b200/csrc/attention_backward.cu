@@ -34,6 +34,7 @@ constexpr int kBwdThreads = 320;
 
 struct BackwardParams {
   AttentionParams a;
+  unsigned* errors;  // the device's error word
   float scale_log2;
   const float2* stats;  // [B, Hq, lq_pad]: lse log2 e - kLog2 (+inf: no probability), delta
   int lq_pad;           // Lq rounded up to kInner
@@ -119,14 +120,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
   const unsigned sm_x1 = base, sm_x2 = sm_x1 + S::kOuterBytes, sm_y = sm_x2 + S::kOuterBytes,
                  sm_stats = sm_y + S::kStages * 2 * S::kInnerBytes;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = warp_uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
   const AttentionParams& a = p.a;
   const int shared_heads = a.Hq / a.Hkv;
   const int outer_rows = KEYS ? a.Lk : a.Lq, outer_heads = KEYS ? a.Hkv : a.Hq;
   const int outer_tiles = (outer_rows + kOuter - 1) / kOuter;
   const int x0 = blockIdx.x % outer_tiles * kOuter, bh = blockIdx.x / outer_tiles;
   const int b = bh / outer_heads, ho = bh % outer_heads;
-  const int n = key_count(a, b);
+  const int n = warp_uniform(key_count(a, b));
   const int q_tiles = p.lq_pad / kInner;
   const int tiles = KEYS ? (x0 < n ? q_tiles * shared_heads : 0) : (n + kInner - 1) / kInner;
   const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
@@ -143,14 +144,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sp_full[i], 1);
-      mbar_init(&ready[i], 128);
+      mbar_init(&ready[i], 4);
     }
   }
   if (warp == 8) tc_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = tmem_slot;
+  const unsigned tmem = (unsigned)warp_uniform((int)tmem_slot);
   const unsigned tm_s = tmem, tm_dp = tmem + 128, tm_acc1 = tmem + 256, tm_acc2 = tmem + 384;
 
   if (warp == 9) {
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(&ready[wg]);
+      mbar_arrive_warp(&ready[wg]);
     }
     if (ok && count > 0) ok = tc_wait_warp(&acc_full, 0);
     if (!ok) gave_up = 1;
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (gave_up) {
     // A wait ran out. Copies still in flight end before the CTA's memory is given up.
     if (threadIdx.x == 0) {
-      raise_device_error(kErrMmaTimeout);
+      atomicOr(p.errors, kErrMmaTimeout);
       const unsigned long long t = tma_global_ns();
       for (int k = 0; k < (1 << 20) && tma_global_ns() - t < 10000000ull; ++k) __nanosleep(1000);
     }
@@ -466,6 +467,7 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   const BackwardPlan plan = backward_plan(a);
   BackwardParams p{};
   p.a = attention_params(a);
+  GS_CUDA(device_error_word(&p.errors));
   p.a.dout = TokenView(dout), p.a.dq = TokenView(dq), p.a.dk = TokenView(dk),
   p.a.dv = TokenView(dv);
   // a scale of 0 weighs all keys alike; -inf, where a key is left out, has to stay what it is

@@ -27,10 +27,14 @@ namespace gs {
 constexpr int kTileQ = 128;   // query rows of one warpgroup
 constexpr int kTileK = 128;   // keys of one tile
 constexpr float kLag = 8.0f;  // powers of two
-constexpr int kFwdThreads = 320;
+constexpr int kFwdThreads = 384;
+// Registers of a softmax thread and of the others: 2 x 128 x 200 + 128 x 104 = 384 x 168, what the
+// CTA is launched with.
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
 
 struct ForwardParams {
   AttentionParams a;
+  unsigned* errors;  // the device's error word
   float scale_log2;  // |scale| log2 e, above 0
   float lag;         // kLag in units of unscaled scores
   int negate;        // scale < 0: scores change sign first
@@ -57,36 +61,39 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   using S = ForwardShared<DP>;
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t q_full, k_full[S::kStages], k_free[S::kStages], v_full[S::kStages],
-      v_free[S::kStages], s_full[2], p_ready[2], o_full[2];
+      v_clean[S::kStages], v_free[S::kStages], s_full[2], s_read[2], p_ready[2], o_done[2], o_full[2];
   __shared__ unsigned tmem_slot;
   __shared__ volatile int gave_up;
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
   const unsigned sm_q = base, sm_k = base + 2 * S::kTileBytes,
                  sm_v = sm_k + S::kStages * S::kTileBytes;
-  const int warp = threadIdx.x / 32;
+  const int warp = warp_uniform(threadIdx.x / 32);
   const AttentionParams& a = p.a;
   const int q_blocks = (a.Lq + 2 * kTileQ - 1) / (2 * kTileQ);
   const int q0 = blockIdx.x % q_blocks * 2 * kTileQ, bh = blockIdx.x / q_blocks;
   const int b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hkv);
-  const int n = key_count(a, b);
+  const int n = warp_uniform(key_count(a, b));
   const int tiles = (n + kTileK - 1) / kTileK;
   const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
   const int t1 = (int)((long long)tiles * (blockIdx.y + 1) / p.splits);
   const int count = t1 - t0;
-  const bool two = q0 + kTileQ < a.Lq;
+  const bool both = q0 + kTileQ < a.Lq;
 
   if (threadIdx.x == 0) {
     gave_up = 0;
     mbar_init(&q_full, 1);
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_free[i], 1);
+      mbar_init(&k_free[i], both ? 2 : 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_free[i], 1);
+      mbar_init(&v_clean[i], 1);
+      mbar_init(&v_free[i], both ? 2 : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 128);
+      mbar_init(&s_read[i], 4);
+      mbar_init(&p_ready[i], 4);
+      mbar_init(&o_done[i], 1);
       mbar_init(&o_full[i], 1);
     }
   }
@@ -94,106 +101,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = tmem_slot;
-  const unsigned tm_s = tmem, tm_o = tmem + 256;
+  const unsigned tmem = (unsigned)warp_uniform((int)tmem_slot);
+  // Tensor memory, 512 columns: S of both tiles 256, O of both 2 DP. Up to D = 64 there is room
+  // for P beside S; above, P takes the first half of S's own columns.
+  constexpr bool kAhead = DP == 64;
+  const unsigned tm_s = tmem, tm_o = tmem + (kAhead ? 384 : 256);
+  const unsigned tm_p = kAhead ? tmem + 256 : tmem;
+  constexpr unsigned kStepP = kAhead ? 64 : 128, kStepO = kAhead ? 64 : 128;
 
-  if (warp == 9) {
-    // ---- copies ----
-    if (threadIdx.x % 32 == 0 && count > 0) {
-      const int bq = b * p.qb, hq = h * p.qh;
-      mbar_arrive_expect_tx(&q_full, (two ? 2 : 1) * S::kTileBytes);
-      for (int t = 0; t < (two ? 2 : 1); ++t)
-        for (int x = 0; x < S::kBoxes; ++x)
-          tma_load_4d(sm_q + t * S::kTileBytes + x * 16384, &map_q, x * 64, q0 + t * kTileQ, hq, bq,
-                      &q_full);
-      for (int j = 0; j < count; ++j) {
-        const int st = j % S::kStages;
-        const unsigned phase = (j / S::kStages & 1) ^ 1;
-        const int key = (t0 + j) * kTileK;
-        if (!tc_wait(&k_free[st], phase)) { gave_up = 1; break; }
-        mbar_arrive_expect_tx(&k_full[st], S::kTileBytes);
-        for (int x = 0; x < S::kBoxes; ++x)
-          tma_load_4d(sm_k + st * S::kTileBytes + x * 16384, &map_k, x * 64, key, hk * p.kh,
-                      b * p.kb, &k_full[st]);
-        if (!tc_wait(&v_free[st], phase)) { gave_up = 1; break; }
-        mbar_arrive_expect_tx(&v_full[st], S::kTileBytes);
-        for (int x = 0; x < S::kBoxes; ++x)
-          tma_load_4d(sm_v + st * S::kTileBytes + x * 16384, &map_v, x * 64, key, hk * p.vh,
-                      b * p.vb, &v_full[st]);
-      }
-    }
-  } else if (warp == 8) {
-    // ---- products ----
-    const int steps = (a.D + 15) / 16;
-    const unsigned idesc_s = tc_idesc<T>(kTileK, false);
-    const unsigned idesc_o = tc_idesc<T>(steps * 16, true);
-    const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
-    const uint64_t desc_q = tc_desc(sm_q, 16), desc_k = tc_desc(sm_k, 16),
-                   desc_v = tc_desc(sm_v, 16384);
-    // descriptor units are 16 bytes
-    const auto scores = [&](int t, int st) {  // S_t = q_t k^T
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const unsigned off = ((k / 4) * 16384 + (k % 4) * 32) / 16;
-        if (k < steps)
-          tc_mma_ss(tm_s + t * 128, desc_q + t * (S::kTileBytes / 16) + off,
-                    desc_k + st * (S::kTileBytes / 16) + off, idesc_s, k > 0);
-      }
-    };
-    const auto values = [&](int t, int st, bool add) {  // O_t += P_t v
-#pragma unroll
-      for (int k = 0; k < kTileK / 16; ++k)
-        tc_mma_ts(tm_o + t * 128, tm_s + t * 128 + k * 8,
-                  desc_v + st * (S::kTileBytes / 16) + k * 128, idesc_o, add || k > 0);
-    };
-    bool ok = count > 0 && tc_wait_warp(&q_full, 0) && tc_wait_warp(&k_full[0], 0);
-    if (ok && elect_one()) {
-      scores(0, 0);
-      tc_commit(&s_full[0]);
-      if (two) {
-        scores(1, 0);
-        tc_commit(&s_full[1]);
-      }
-      tc_commit(&k_free[0]);
-    }
-    for (int j = 0; ok && j < count; ++j) {
-      const int st = j % S::kStages, next = (j + 1) % S::kStages;
-      ok = tc_wait_warp(&v_full[st], j / S::kStages & 1);
-      if (!ok) break;
-      // What v holds at keys that no query of the CTA keeps must not reach the product, which
-      // would make 0 times NaN of it: those rows are set to zero.
-      const int key = (t0 + j) * kTileK;
-      if (n - key < kTileK || key_mask)
-        clear_rows<S::kBoxes>(sm_v + st * S::kTileBytes, kTileK, n - key,
-                              key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
-      if (j + 1 < count) ok = tc_wait_warp(&k_full[next], (j + 1) / S::kStages & 1);
-      if (!ok) break;
-      for (int t = 0; t < (two ? 2 : 1); ++t) {
-        ok = tc_wait_warp(&p_ready[t], j & 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          values(t, st, j > 0);
-          if (t == (two ? 1 : 0)) tc_commit(&v_free[st]);
-          if (j + 1 < count) {
-            scores(t, next);
-            tc_commit(&s_full[t]);
-            if (t == (two ? 1 : 0)) tc_commit(&k_free[next]);
-          } else {
-            tc_commit(&o_full[t]);
-          }
-        }
-        __syncwarp();
-      }
-    }
-    if (!ok && count > 0) gave_up = 1;
-  } else {
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---- softmax: one thread for each query row ----
     const int t = warp / 4;
     const int i = q0 + t * kTileQ + threadIdx.x % 128;
-    if (t == 0 || two) {
+    if (t == 0 || both) {
       const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
-      const unsigned my_s = tm_s + t * 128 + lanes, my_o = tm_o + t * 128 + lanes;
+      const unsigned my_s = tm_s + t * 128 + lanes, my_o = tm_o + t * kStepO + lanes,
+                     my_p = tm_p + t * kStepP + lanes;
       const uint4* keep_row =
           a.bits ? reinterpret_cast<const uint4*>(a.bits + b * a.bits_b + h * a.bits_h +
                                                   (long long)min(i, a.Lq - 1) * a.bits_q)
@@ -211,6 +135,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
         for (int c = 0; c < kTileK; c += 32) tc_ld32(my_s + c, s + c);
         tc_wait_ld();
+        if (kAhead) {
+          tc_fence_before();
+          mbar_arrive_warp(&s_read[t]);
+        }
         if (p.negate) {
 #pragma unroll
           for (int k = 0; k < kTileK; ++k) s[k] ^= 0x80000000u;
@@ -223,9 +151,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < kTileK; ++k) top[k % 4] = fmaxf(top[k % 4], __uint_as_float(s[k]));
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        const bool grew = mx > m + p.lag;
+        for (int k = 0; k < kTileK; k += 2)
+          top[k / 2 % 4] = max_nan(max_nan(top[k / 2 % 4], __uint_as_float(s[k])),
+                                   __uint_as_float(s[k + 1]));
+        const float mx = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+        const bool grew = !(mx <= m + p.lag);  // NaN too: then the row is NaN from here on
+        if (kAhead && j > 0) {  // the product that read the P before, and added to O, is over
+          ok = tc_wait_warp(&o_done[t], (j - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+        }
         if (__any_sync(~0u, grew)) {
           const float f = grew ? fast_exp2((m - mx) * p.scale_log2) : 1.0f;
           if (grew) m = mx;
@@ -241,25 +176,32 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             }
           }
         }
-        const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
-        float sum[2] = {0.0f, 0.0f};
+        // m - m is 0, or NaN where the row holds an infinite score
+        const float off = m == -INFINITY ? 0.0f : fmaf(m, p.scale_log2, m - m);
+        const Two scale2 = two(p.scale_log2, p.scale_log2), off2 = two(-off, -off);
+        Two sum[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
 #pragma unroll
         for (int c = 0; c < kTileK; c += 32) {
           unsigned packed[16];
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float e0 = fast_exp2(fmaf(__uint_as_float(s[c + k]), p.scale_log2, -off));
-            const float e1 = fast_exp2(fmaf(__uint_as_float(s[c + k + 1]), p.scale_log2, -off));
-            sum[0] += e0;
-            sum[1] += e1;
-            packed[k / 2] = pack2<T>(e0, e1);
+          for (int k = 0; k < 16; ++k) {
+            const Two x = fma2(two(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])),
+                               scale2, off2);
+            float e0, e1;
+            split(x, e0, e1);
+            e0 = fast_exp2(e0);
+            e1 = fast_exp2(e1);
+            sum[k % 2] = add2(sum[k % 2], two(e0, e1));
+            packed[k] = pack2<T>(e0, e1);
           }
-          tc_st16(my_s + c / 2, packed);
+          tc_st16(my_p + c / 2, packed);
         }
-        l += sum[0] + sum[1];
+        float sum0, sum1;
+        split(add2(sum[0], sum[1]), sum0, sum1);
+        l += sum0 + sum1;
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_ready[t]);
+        mbar_arrive_warp(&p_ready[t]);
       }
       if (ok && count > 0) ok = tc_wait_warp(&o_full[t], 0);
       if (!ok) gave_up = 1;
@@ -306,13 +248,111 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           a.lse[row] = lse;
       }
     }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 9) {
+      // ---- copies ----
+      if (threadIdx.x % 32 == 0 && count > 0) {
+        const int bq = b * p.qb, hq = h * p.qh;
+        mbar_arrive_expect_tx(&q_full, (both ? 2 : 1) * S::kTileBytes);
+        for (int t = 0; t < (both ? 2 : 1); ++t)
+          for (int x = 0; x < S::kBoxes; ++x)
+            tma_load_4d(sm_q + t * S::kTileBytes + x * 16384, &map_q, x * 64, q0 + t * kTileQ, hq, bq,
+                        &q_full);
+        for (int j = 0; j < count; ++j) {
+          const int st = j % S::kStages;
+          const unsigned phase = (j / S::kStages & 1) ^ 1;
+          const int key = (t0 + j) * kTileK;
+          if (!tc_wait(&k_free[st], phase)) { gave_up = 1; break; }
+          mbar_arrive_expect_tx(&k_full[st], S::kTileBytes);
+          for (int x = 0; x < S::kBoxes; ++x)
+            tma_load_4d(sm_k + st * S::kTileBytes + x * 16384, &map_k, x * 64, key, hk * p.kh,
+                        b * p.kb, &k_full[st]);
+          if (!tc_wait(&v_free[st], phase)) { gave_up = 1; break; }
+          mbar_arrive_expect_tx(&v_full[st], S::kTileBytes);
+          for (int x = 0; x < S::kBoxes; ++x)
+            tma_load_4d(sm_v + st * S::kTileBytes + x * 16384, &map_v, x * 64, key, hk * p.vh,
+                        b * p.vb, &v_full[st]);
+        }
+      }
+    } else if (warp == 11) {
+      // ---- what v holds at keys that no query of the CTA keeps must not reach the product, which
+      // would make 0 times NaN of it: those rows are set to zero before the product may read them
+      const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
+      for (int j = 0; j < count; ++j) {
+        const int st = j % S::kStages, key = (t0 + j) * kTileK;
+        if (!tc_wait_warp(&v_full[st], j / S::kStages & 1)) { gave_up = 1; break; }
+        if (n - key < kTileK || key_mask)
+          clear_rows<S::kBoxes>(sm_v + st * S::kTileBytes, kTileK, n - key,
+                                key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
+        mbar_arrive_warp(&v_clean[st]);
+      }
+    } else if (warp == 8 || (warp == 10 && both)) {
+      // ---- products: a warp for each query tile, on different schedulers ----
+      const int t = warp == 10;
+      const int steps = (a.D + 15) / 16;
+      const unsigned idesc_s = tc_idesc<T>(kTileK, false);
+      const unsigned idesc_o = tc_idesc<T>(steps * 16, true);
+      // descriptor units are 16 bytes
+      const uint64_t desc_q = tc_desc(sm_q + t * S::kTileBytes, 16), desc_k = tc_desc(sm_k, 16),
+                     desc_v = tc_desc(sm_v, 16384);
+      const unsigned tm_st = tm_s + t * 128, tm_pt = tm_p + t * kStepP, tm_ot = tm_o + t * kStepO;
+      // S = q k^T of tile j, once k is there and (where P has its own columns) the softmax has read
+      // the S before
+      const auto next_scores = [&](int j) {
+        const int st = j % S::kStages;
+        if (!tc_wait_warp(&k_full[st], j / S::kStages & 1)) return false;
+        if (kAhead && j > 0) {
+          if (!tc_wait_warp(&s_read[t], (j - 1) & 1)) return false;
+          tc_fence_after();
+        }
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const unsigned off = ((k / 4) * 16384 + (k % 4) * 32) / 16;
+            if (k < steps)
+              tc_mma_ss(tm_st, desc_q + off, desc_k + st * (S::kTileBytes / 16) + off, idesc_s, k > 0);
+          }
+          tc_commit(&s_full[t]);
+          tc_commit(&k_free[st]);
+        }
+        __syncwarp();
+        return true;
+      };
+      const auto values = [&](int st, bool add) {  // O += P v
+#pragma unroll
+        for (int k = 0; k < kTileK / 16; ++k)
+          tc_mma_ts(tm_ot, tm_pt + k * 8, desc_v + st * (S::kTileBytes / 16) + k * 128, idesc_o,
+                    add || k > 0);
+      };
+      constexpr int kLead = kAhead ? 2 : 1;  // tiles that S is ahead of P
+      bool ok = count > 0 && tc_wait_warp(&q_full, 0);
+      for (int j = 0; j < kLead; ++j) ok = ok && (j >= count || next_scores(j));
+      for (int j = 0; ok && j < count; ++j) {
+        const int st = j % S::kStages;
+        ok = tc_wait_warp(&v_clean[st], j / S::kStages & 1);
+        if (!ok) break;
+        ok = tc_wait_warp(&p_ready[t], j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          values(st, j > 0);
+          if (kAhead) tc_commit(&o_done[t]);
+          tc_commit(&v_free[st]);
+          if (j + 1 == count) tc_commit(&o_full[t]);
+        }
+        __syncwarp();
+        if (j + kLead < count) ok = next_scores(j + kLead);
+      }
+      if (!ok && count > 0) gave_up = 1;
+    }
   }
   tc_fence_before();
   __syncthreads();
   if (gave_up) {
     // A wait ran out. Copies still in flight end before the CTA's memory is given up.
     if (threadIdx.x == 0) {
-      raise_device_error(kErrMmaTimeout);
+      atomicOr(p.errors, kErrMmaTimeout);
       const unsigned long long t = tma_global_ns();
       for (int k = 0; k < (1 << 20) && tma_global_ns() - t < 10000000ull; ++k) __nanosleep(1000);
     }
@@ -409,6 +449,7 @@ cudaError_t attention_combine(const gs_attention_args& args, int splits, const f
 int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t stream) {
   ForwardParams p{};
   p.a = attention_params(a);
+  GS_CUDA(device_error_word(&p.errors));
   const float magnitude = std::max(std::fabs(a.scale), 1e-30f);  // a scale of 0 weighs all alike
   p.scale_log2 = magnitude * 1.4426950408889634f;
   p.lag = std::min(kLag / p.scale_log2, 1e30f);

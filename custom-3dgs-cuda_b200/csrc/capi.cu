@@ -30,6 +30,20 @@ int set_error(int code, const std::string& msg) {
 
 void clear_error() { t_last_error.clear(); }
 
+cudaError_t device_error_word(unsigned** word) {
+  static constexpr int kMaxDevices = 64;
+  static std::atomic<unsigned*> known[kMaxDevices] = {};
+  int dev = 0;
+  if (const cudaError_t err = cudaGetDevice(&dev)) return err;
+  if (dev >= 0 && dev < kMaxDevices)
+    if ((*word = known[dev].load(std::memory_order_acquire))) return cudaSuccess;
+  void* at = nullptr;
+  if (const cudaError_t err = cudaGetSymbolAddress(&at, g_device_errors)) return err;
+  *word = static_cast<unsigned*>(at);
+  if (dev >= 0 && dev < kMaxDevices) known[dev].store(*word, std::memory_order_release);
+  return cudaSuccess;
+}
+
 }  // namespace gs
 
 extern "C" const char* gs_last_error(void) { return gs::t_last_error.c_str(); }

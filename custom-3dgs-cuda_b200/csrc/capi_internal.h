@@ -20,6 +20,10 @@ void mark_stage(int k, cudaStream_t stream);
 int set_error(int code, const std::string& msg);
 void clear_error();
 
+// Address of the current device's error word (gs_device_error_bits), for kernels compiled as whole
+// programs.
+cudaError_t device_error_word(unsigned** word);
+
 }  // namespace gs
 
 #define GS_API_BEGIN() \

@@ -4,18 +4,12 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "device_errors.h"
+
 namespace gs {
 
 constexpr int kTileSide = 16;                     // 16 x 16 pixel tiles
 constexpr int kTilePixels = kTileSide * kTileSide;
-
-// Device error bits (OR-ed into g_device_errors by the kernels).
-constexpr unsigned kErrLookbackTimeout = 1u;  // a decoupled look-back wait hit its limit
-constexpr unsigned kErrCapacity = 2u;         // pair count exceeded the pair capacity
-constexpr unsigned kErrBadIndex = 4u;         // an index was out of range
-constexpr unsigned kErrPeerTimeout = 8u;      // a cross-GPU barrier wait hit its limit
-constexpr unsigned kErrCopyTimeout = 16u;     // a wait for a tensor-memory-accelerator copy hit its limit
-constexpr unsigned kErrMmaTimeout = 32u;      // a wait inside an attention kernel hit its limit
 
 // Iteration limit of every spin-wait. Each iteration is one L2 round trip plus a short
 // sleep, so the limit bounds a wait to well under a second.

@@ -56,13 +56,7 @@ __device__ __forceinline__ float row_sum(float v, float* shared) {
   return v;
 }
 
-// The larger of two, NaN where either is: a row with a NaN says so in its scale.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float c;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-  return c;
-}
-
+// NaN where the row holds one, so that its scale says so.
 template <int ROW>
 __device__ __forceinline__ float row_max(float v, float* shared) {
 #pragma unroll

@@ -47,8 +47,8 @@ __device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, unsigned parity) {
 }
 
 // True in one lane of the (converged) warp. The products and commits below are issued under it
-// rather than under `lane == 0`: the compiler then knows that one thread runs them and keeps their
-// descriptors in uniform registers (105 -> 25 clocks a product).
+// rather than under `lane == 0`: the compiler then knows that one thread runs them (105 clocks to
+// issue a product under `lane == 0`, under 64 so).
 __device__ __forceinline__ bool elect_one() {
   unsigned is;
   asm volatile(
@@ -57,8 +57,19 @@ __device__ __forceinline__ bool elect_one() {
   return is != 0;
 }
 
+// A value that all lanes of the (converged) warp share, so that the compiler knows it: branches on
+// it are not divergent and descriptors made of it live in uniform registers.
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(~0u, v, 0); }
+
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// One arrival for the warp, after what its lanes have done (32 arrivals of a warp on one barrier
+// would queue up).
+__device__ __forceinline__ void mbar_arrive_warp(uint64_t* bar) {
+  __syncwarp();
+  if (elect_one()) mbar_arrive(bar);
 }
 
 // Box at (x, y, z, w), innermost first, into swizzled shared memory, completing on `bar`.
@@ -201,6 +212,27 @@ __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two floats in a 64-bit register: one instruction adds or multiplies both.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(Two v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // Host: describes a [B, L, H, D] tensor of 16-bit numbers as (D, L, H, B), innermost first, copied

@@ -14,8 +14,6 @@
 
 #include <mutex>
 
-#include "gs_common.cuh"
-
 namespace gs {
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) {

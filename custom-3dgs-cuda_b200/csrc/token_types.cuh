@@ -55,6 +55,13 @@ __device__ __forceinline__ void store_pack(T* p, const float (&in)[N]) {
   *reinterpret_cast<Pack<T, N>*>(p) = a;
 }
 
+// The larger of two, NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+
 inline size_t element_size(int dtype) { return dtype == GS_FP32 ? 4 : 2; }
 inline bool known_type(int dtype) {
   return dtype == GS_FP32 || dtype == GS_FP16 || dtype == GS_BF16;
