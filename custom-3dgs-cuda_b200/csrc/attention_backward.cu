@@ -8,12 +8,21 @@
 // tiles of 128 queries and walks over the keys (dq). Both recompute S and dP: 7 products for
 // each pair of tiles instead of the 5 that one kernel with shared sums would need.
 //
-// Both are the same kernel, with KEYS telling which side is owned. The owned ("outer") tiles stay
-// in shared memory, the others ("inner", 64 rows) stream through. S and dP, outer rows x inner
-// rows, are products into tensor memory; a thread for each outer row turns them into P and dS in
-// 16 bits, in place; those are the next products' left operands, read from tensor memory, with
-// the same inner tiles read across as right operands. S and dP exist twice: two warpgroups take
-// inner tiles in turn, one works on a tile while the other's products run.
+// Both are the same kernel, with KEYS telling which side is owned. The owned ("outer") tile of 128
+// rows stays in shared memory, the others ("inner", 128 rows) stream through. S and dP, outer rows
+// x inner rows, are products into tensor memory; two warpgroups, each with a thread for each outer
+// row and half of the inner columns, turn S into P and then dP into dS, both in 16 bits and back in
+// tensor memory, where they are the left operands of the sums, with the same inner tile read
+// across as the right operand.
+//
+// What bounds it: at D = 128 a pair of tiles takes 512 clocks of the tensor pipe for each product
+// (2,048 for dk and dv, 1,536 for dq), and the exponentials 1,024 clocks of the special-function
+// unit; at D = 64 the products take half of that. So S of the next tile has to be formed while
+// this one's P and dS are: where tensor memory has room (512 columns: S 128, dP 128, a sum D, P and
+// dS 64 each) P and dS have their own columns, S and dP are free again as soon as they have been
+// read, and one warp issues S and dP, another the sums. For dk and dv at D above 64 there is no
+// room: P takes S's columns and dS dP's, and one warp issues dv, the next S, dk, the next dP, each
+// as its operand arrives, so that S is formed beside the dS of the tile before.
 //
 // P and dS are rounded to the products' 16-bit type, a relative error for bfloat16 down to 2^-126,
 // where the exponential's results and the products' operands end. Both are formed 2^32 times
@@ -29,14 +38,18 @@
 
 namespace gs {
 
-constexpr int kOuter = 128, kInner = 64;
-constexpr int kBwdThreads = 320;
+constexpr int kOuter = 128, kInner = 128;
+constexpr int kBwdThreads = 384;
+// Registers of a thread of the P and dS warps and of the others: 2 x 128 x 200 + 128 x 104 =
+// 384 x 168, what the CTA is launched with.
+constexpr int kMathRegs = 200, kRestRegs = 104;
 
 struct BackwardParams {
   AttentionParams a;
   unsigned* errors;  // the device's error word
   float scale_log2;
-  const float2* stats;  // [B, Hq, lq_pad]: lse log2 e - kLog2 (+inf: no probability), delta
+  // [B, Hq, lq_pad / kInner, 2, kInner]: lse log2 e - kLog2 (+inf: no probability), delta
+  const float* stats;
   int lq_pad;           // Lq rounded up to kInner
   int splits;           // of the inner tiles
   int x1b, x1h, x2b, x2h, y1b, y1h, y2b, y2h;  // 0 where items or heads share the tensor, else 1
@@ -44,14 +57,14 @@ struct BackwardParams {
   float* part2;  // dv
 };
 
-template <int DP>
+template <int DP, bool KEYS>
 struct BackwardShared {
   static constexpr int kBoxes = DP / 64;
   static constexpr int kOuterBytes = kBoxes * kOuter * 128;
   static constexpr int kInnerBytes = kBoxes * kInner * 128;
-  static constexpr int kStages = DP == 128 ? 4 : 6;
-  static constexpr int kBytes =
-      1024 + 2 * kOuterBytes + kStages * (2 * kInnerBytes + kInner * 8);
+  static constexpr bool kOwnP = !(KEYS && DP == 128);  // P and dS have their own columns
+  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr int kBytes = 1024 + 2 * kOuterBytes + kStages * (2 * kInnerBytes + kInner * 8);
 };
 
 // P is formed 2^kLog2 times larger; kDs brings dS back where its type cannot hold that, kAcc1 and
@@ -68,10 +81,10 @@ struct ProbabilityScale<__half> {
 };
 
 // delta and lse in powers of two of every query row, 8 lanes a row; the rows, padded to a multiple
-// of 64 for each head, fill the grid exactly.
+// of kInner for each head, fill the grid exactly.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams a, int lq_pad,
-                                                                float2* stats) {
+                                                                float* stats) {
   const int sub = threadIdx.x % 8;
   const long long at = (long long)blockIdx.x * 32 + threadIdx.x / 8;
   const int i = (int)(at % lq_pad), h = (int)(at / lq_pad % a.Hq), b = (int)(at / lq_pad / a.Hq);
@@ -92,7 +105,19 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams 
   }
 #pragma unroll
   for (int w = 4; w; w >>= 1) delta += __shfl_xor_sync(~0u, delta, w);
-  if (sub == 0) stats[at] = make_float2(lse, delta);
+  if (sub == 0) {
+    float* tile = stats + at / kInner * (2 * kInner) + at % kInner;
+    tile[0] = lse;
+    tile[kInner] = delta;
+  }
+}
+
+__device__ __forceinline__ float4 ld_shared4(unsigned at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at));
+  return v;
 }
 
 __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes,
@@ -104,6 +129,60 @@ __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigne
       : "memory");
 }
 
+// Where a column's bit in `keep` is 0: no probability (s to the side of the exponent's sign that
+// gives 0), and 0 times what the value product holds there, NaN included, is 0.
+__device__ __forceinline__ void hide(const unsigned (&keep)[2], bool negative, unsigned* s,
+                                     unsigned* dp) {
+  const unsigned none = negative ? 0x7f800000u : kMinusInf;
+#pragma unroll
+  for (int k = 0; k < 64; ++k)
+    if (!(keep[k / 32] >> (k % 32) & 1u)) {
+      if (s) s[k] = none;
+      dp[k] = 0u;
+    }
+}
+
+// P = 2^(S c - lse) of 32 columns, in place. lse is the columns' in shared memory (KEYS) or the
+// row's own.
+template <bool KEYS>
+__device__ __forceinline__ void probabilities(unsigned* s, float c, unsigned at, float own) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 4) {
+    float4 l = make_float4(own, own, own, own);
+    if (KEYS) l = ld_shared4(at + k * 4);
+    s[k] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[k]), c, -l.x)));
+    s[k + 1] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[k + 1]), c, -l.y)));
+    s[k + 2] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[k + 2]), c, -l.z)));
+    s[k + 3] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[k + 3]), c, -l.w)));
+  }
+}
+
+// dS = P (dP - delta) scale of 32 columns, in P's place.
+template <bool KEYS>
+__device__ __forceinline__ void differences(unsigned* p, const unsigned* dp, unsigned at,
+                                            float own, float scale) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 4) {
+    float4 d = make_float4(own, own, own, own);
+    if (KEYS) d = ld_shared4(at + k * 4);
+    const auto ds = [&](int i, float delta) {
+      return __float_as_uint(__uint_as_float(p[i]) * ((__uint_as_float(dp[i]) - delta) * scale));
+    };
+    p[k] = ds(k, d.x), p[k + 1] = ds(k + 1, d.y);
+    p[k + 2] = ds(k + 2, d.z), p[k + 3] = ds(k + 3, d.w);
+  }
+}
+
+// 32 columns rounded to 16 bits, into 16 columns of tensor memory.
+template <typename T>
+__device__ __forceinline__ void store_packed(unsigned at, const unsigned* v) {
+  unsigned packed[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    packed[k] = pack2<T>(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+  tc_st16(at, packed);
+}
+
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attention_backward_kernel(const __grid_constant__ BackwardParams p,
@@ -111,10 +190,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                               const __grid_constant__ CUtensorMap map_x2,
                               const __grid_constant__ CUtensorMap map_y1,
                               const __grid_constant__ CUtensorMap map_y2) {
-  using S = BackwardShared<DP>;
+  using S = BackwardShared<DP, KEYS>;
   using PS = ProbabilityScale<T>;
   extern __shared__ unsigned char raw[];
-  __shared__ uint64_t x_full, y_full[S::kStages], y_free[S::kStages], sp_full[2], ready[2], acc_full;
+  __shared__ uint64_t x_full, y_full[S::kStages], y_free[S::kStages], s_full, s_read, dp_full,
+      p_ready, ds_ready, acc_done, acc_full;
   __shared__ unsigned tmem_slot;
   __shared__ volatile int gave_up;
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -142,109 +222,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&y_full[i], 1);
       mbar_init(&y_free[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sp_full[i], 1);
-      mbar_init(&ready[i], 4);
-    }
+    for (uint64_t* bar : {&s_full, &dp_full, &acc_done}) mbar_init(bar, 1);
+    for (uint64_t* bar : {&s_read, &p_ready, &ds_ready}) mbar_init(bar, 8);
   }
   if (warp == 8) tc_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = (unsigned)warp_uniform((int)tmem_slot);
-  const unsigned tm_s = tmem, tm_dp = tmem + 128, tm_acc1 = tmem + 256, tm_acc2 = tmem + 384;
-
-  if (warp == 9) {
-    // ---- copies ----
-    if (lane == 0 && count > 0) {
-      mbar_arrive_expect_tx(&x_full, 2 * S::kOuterBytes);
-      for (int x = 0; x < S::kBoxes; ++x) {
-        tma_load_4d(sm_x1 + x * kOuter * 128, &map_x1, x * 64, x0, ho * p.x1h, b * p.x1b, &x_full);
-        tma_load_4d(sm_x2 + x * kOuter * 128, &map_x2, x * 64, x0, ho * p.x2h, b * p.x2b, &x_full);
-      }
-      for (int j = 0; j < count; ++j) {
-        const int st = j % S::kStages;
-        if (!tc_wait(&y_free[st], (j / S::kStages & 1) ^ 1)) { gave_up = 1; break; }
-        const int t = t0 + j;
-        const int head = KEYS ? ho * shared_heads + t / q_tiles : ho / shared_heads;
-        const int row = (KEYS ? t % q_tiles : t) * kInner;
-        const unsigned dst = sm_y + st * 2 * S::kInnerBytes;
-        mbar_arrive_expect_tx(&y_full[st], 2 * S::kInnerBytes + (KEYS ? kInner * 8 : 0));
-        for (int x = 0; x < S::kBoxes; ++x) {
-          tma_load_4d(dst + x * kInner * 128, &map_y1, x * 64, row, head * p.y1h, b * p.y1b,
-                      &y_full[st]);
-          tma_load_4d(dst + S::kInnerBytes + x * kInner * 128, &map_y2, x * 64, row, head * p.y2h,
-                      b * p.y2b, &y_full[st]);
-        }
-        if (KEYS)
-          bulk_load(sm_stats + st * kInner * 8,
-                    p.stats + ((long long)b * a.Hq + head) * p.lq_pad + row, kInner * 8,
-                    &y_full[st]);
-      }
-    }
-  } else if (warp == 8) {
-    // ---- products ----
-    const int steps = (a.D + 15) / 16;
-    const unsigned idesc_s = tc_idesc<T>(kInner, false);
-    const unsigned idesc_acc = tc_idesc<T>(steps * 16, true);
-    // descriptor units are 16 bytes; y is read along its rows and across them
-    const uint64_t desc_x1 = tc_desc(sm_x1, 16), desc_x2 = tc_desc(sm_x2, 16),
-                   desc_y = tc_desc(sm_y, 16), desc_yt = tc_desc(sm_y, kInner * 128);
-    bool ok = count > 0 && tc_wait_warp(&x_full, 0);
-    const auto scores = [&](int j) {  // S and dP of inner tile j
-      const int st = j % S::kStages, buf = j & 1;
-      if (!tc_wait_warp(&y_full[st], j / S::kStages & 1)) return false;
-      if (!KEYS) {
-        // keys that all queries leave out: what they hold must not reach dq, where 0 times NaN
-        // would be added
-        const int key = (t0 + j) * kInner;
-        if (n - key < kInner || key_mask)
-          clear_rows<S::kBoxes>(sm_y + st * 2 * S::kInnerBytes, kInner, n - key,
-                                key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
-      }
-      if (elect_one()) {
-        const uint64_t in1 = desc_y + st * (2 * S::kInnerBytes / 16),
-                       in2 = in1 + S::kInnerBytes / 16;
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-          if (k < steps)
-            tc_mma_ss(tm_s + buf * 64, desc_x1 + (k / 4) * (kOuter * 8) + (k % 4) * 2,
-                      in1 + (k / 4) * (kInner * 8) + (k % 4) * 2, idesc_s, k > 0);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-          if (k < steps)
-            tc_mma_ss(tm_dp + buf * 64, desc_x2 + (k / 4) * (kOuter * 8) + (k % 4) * 2,
-                      in2 + (k / 4) * (kInner * 8) + (k % 4) * 2, idesc_s, k > 0);
-        tc_commit(&sp_full[buf]);
-      }
-      __syncwarp();
-      return true;
-    };
-    ok = ok && scores(0) && (count < 2 || scores(1));
-    for (int j = 0; ok && j < count; ++j) {
-      const int st = j % S::kStages, buf = j & 1;
-      ok = tc_wait_warp(&ready[buf], j / 2 & 1);
-      if (!ok) break;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t in1 = desc_yt + st * (2 * S::kInnerBytes / 16),
-                       in2 = in1 + S::kInnerBytes / 16;
-        if (KEYS) {
-#pragma unroll
-          for (int k = 0; k < kInner / 16; ++k)
-            tc_mma_ts(tm_acc2, tm_s + buf * 64 + k * 8, in2 + k * 128, idesc_acc, j > 0 || k > 0);
-        }
-#pragma unroll
-        for (int k = 0; k < kInner / 16; ++k)
-          tc_mma_ts(tm_acc1, tm_dp + buf * 64 + k * 8, in1 + k * 128, idesc_acc, j > 0 || k > 0);
-        tc_commit(&y_free[st]);
-        if (j + 1 == count) tc_commit(&acc_full);
-      }
-      __syncwarp();
-      if (j + 2 < count) ok = scores(j + 2);
-    }
-    if (!ok && count > 0) gave_up = 1;
-  } else {
+  // Tensor memory: S, dP, the sums, P and dS (in S's and dP's columns unless kOwnP). The 16-bit
+  // numbers of warpgroup w's 64 inner columns take 32 columns from w * kHalf on.
+  constexpr unsigned kHalf = S::kOwnP ? 32 : 64;
+  const unsigned tm_s = tmem, tm_dp = tmem + 128, tm_acc1 = tmem + 256,
+                 tm_acc2 = tmem + 256 + DP;
+  const unsigned tm_p = S::kOwnP ? tmem + 384 : tm_s, tm_ds = S::kOwnP ? tmem + 448 : tm_dp;
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMathRegs));
     // ---- P and dS: one thread for each outer row ----
     const int wg = warp / 4, row = threadIdx.x % 128, x = x0 + row;
     const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
@@ -257,75 +250,101 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       alive = below(n - x0, warp % 4);
       if (key_mask) alive &= a.bits[b * a.bits_b + x0 / 32 + warp % 4];
     } else {
-      if (x < a.Lq) mine = p.stats[((long long)b * a.Hq + ho) * p.lq_pad + x];
+      if (x < a.Lq) {
+        const float* tile = p.stats + (((long long)b * a.Hq + ho) * p.lq_pad + x0) * 2 + row;
+        mine = make_float2(tile[0], tile[kInner]);
+      }
       if (a.bits)
         keep_row = a.bits + b * a.bits_b + ho * a.bits_h + (long long)min(x, a.Lq - 1) * a.bits_q;
     }
+    const unsigned my_s = tm_s + lanes + wg * 64, my_dp = tm_dp + lanes + wg * 64,
+                   my_p = tm_p + lanes + wg * kHalf, my_ds = tm_ds + lanes + wg * kHalf;
     bool ok = true;
-    for (int j = wg; j < count; j += 2) {
+    for (int j = 0; j < count; ++j) {
       const int st = j % S::kStages, t = t0 + j;
-      ok = tc_wait_warp(&sp_full[wg], j / 2 & 1);
-      if (!ok) break;
-      // the statistics came by the copy engine: their own barrier makes them visible
-      if (KEYS) ok = tc_wait_warp(&y_full[st], j / S::kStages & 1);
-      if (!ok) break;
-      tc_fence_after();
-      const int y0 = (KEYS ? t % q_tiles : t) * kInner;
-      const bool hidden = a.bits || (KEYS ? x0 + kOuter > n : y0 + kInner > n);
+      const int y0 = (KEYS ? t % q_tiles : t) * kInner + wg * 64;  // first of this thread's columns
+      const bool hidden = a.bits || (KEYS ? x0 + kOuter > n : y0 + 64 > n);
+      unsigned keep[2] = {~0u, ~0u};
+      if (hidden) {
 #pragma unroll
-      for (int h = 0; h < kInner; h += 32) {
-        unsigned s[32], dp[32], pp[16], ds[16];
-        tc_ld32(tm_s + wg * 64 + lanes + h, s);
-        tc_ld32(tm_dp + wg * 64 + lanes + h, dp);
-        tc_wait_ld();
-        if (hidden) {
-          unsigned keep;  // of the thread's 32 scores
+        for (int w = 0; w < 2; ++w) {
           if (KEYS) {
-            keep = alive >> lane & 1u ? ~0u : 0u;
+            keep[w] = alive >> lane & 1u ? ~0u : 0u;
             if (a.bits && !key_mask) {
-              // lane k has the word of query y0 + h + k for the warp's 32 keys; each lane gathers
-              // its own key's bit of all 32
+              // lane k has the word of query y0 + 32 w + k for the warp's 32 keys; each lane
+              // gathers its own key's bit of all 32
               const int head = ho * shared_heads + t / q_tiles;
               const unsigned word =
                   a.bits[b * a.bits_b + head * a.bits_h +
-                         (long long)min(y0 + h + lane, a.Lq - 1) * a.bits_q + x0 / 32 + warp % 4];
-              unsigned mine = 0;
+                         (long long)min(y0 + 32 * w + lane, a.Lq - 1) * a.bits_q + x0 / 32 +
+                         warp % 4];
+              unsigned column = 0;
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                mine |= (__shfl_sync(~0u, word, k) >> lane & 1u) << k;
-              keep &= mine;
+                column |= (__shfl_sync(~0u, word, k) >> lane & 1u) << k;
+              keep[w] &= column;
             }
           } else {
-            keep = below(n - y0, h / 32);
-            if (keep_row) keep &= keep_row[(y0 + h) / 32];
+            keep[w] = below(n - y0, w);
+            if (keep_row) keep[w] &= keep_row[y0 / 32 + w];
           }
-          // no probability, and 0 times what the value product holds there, NaN included, is 0
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (!(keep >> k & 1u)) s[k] = c < 0.0f ? 0x7f800000u : kMinusInf, dp[k] = 0u;
+        }
+      }
+      ok = tc_wait_warp(&s_full, j & 1);
+      // the statistics came by the copy engine: their own barrier makes them visible
+      if (KEYS && ok) ok = tc_wait_warp(&y_full[st], j / S::kStages & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const unsigned stat = sm_stats + st * kInner * 8 + wg * 64 * 4;
+      unsigned pr[64], dp[64];  // S, then P in 32 bits; dP
+      tc_ld32(my_s, pr);
+      tc_ld32(my_s + 32, pr + 32);
+      if constexpr (S::kOwnP) {
+        tc_ld32(my_dp, dp);
+        tc_ld32(my_dp + 32, dp + 32);
+        tc_wait_ld();
+        tc_fence_before();
+        mbar_arrive_warp(&s_read);  // the next scores may overwrite these
+        if (hidden) hide(keep, c < 0.0f, pr, dp);
+        if (j > 0) {  // the products that read the P and dS before are over
+          ok = tc_wait_warp(&acc_done, (j - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
         }
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          float4 st2;  // lse and delta of inner rows h + k, h + k + 1
-          if (KEYS)
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(st2.x), "=f"(st2.y), "=f"(st2.z), "=f"(st2.w)
-                         : "r"(sm_stats + st * kInner * 8 + (h + k) * 8));
-          else
-            st2 = make_float4(mine.x, mine.y, mine.x, mine.y);
-          const float p0 = fast_exp2(fmaf(__uint_as_float(s[k]), c, -st2.x));
-          const float p1 = fast_exp2(fmaf(__uint_as_float(s[k + 1]), c, -st2.z));
-          const float d0 = p0 * ((__uint_as_float(dp[k]) - st2.y) * PS::kDs);
-          const float d1 = p1 * ((__uint_as_float(dp[k + 1]) - st2.w) * PS::kDs);
-          if (KEYS) pp[k / 2] = pack2<T>(p0, p1);
-          ds[k / 2] = pack2<T>(d0, d1);
+        for (int h = 0; h < 64; h += 32) {
+          probabilities<KEYS>(pr + h, c, stat + h * 4, mine.x);
+          if (KEYS) store_packed<T>(my_p + h / 2, pr + h);
+          differences<KEYS>(pr + h, dp + h, stat + kInner * 4 + h * 4, mine.y, PS::kDs);
+          store_packed<T>(my_ds + h / 2, pr + h);
         }
-        if (KEYS) tc_st16(tm_s + wg * 64 + lanes + h / 2, pp);
-        tc_st16(tm_dp + wg * 64 + lanes + h / 2, ds);
+      } else {
+        tc_wait_ld();
+        if (hidden) hide(keep, c < 0.0f, pr, dp);
+#pragma unroll
+        for (int h = 0; h < 64; h += 32) {
+          probabilities<KEYS>(pr + h, c, stat + h * 4, mine.x);
+          store_packed<T>(my_p + h / 2, pr + h);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive_warp(&p_ready);
+        ok = tc_wait_warp(&dp_full, j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        tc_ld32(my_dp, dp);
+        tc_ld32(my_dp + 32, dp + 32);
+        tc_wait_ld();
+        if (hidden) hide(keep, c < 0.0f, nullptr, dp);
+#pragma unroll
+        for (int h = 0; h < 64; h += 32) {
+          differences<KEYS>(pr + h, dp + h, stat + kInner * 4 + h * 4, mine.y, PS::kDs);
+          store_packed<T>(my_ds + h / 2, pr + h);
+        }
       }
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive_warp(&ready[wg]);
+      mbar_arrive_warp(&ds_ready);
     }
     if (ok && count > 0) ok = tc_wait_warp(&acc_full, 0);
     if (!ok) gave_up = 1;
@@ -367,6 +386,141 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           *reinterpret_cast<float4*>(out + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
         }
       }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
+    if (warp == 9) {
+      // ---- copies ----
+      if (lane == 0 && count > 0) {
+        mbar_arrive_expect_tx(&x_full, 2 * S::kOuterBytes);
+        for (int x = 0; x < S::kBoxes; ++x) {
+          tma_load_4d(sm_x1 + x * kOuter * 128, &map_x1, x * 64, x0, ho * p.x1h, b * p.x1b, &x_full);
+          tma_load_4d(sm_x2 + x * kOuter * 128, &map_x2, x * 64, x0, ho * p.x2h, b * p.x2b, &x_full);
+        }
+        for (int j = 0; j < count; ++j) {
+          const int st = j % S::kStages;
+          if (!tc_wait(&y_free[st], (j / S::kStages & 1) ^ 1)) { gave_up = 1; break; }
+          const int t = t0 + j;
+          const int head = KEYS ? ho * shared_heads + t / q_tiles : ho / shared_heads;
+          const int row = (KEYS ? t % q_tiles : t) * kInner;
+          const unsigned dst = sm_y + st * 2 * S::kInnerBytes;
+          mbar_arrive_expect_tx(&y_full[st], 2 * S::kInnerBytes + (KEYS ? kInner * 8 : 0));
+          for (int x = 0; x < S::kBoxes; ++x) {
+            tma_load_4d(dst + x * kInner * 128, &map_y1, x * 64, row, head * p.y1h, b * p.y1b,
+                        &y_full[st]);
+            tma_load_4d(dst + S::kInnerBytes + x * kInner * 128, &map_y2, x * 64, row, head * p.y2h,
+                        b * p.y2b, &y_full[st]);
+          }
+          if (KEYS)
+            bulk_load(sm_stats + st * kInner * 8,
+                      p.stats + (((long long)b * a.Hq + head) * p.lq_pad + row) * 2, kInner * 8,
+                      &y_full[st]);
+        }
+      }
+    } else if (warp == 8 || (warp == 10 && S::kOwnP)) {
+      // ---- products ----
+      const int steps = (a.D + 15) / 16;
+      const unsigned idesc_s = tc_idesc<T>(kInner, false);
+      const unsigned idesc_acc = tc_idesc<T>(steps * 16, true);
+      // descriptor units are 16 bytes; y is read along its rows and across them
+      const uint64_t desc_x1 = tc_desc(sm_x1, 16), desc_x2 = tc_desc(sm_x2, 16),
+                     desc_y = tc_desc(sm_y, 16), desc_yt = tc_desc(sm_y, kInner * 128);
+      // S (second = 0) or dP (1) of inner tile j
+      const auto scores = [&](int j, int second) {
+        const uint64_t in = desc_y + (j % S::kStages * 2 + second) * (S::kInnerBytes / 16);
+        const uint64_t out = second ? desc_x2 : desc_x1;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+          if (k < steps)
+            tc_mma_ss(second ? tm_dp : tm_s, out + (k / 4) * (kOuter * 8) + (k % 4) * 2,
+                      in + (k / 4) * (kInner * 8) + (k % 4) * 2, idesc_s, k > 0);
+      };
+      // acc2 += P y2 (second = 1) or acc1 += dS y1 (0)
+      const auto sums = [&](int j, int second) {
+        const uint64_t in = desc_yt + (j % S::kStages * 2 + second) * (S::kInnerBytes / 16);
+#pragma unroll
+        for (int k = 0; k < kInner / 16; ++k)
+          tc_mma_ts(second ? tm_acc2 : tm_acc1,
+                    (second ? tm_p : tm_ds) + (k / 4) * kHalf + (k % 4) * 8, in + k * 128,
+                    idesc_acc, j > 0 || k > 0);
+      };
+      const auto arrived = [&](int j) {  // the inner tile
+        if (!tc_wait_warp(&y_full[j % S::kStages], j / S::kStages & 1)) return false;
+        if (!KEYS && warp == 8) {
+          // keys that all queries leave out: what they hold must not reach dq, where 0 times NaN
+          // would be added
+          const int key = (t0 + j) * kInner;
+          if (n - key < kInner || key_mask)
+            clear_rows<S::kBoxes>(sm_y + j % S::kStages * 2 * S::kInnerBytes, kInner, n - key,
+                                  key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
+        }
+        return true;
+      };
+      const auto when = [&](uint64_t* bar, int j) {
+        const bool done = tc_wait_warp(bar, j & 1);
+        tc_fence_after();
+        return done;
+      };
+      bool ok = count > 0;
+      if (warp == 8) ok = ok && tc_wait_warp(&x_full, 0);
+      if (S::kOwnP && warp == 8) {
+        for (int j = 0; ok && j < count; ++j) {
+          ok = arrived(j) && (j == 0 || when(&s_read, j - 1));
+          if (ok && elect_one()) {
+            scores(j, 0);
+            scores(j, 1);
+            tc_commit(&s_full);
+          }
+          __syncwarp();
+        }
+      } else if (S::kOwnP) {
+        for (int j = 0; ok && j < count; ++j) {
+          ok = arrived(j) && when(&ds_ready, j);
+          if (ok && elect_one()) {
+            if (KEYS) sums(j, 1);
+            sums(j, 0);
+            tc_commit(&acc_done);
+            tc_commit(&y_free[j % S::kStages]);
+            if (j + 1 == count) tc_commit(&acc_full);
+          }
+          __syncwarp();
+        }
+      } else {
+        ok = ok && arrived(0);
+        if (ok && elect_one()) {
+          scores(0, 0);
+          tc_commit(&s_full);
+          scores(0, 1);
+          tc_commit(&dp_full);
+        }
+        __syncwarp();
+        for (int j = 0; ok && j < count; ++j) {
+          ok = when(&p_ready, j);
+          if (ok && elect_one()) sums(j, 1);
+          __syncwarp();
+          if (j + 1 < count) {
+            ok = ok && arrived(j + 1);
+            if (ok && elect_one()) {
+              scores(j + 1, 0);
+              tc_commit(&s_full);
+            }
+            __syncwarp();
+          }
+          ok = ok && when(&ds_ready, j);
+          if (ok && elect_one()) {
+            sums(j, 0);
+            tc_commit(&y_free[j % S::kStages]);
+            if (j + 1 < count) {
+              scores(j + 1, 1);
+              tc_commit(&dp_full);
+            } else {
+              tc_commit(&acc_full);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok && count > 0) gave_up = 1;
     }
   }
   tc_fence_before();
@@ -412,12 +566,12 @@ struct BackwardPlan {
   size_t bytes = 0;
 };
 
-// The inner tiles are split where the outer tiles leave SMs idle, each split with at least four.
+// The inner tiles are split where the outer tiles leave SMs idle, each split with at least two.
 static BackwardPlan backward_plan(const gs_attention_args& a) {
   BackwardPlan plan;
   const auto tiles = [](long long rows, long long tile) { return (rows + tile - 1) / tile; };
   const auto splits = [](long long ctas, long long inner) {
-    return (int)std::max(1ll, std::min(kSms / std::max(1ll, ctas), inner / 4));
+    return (int)std::max(1ll, std::min(kSms / std::max(1ll, ctas), inner / 2));
   };
   plan.lq_pad = tiles(a.Lq, kInner) * kInner;
   if (a.Hkv > 0)
@@ -429,7 +583,7 @@ static BackwardPlan backward_plan(const gs_attention_args& a) {
   if (plan.query_splits > 1)
     plan.query_floats = (long long)plan.query_splits * a.B * a.Hq * a.Lq * a.D;
   // dk, dv and dq in turn use the same parts
-  plan.bytes = (size_t)(a.B * a.Hq * plan.lq_pad) * sizeof(float2) +
+  plan.bytes = (size_t)(a.B * a.Hq * plan.lq_pad) * 2 * sizeof(float) +
                (size_t)std::max(2 * plan.key_floats, plan.query_floats) * sizeof(float);
   return plan;
 }
@@ -443,11 +597,11 @@ static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&
                                    cudaStream_t stream) {
   const auto kernel = attention_backward_kernel<T, DP, KEYS>;
   const cudaError_t err = cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BackwardShared<DP>::kBytes);
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BackwardShared<DP, KEYS>::kBytes);
   if (err != cudaSuccess) return err;
   const int rows = KEYS ? p.a.Lk : p.a.Lq, heads = KEYS ? p.a.Hkv : p.a.Hq;
   const dim3 grid((rows + kOuter - 1) / kOuter * p.a.B * heads, p.splits);
-  kernel<<<grid, kBwdThreads, BackwardShared<DP>::kBytes, stream>>>(p, m[0], m[1], m[2], m[3]);
+  kernel<<<grid, kBwdThreads, BackwardShared<DP, KEYS>::kBytes, stream>>>(p, m[0], m[1], m[2], m[3]);
   return cudaGetLastError();
 }
 
@@ -475,10 +629,10 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   p.lq_pad = (int)plan.lq_pad;
   const size_t mask_bytes = attention_mask_bytes(a);
   if (const int status = attention_pack_mask(a, p.a, workspace, stream)) return status;
-  float2* stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + mask_bytes);
+  float* stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);
   p.stats = stats;
   const long long stat_rows = a.B * a.Hq * plan.lq_pad;
-  float* parts = reinterpret_cast<float*>(stats + stat_rows);
+  float* parts = stats + 2 * stat_rows;
   if (stat_rows) {
     attention_prepare_kernel<T>
         <<<(unsigned)(stat_rows / 32), 256, 0, stream>>>(p.a, p.lq_pad, stats);
