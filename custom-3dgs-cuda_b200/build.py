@@ -22,6 +22,8 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 BUILD = HERE / "_build"
 LIB = HERE / "custom_rasterizer_cuda" / "libgs3d_b200.so"
+BINDING_SRC = CSRC / "token_binding.cpp"
+BINDING = HERE / "gs3d_b200" / "_native.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -66,8 +68,39 @@ def _compile(src: Path, obj: Path, verbose: bool, extra: list[str]) -> None:
         print(res.stdout, res.stderr, flush=True)
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles the torch side of the token operators, gs3d_b200/_native.so (host code only)."""
+    newest = max(BINDING_SRC.stat().st_mtime, (INCLUDE / "gs3d_b200.h").stat().st_mtime)
+    if not force and BINDING.exists() and BINDING.stat().st_mtime >= newest:
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(nvcc()).resolve().parents[1]
+    includes = [INCLUDE, *cpp_extension.include_paths(), cuda / "include",
+                sysconfig.get_paths()["include"]]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-DTORCH_EXTENSION_NAME=_native",
+           *(a for i in includes for a in ("-isystem" if i != INCLUDE else "-I", str(i))),
+           str(BINDING_SRC), "-o", str(tmp),
+           *(f"-L{p}" for p in cpp_extension.library_paths()),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compiles every csrc/*.cu for sm_100a and links libgs3d_b200.so; returns its path."""
+    """Compiles every csrc/*.cu for sm_100a and links libgs3d_b200.so, compiles the torch binding
+    of the token operators; returns the library's path."""
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     head_time = _newest_header()
@@ -81,6 +114,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
                  or obj.stat().st_mtime < max(src.stat().st_mtime, head_time))
         if stale:
             jobs.append((src, obj))
+    binding = cf.ThreadPoolExecutor(1).submit(build_binding, force, verbose)
     if jobs:
         workers = min(len(jobs), os.cpu_count() or 4)
         with cf.ThreadPoolExecutor(workers) as pool:
@@ -98,6 +132,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    binding.result()
     return LIB
 
 

@@ -63,8 +63,13 @@ struct BackwardShared {
   static constexpr int kOuterBytes = kBoxes * kOuter * 128;
   static constexpr int kInnerBytes = kBoxes * kInner * 128;
   static constexpr bool kOwnP = !(KEYS && DP == 128);  // P and dS have their own columns
-  static constexpr int kStages = DP == 64 ? 4 : 2;
-  static constexpr int kBytes = 1024 + 2 * kOuterBytes + kStages * (2 * kInnerBytes + kInner * 8);
+  // Tiles of y1 and of y2 in shared memory: what 227 KB hold. dq needs y2 (v) for dP alone and
+  // gives it up a tile earlier than y1 (k).
+  static constexpr int kStages1 = DP == 64 ? 4 : KEYS ? 2 : 3;
+  static constexpr int kStages2 = DP == 64 ? 4 : 2;
+  static constexpr int kStatBytes = KEYS ? kInner * 8 : 0;  // beside each y1
+  static constexpr int kBytes = 1024 + 2 * kOuterBytes + (kStages1 + kStages2) * kInnerBytes +
+                                kStages1 * kStatBytes;
 };
 
 // P is formed 2^kLog2 times larger; kDs brings dS back where its type cannot hold that, kAcc1 and
@@ -193,13 +198,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   using S = BackwardShared<DP, KEYS>;
   using PS = ProbabilityScale<T>;
   extern __shared__ unsigned char raw[];
-  __shared__ uint64_t x_full, y_full[S::kStages], y_free[S::kStages], s_full, s_read, dp_full,
-      p_ready, ds_ready, acc_done, acc_full;
+  __shared__ uint64_t x_full, y1_full[S::kStages1], y1_free[S::kStages1], y2_full[S::kStages2],
+      y2_free[S::kStages2], s_full, s_read, dp_full, p_ready, ds_ready, acc_done, acc_full;
   __shared__ unsigned tmem_slot;
   __shared__ volatile int gave_up;
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
-  const unsigned sm_x1 = base, sm_x2 = sm_x1 + S::kOuterBytes, sm_y = sm_x2 + S::kOuterBytes,
-                 sm_stats = sm_y + S::kStages * 2 * S::kInnerBytes;
+  const unsigned sm_x1 = base, sm_x2 = sm_x1 + S::kOuterBytes, sm_y1 = sm_x2 + S::kOuterBytes,
+                 sm_y2 = sm_y1 + S::kStages1 * S::kInnerBytes,
+                 sm_stats = sm_y2 + S::kStages2 * S::kInnerBytes;
   const int warp = warp_uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
   const AttentionParams& a = p.a;
   const int shared_heads = a.Hq / a.Hkv;
@@ -218,9 +224,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     gave_up = 0;
     mbar_init(&x_full, 1);
     mbar_init(&acc_full, 1);
-    for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&y_full[i], 1);
-      mbar_init(&y_free[i], 1);
+    for (int i = 0; i < S::kStages1; ++i) {
+      mbar_init(&y1_full[i], 1);
+      mbar_init(&y1_free[i], 1);
+    }
+    for (int i = 0; i < S::kStages2; ++i) {
+      mbar_init(&y2_full[i], 1);
+      mbar_init(&y2_free[i], 1);
     }
     for (uint64_t* bar : {&s_full, &dp_full, &acc_done}) mbar_init(bar, 1);
     for (uint64_t* bar : {&s_read, &p_ready, &ds_ready}) mbar_init(bar, 8);
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                    my_p = tm_p + lanes + wg * kHalf, my_ds = tm_ds + lanes + wg * kHalf;
     bool ok = true;
     for (int j = 0; j < count; ++j) {
-      const int st = j % S::kStages, t = t0 + j;
+      const int st = j % S::kStages1, t = t0 + j;
       const int y0 = (KEYS ? t % q_tiles : t) * kInner + wg * 64;  // first of this thread's columns
       const bool hidden = a.bits || (KEYS ? x0 + kOuter > n : y0 + 64 > n);
       unsigned keep[2] = {~0u, ~0u};
@@ -292,10 +302,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       ok = tc_wait_warp(&s_full, j & 1);
       // the statistics came by the copy engine: their own barrier makes them visible
-      if (KEYS && ok) ok = tc_wait_warp(&y_full[st], j / S::kStages & 1);
+      if (KEYS && ok) ok = tc_wait_warp(&y1_full[st], j / S::kStages1 & 1);
       if (!ok) break;
       tc_fence_after();
-      const unsigned stat = sm_stats + st * kInner * 8 + wg * 64 * 4;
+      const unsigned stat = sm_stats + st * S::kStatBytes + wg * 64 * 4;
       unsigned pr[64], dp[64];  // S, then P in 32 bits; dP
       tc_ld32(my_s, pr);
       tc_ld32(my_s + 32, pr + 32);
@@ -306,18 +316,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_before();
         mbar_arrive_warp(&s_read);  // the next scores may overwrite these
         if (hidden) hide(keep, c < 0.0f, pr, dp);
-        if (j > 0) {  // the products that read the P and dS before are over
-          ok = tc_wait_warp(&acc_done, (j - 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
-        }
 #pragma unroll
         for (int h = 0; h < 64; h += 32) {
           probabilities<KEYS>(pr + h, c, stat + h * 4, mine.x);
+          if (h == 0 && j > 0) {  // the products that read the P and dS before are over
+            ok = tc_wait_warp(&acc_done, (j - 1) & 1);
+            tc_fence_after();
+          }
           if (KEYS) store_packed<T>(my_p + h / 2, pr + h);
           differences<KEYS>(pr + h, dp + h, stat + kInner * 4 + h * 4, mine.y, PS::kDs);
           store_packed<T>(my_ds + h / 2, pr + h);
         }
+        if (!ok) break;
       } else {
         tc_wait_ld();
         if (hidden) hide(keep, c < 0.0f, pr, dp);
@@ -398,23 +408,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tma_load_4d(sm_x2 + x * kOuter * 128, &map_x2, x * 64, x0, ho * p.x2h, b * p.x2b, &x_full);
         }
         for (int j = 0; j < count; ++j) {
-          const int st = j % S::kStages;
-          if (!tc_wait(&y_free[st], (j / S::kStages & 1) ^ 1)) { gave_up = 1; break; }
           const int t = t0 + j;
           const int head = KEYS ? ho * shared_heads + t / q_tiles : ho / shared_heads;
-          const int row = (KEYS ? t % q_tiles : t) * kInner;
-          const unsigned dst = sm_y + st * 2 * S::kInnerBytes;
-          mbar_arrive_expect_tx(&y_full[st], 2 * S::kInnerBytes + (KEYS ? kInner * 8 : 0));
-          for (int x = 0; x < S::kBoxes; ++x) {
-            tma_load_4d(dst + x * kInner * 128, &map_y1, x * 64, row, head * p.y1h, b * p.y1b,
-                        &y_full[st]);
-            tma_load_4d(dst + S::kInnerBytes + x * kInner * 128, &map_y2, x * 64, row, head * p.y2h,
-                        b * p.y2b, &y_full[st]);
-          }
+          const int y = (KEYS ? t % q_tiles : t) * kInner;
+          const int st1 = j % S::kStages1, st2 = j % S::kStages2;
+          if (!tc_wait(&y1_free[st1], (j / S::kStages1 & 1) ^ 1)) { gave_up = 1; break; }
+          mbar_arrive_expect_tx(&y1_full[st1], S::kInnerBytes + S::kStatBytes);
+          for (int x = 0; x < S::kBoxes; ++x)
+            tma_load_4d(sm_y1 + st1 * S::kInnerBytes + x * kInner * 128, &map_y1, x * 64, y,
+                        head * p.y1h, b * p.y1b, &y1_full[st1]);
           if (KEYS)
-            bulk_load(sm_stats + st * kInner * 8,
-                      p.stats + (((long long)b * a.Hq + head) * p.lq_pad + row) * 2, kInner * 8,
-                      &y_full[st]);
+            bulk_load(sm_stats + st1 * S::kStatBytes,
+                      p.stats + (((long long)b * a.Hq + head) * p.lq_pad + y) * 2, S::kStatBytes,
+                      &y1_full[st1]);
+          if (!tc_wait(&y2_free[st2], (j / S::kStages2 & 1) ^ 1)) { gave_up = 1; break; }
+          mbar_arrive_expect_tx(&y2_full[st2], S::kInnerBytes);
+          for (int x = 0; x < S::kBoxes; ++x)
+            tma_load_4d(sm_y2 + st2 * S::kInnerBytes + x * kInner * 128, &map_y2, x * 64, y,
+                        head * p.y2h, b * p.y2b, &y2_full[st2]);
         }
       }
     } else if (warp == 8 || (warp == 10 && S::kOwnP)) {
@@ -424,10 +435,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const unsigned idesc_acc = tc_idesc<T>(steps * 16, true);
       // descriptor units are 16 bytes; y is read along its rows and across them
       const uint64_t desc_x1 = tc_desc(sm_x1, 16), desc_x2 = tc_desc(sm_x2, 16),
-                     desc_y = tc_desc(sm_y, 16), desc_yt = tc_desc(sm_y, kInner * 128);
+                     desc_y1 = tc_desc(sm_y1, 16), desc_y2 = tc_desc(sm_y2, 16),
+                     desc_y1t = tc_desc(sm_y1, kInner * 128),
+                     desc_y2t = tc_desc(sm_y2, kInner * 128);
+      const auto in1 = [](int j) { return j % S::kStages1 * (S::kInnerBytes / 16); };
+      const auto in2 = [](int j) { return j % S::kStages2 * (S::kInnerBytes / 16); };
       // S (second = 0) or dP (1) of inner tile j
       const auto scores = [&](int j, int second) {
-        const uint64_t in = desc_y + (j % S::kStages * 2 + second) * (S::kInnerBytes / 16);
+        const uint64_t in = second ? desc_y2 + in2(j) : desc_y1 + in1(j);
         const uint64_t out = second ? desc_x2 : desc_x1;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
@@ -437,24 +452,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       };
       // acc2 += P y2 (second = 1) or acc1 += dS y1 (0)
       const auto sums = [&](int j, int second) {
-        const uint64_t in = desc_yt + (j % S::kStages * 2 + second) * (S::kInnerBytes / 16);
+        const uint64_t in = second ? desc_y2t + in2(j) : desc_y1t + in1(j);
 #pragma unroll
         for (int k = 0; k < kInner / 16; ++k)
           tc_mma_ts(second ? tm_acc2 : tm_acc1,
                     (second ? tm_p : tm_ds) + (k / 4) * kHalf + (k % 4) * 8, in + k * 128,
                     idesc_acc, j > 0 || k > 0);
       };
-      const auto arrived = [&](int j) {  // the inner tile
-        if (!tc_wait_warp(&y_full[j % S::kStages], j / S::kStages & 1)) return false;
+      const auto arrived1 = [&](int j) {
+        const int st = j % S::kStages1;
+        if (!tc_wait_warp(&y1_full[st], j / S::kStages1 & 1)) return false;
         if (!KEYS && warp == 8) {
           // keys that all queries leave out: what they hold must not reach dq, where 0 times NaN
           // would be added
           const int key = (t0 + j) * kInner;
           if (n - key < kInner || key_mask)
-            clear_rows<S::kBoxes>(sm_y + j % S::kStages * 2 * S::kInnerBytes, kInner, n - key,
+            clear_rows<S::kBoxes>(sm_y1 + st * S::kInnerBytes, kInner, n - key,
                                   key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
         }
         return true;
+      };
+      const auto arrived2 = [&](int j) {
+        return tc_wait_warp(&y2_full[j % S::kStages2], j / S::kStages2 & 1);
       };
       const auto when = [&](uint64_t* bar, int j) {
         const bool done = tc_wait_warp(bar, j & 1);
@@ -465,28 +484,33 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (warp == 8) ok = ok && tc_wait_warp(&x_full, 0);
       if (S::kOwnP && warp == 8) {
         for (int j = 0; ok && j < count; ++j) {
-          ok = arrived(j) && (j == 0 || when(&s_read, j - 1));
+          ok = arrived1(j) && (j == 0 || when(&s_read, j - 1));
+          if (ok && elect_one()) scores(j, 0);
+          __syncwarp();
+          ok = ok && arrived2(j);
           if (ok && elect_one()) {
-            scores(j, 0);
             scores(j, 1);
             tc_commit(&s_full);
+            if (!KEYS) tc_commit(&y2_free[j % S::kStages2]);
           }
           __syncwarp();
         }
       } else if (S::kOwnP) {
         for (int j = 0; ok && j < count; ++j) {
-          ok = arrived(j) && when(&ds_ready, j);
+          ok = tc_wait_warp(&y1_full[j % S::kStages1], j / S::kStages1 & 1) &&
+               (!KEYS || arrived2(j)) && when(&ds_ready, j);
           if (ok && elect_one()) {
             if (KEYS) sums(j, 1);
             sums(j, 0);
             tc_commit(&acc_done);
-            tc_commit(&y_free[j % S::kStages]);
+            if (KEYS) tc_commit(&y2_free[j % S::kStages2]);
+            tc_commit(&y1_free[j % S::kStages1]);
             if (j + 1 == count) tc_commit(&acc_full);
           }
           __syncwarp();
         }
       } else {
-        ok = ok && arrived(0);
+        ok = ok && arrived1(0) && arrived2(0);
         if (ok && elect_one()) {
           scores(0, 0);
           tc_commit(&s_full);
@@ -496,20 +520,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
         for (int j = 0; ok && j < count; ++j) {
           ok = when(&p_ready, j);
-          if (ok && elect_one()) sums(j, 1);
+          if (ok && elect_one()) {
+            sums(j, 1);  // dP of this tile was issued before: y2 is free after both
+            tc_commit(&y2_free[j % S::kStages2]);
+          }
           __syncwarp();
           if (j + 1 < count) {
-            ok = ok && arrived(j + 1);
+            ok = ok && arrived1(j + 1);
             if (ok && elect_one()) {
               scores(j + 1, 0);
               tc_commit(&s_full);
             }
             __syncwarp();
+            ok = ok && arrived2(j + 1);
           }
           ok = ok && when(&ds_ready, j);
           if (ok && elect_one()) {
             sums(j, 0);
-            tc_commit(&y_free[j % S::kStages]);
+            tc_commit(&y1_free[j % S::kStages1]);
             if (j + 1 < count) {
               scores(j + 1, 1);
               tc_commit(&dp_full);
