@@ -90,6 +90,7 @@ struct ProbabilityScale<__half> {
 template <typename T>
 __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams a, int lq_pad,
                                                                 float* stats) {
+  let_next_start();
   const int sub = threadIdx.x % 8;
   const long long at = (long long)blockIdx.x * 32 + threadIdx.x / 8;
   const int i = (int)(at % lq_pad), h = (int)(at / lq_pad % a.Hq), b = (int)(at / lq_pad / a.Hq);
@@ -236,6 +237,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (uint64_t* bar : {&s_read, &p_ready, &ds_ready}) mbar_init(bar, 8);
   }
   if (warp == 8) tc_alloc(&tmem_slot, 512);
+  // dk and dv need the rows' statistics and with them the packed mask; the CTAs of dq that start
+  // beside the last of dk's and dv's then find both, and only end after them
+  if (KEYS) wait_for_previous();
+  let_next_start();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -566,6 +571,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tc_fence_after();
     tc_free(tmem, 512);
   }
+  if (!KEYS) wait_for_previous();
 }
 
 // out[b, row, h] = the sum of the splits' parts, in order.
@@ -622,13 +628,16 @@ size_t attention_backward_workspace(const gs_attention_args& a) {
 
 template <typename T, int DP, bool KEYS>
 static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&m)[4],
-                                   cudaStream_t stream) {
+                                   bool overlapped, cudaStream_t stream) {
   const auto kernel = attention_backward_kernel<T, DP, KEYS>;
   const cudaError_t err = cudaFuncSetAttribute(
       kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BackwardShared<DP, KEYS>::kBytes);
   if (err != cudaSuccess) return err;
   const int rows = KEYS ? p.a.Lk : p.a.Lq, heads = KEYS ? p.a.Hkv : p.a.Hq;
   const dim3 grid((rows + kOuter - 1) / kOuter * p.a.B * heads, p.splits);
+  if (overlapped)
+    return launch_overlapped(kernel, grid, kBwdThreads, BackwardShared<DP, KEYS>::kBytes, stream, p,
+                             m[0], m[1], m[2], m[3]);
   kernel<<<grid, kBwdThreads, BackwardShared<DP, KEYS>::kBytes, stream>>>(p, m[0], m[1], m[2], m[3]);
   return cudaGetLastError();
 }
@@ -685,8 +694,8 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
     p.x1h = p.x2h = a.Hkv > 1, p.y1h = p.y2h = a.Hq > 1;
     p.splits = plan.key_splits;
     p.part1 = parts, p.part2 = parts + plan.key_floats;
-    GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, true>(p, m, stream))
-                      : (launch_backward<T, 128, true>(p, m, stream)));
+    GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, true>(p, m, stat_rows > 0, stream))
+                      : (launch_backward<T, 128, true>(p, m, stat_rows > 0, stream)));
     count_launches(1u);
     if (p.splits > 1) {
       GS_CUDA(launch_add<T>(p.part1, p.splits, p.a.dk, a.Lk, a.Hkv, a.B, a.D, stream));
@@ -706,8 +715,10 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   p.x1h = p.x2h = a.Hq > 1, p.y1h = p.y2h = a.Hkv > 1;
   p.splits = plan.query_splits;
   p.part1 = parts, p.part2 = nullptr;
-  GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, false>(p, m, stream))
-                    : (launch_backward<T, 128, false>(p, m, stream)));
+  // dq starts beside the end of dk and dv, unless both use the parts in turn
+  const bool beside = a.Lk > 0 && (plan.key_splits == 1 || plan.query_splits == 1);
+  GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, false>(p, m, beside, stream))
+                    : (launch_backward<T, 128, false>(p, m, beside, stream)));
   count_launches(1u);
   if (p.splits > 1) {
     GS_CUDA(launch_add<T>(p.part1, p.splits, p.a.dq, a.Lq, a.Hq, a.B, a.D, stream));

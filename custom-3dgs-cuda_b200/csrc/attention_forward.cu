@@ -38,6 +38,7 @@ struct ForwardParams {
   float scale_log2;  // |scale| log2 e, above 0
   float lag;         // kLag in units of unscaled scores
   int negate;        // scale < 0: scores change sign first
+  int tiles;   // query tiles a CTA holds, 1 or 2
   int splits;
   int kb, kh, vb, vh, qb, qh;  // 0 where all batch items (heads) share the tensor, else 1
   float* part_out;  // [splits, B, Hq, Lq, D] where splits > 1
@@ -69,17 +70,31 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                  sm_v = sm_k + S::kStages * S::kTileBytes;
   const int warp = warp_uniform(threadIdx.x / 32);
   const AttentionParams& a = p.a;
-  const int q_blocks = (a.Lq + 2 * kTileQ - 1) / (2 * kTileQ);
-  const int q0 = blockIdx.x % q_blocks * 2 * kTileQ, bh = blockIdx.x / q_blocks;
+  const int rows_a_cta = p.tiles * kTileQ, q_blocks = (a.Lq + rows_a_cta - 1) / rows_a_cta;
+  const int q0 = blockIdx.x % q_blocks * rows_a_cta, bh = blockIdx.x / q_blocks;
   const int b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hkv);
   const int n = warp_uniform(key_count(a, b));
   const int tiles = (n + kTileK - 1) / kTileK;
   const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
   const int t1 = (int)((long long)tiles * (blockIdx.y + 1) / p.splits);
   const int count = t1 - t0;
-  const bool both = q0 + kTileQ < a.Lq;
+  const bool both = p.tiles == 2 && q0 + kTileQ < a.Lq;
 
-  if (threadIdx.x == 0) {
+  const auto load_k = [&](int j) {
+    const int st = j % S::kStages;
+    mbar_arrive_expect_tx(&k_full[st], S::kTileBytes);
+    for (int x = 0; x < S::kBoxes; ++x)
+      tma_load_4d(sm_k + st * S::kTileBytes + x * 16384, &map_k, x * 64, (t0 + j) * kTileK,
+                  hk * p.kh, b * p.kb, &k_full[st]);
+  };
+  const auto load_v = [&](int j) {
+    const int st = j % S::kStages;
+    mbar_arrive_expect_tx(&v_full[st], S::kTileBytes);
+    for (int x = 0; x < S::kBoxes; ++x)
+      tma_load_4d(sm_v + st * S::kTileBytes + x * 16384, &map_v, x * 64, (t0 + j) * kTileK,
+                  hk * p.vh, b * p.vb, &v_full[st]);
+  };
+  if (warp == 9 && threadIdx.x % 32 == 0) {
     gave_up = 0;
     mbar_init(&q_full, 1);
     for (int i = 0; i < S::kStages; ++i) {
@@ -96,7 +111,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       mbar_init(&o_done[i], 1);
       mbar_init(&o_full[i], 1);
     }
+    if (count > 0) {  // the first copies start while the other warps get ready
+      const int bq = b * p.qb, hq = h * p.qh;
+      mbar_arrive_expect_tx(&q_full, (both ? 2 : 1) * S::kTileBytes);
+      for (int t = 0; t < (both ? 2 : 1); ++t)
+        for (int x = 0; x < S::kBoxes; ++x)
+          tma_load_4d(sm_q + t * S::kTileBytes + x * 16384, &map_q, x * 64, q0 + t * kTileQ, hq, bq,
+                      &q_full);
+      for (int j = 0; j < S::kStages && j < count; ++j) {
+        load_k(j);
+        load_v(j);
+      }
+    }
   }
+  let_next_start();
   if (warp == 8) tc_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -124,10 +152,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                  : nullptr;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
+      if (a.bits) wait_for_previous();  // the kernel that packs the mask
+      uint4 keep_next = make_uint4(~0u, ~0u, ~0u, ~0u);
+      if (keep_row && count > 0) keep_next = keep_row[t0];
       for (int j = 0; j < count; ++j) {
         const int key = (t0 + j) * kTileK;
-        uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);
-        if (keep_row) keep = keep_row[t0 + j];
+        const uint4 keep = keep_next;
+        if (keep_row && j + 1 < count) keep_next = keep_row[t0 + j + 1];
         ok = tc_wait_warp(&s_full[t], j & 1);
         if (!ok) break;
         tc_fence_after();
@@ -251,34 +282,21 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 9) {
-      // ---- copies ----
-      if (threadIdx.x % 32 == 0 && count > 0) {
-        const int bq = b * p.qb, hq = h * p.qh;
-        mbar_arrive_expect_tx(&q_full, (both ? 2 : 1) * S::kTileBytes);
-        for (int t = 0; t < (both ? 2 : 1); ++t)
-          for (int x = 0; x < S::kBoxes; ++x)
-            tma_load_4d(sm_q + t * S::kTileBytes + x * 16384, &map_q, x * 64, q0 + t * kTileQ, hq, bq,
-                        &q_full);
-        for (int j = 0; j < count; ++j) {
+      // ---- copies: the first tiles are on their way ----
+      if (threadIdx.x % 32 == 0)
+        for (int j = S::kStages; j < count; ++j) {
           const int st = j % S::kStages;
           const unsigned phase = (j / S::kStages & 1) ^ 1;
-          const int key = (t0 + j) * kTileK;
           if (!tc_wait(&k_free[st], phase)) { gave_up = 1; break; }
-          mbar_arrive_expect_tx(&k_full[st], S::kTileBytes);
-          for (int x = 0; x < S::kBoxes; ++x)
-            tma_load_4d(sm_k + st * S::kTileBytes + x * 16384, &map_k, x * 64, key, hk * p.kh,
-                        b * p.kb, &k_full[st]);
+          load_k(j);
           if (!tc_wait(&v_free[st], phase)) { gave_up = 1; break; }
-          mbar_arrive_expect_tx(&v_full[st], S::kTileBytes);
-          for (int x = 0; x < S::kBoxes; ++x)
-            tma_load_4d(sm_v + st * S::kTileBytes + x * 16384, &map_v, x * 64, key, hk * p.vh,
-                        b * p.vb, &v_full[st]);
+          load_v(j);
         }
-      }
     } else if (warp == 11) {
       // ---- what v holds at keys that no query of the CTA keeps must not reach the product, which
       // would make 0 times NaN of it: those rows are set to zero before the product may read them
       const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
+      if (key_mask) wait_for_previous();
       for (int j = 0; j < count; ++j) {
         const int st = j % S::kStages, key = (t0 + j) * kTileK;
         if (!tc_wait_warp(&v_full[st], j / S::kStages & 1)) { gave_up = 1; break; }
@@ -364,56 +382,85 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   }
 }
 
-// out = sum over splits of exp(lse_s - lse) out_s: one warp for each row.
+// out = sum over splits of exp(lse_s - lse) out_s: a warp for each row, a lane for 4 of its
+// numbers; the weights of 32 splits at a time are formed by one lane each.
 template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(AttentionParams a, int splits,
+__global__ void __launch_bounds__(128) combine_kernel(AttentionParams a, int splits,
                                                       const float* part_out,
                                                       const float* part_lse) {
+  wait_for_previous();
   const int lane = threadIdx.x % 32;
-  const long long rows = (long long)a.B * a.Hq * a.Lq;
-  const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+  const unsigned rows = (unsigned)a.B * a.Hq * a.Lq;
+  const unsigned row = blockIdx.x * 4 + threadIdx.x / 32;
   if (row >= rows) return;
-  const int i = (int)(row % a.Lq), h = (int)(row / a.Lq % a.Hq), b = (int)(row / a.Lq / a.Hq);
-  float top = -INFINITY;
-  for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + row]);
+  float mine = lane < splits ? part_lse[(long long)lane * rows + row] : -INFINITY, top = mine;
+  for (int s = lane + 32; s < splits; s += 32) top = fmaxf(top, part_lse[(long long)s * rows + row]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-  float total = 0.0f;
-  if (top > -INFINITY)
-    for (int s = lane; s < splits; s += 32) total += expf(part_lse[s * rows + row] - top);
+  const float shift = top == -INFINITY ? 0.0f : top;
+  const int d = lane * 4;
+  float total = 0.0f, acc[4] = {};
+  for (int s0 = 0; s0 < splits; s0 += 32) {
+    if (s0) mine = s0 + lane < splits ? part_lse[(long long)(s0 + lane) * rows + row] : -INFINITY;
+    const float w = expf(mine - shift);
+    total += w;
+    const int n = min(32, splits - s0);
+    const float* part = part_out + ((long long)s0 * rows + row) * a.D + d;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float ws = __shfl_sync(~0u, w, s);
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (d < a.D) o = *reinterpret_cast<const float4*>(part + (long long)s * rows * a.D);
+      acc[0] = fmaf(ws, o.x, acc[0]), acc[1] = fmaf(ws, o.y, acc[1]);
+      acc[2] = fmaf(ws, o.z, acc[2]), acc[3] = fmaf(ws, o.w, acc[3]);
+    }
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-  const float lse = top > -INFINITY ? top + logf(total) : -INFINITY;
-  const int d = lane * 4;
-  float acc[4] = {};
-  if (d < a.D && lse != -INFINITY)
-    for (int s = 0; s < splits; ++s) {
-      const float ls = part_lse[s * rows + row];
-      if (ls == -INFINITY) continue;
-      const float w = expf(ls - lse);
-      const float4 o = *reinterpret_cast<const float4*>(part_out + (s * rows + row) * a.D + d);
-      acc[0] = fmaf(w, o.x, acc[0]);
-      acc[1] = fmaf(w, o.y, acc[1]);
-      acc[2] = fmaf(w, o.z, acc[2]);
-      acc[3] = fmaf(w, o.w, acc[3]);
-    }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   if (d < a.D) {
-    const uint2 w = make_uint2(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]));
-    *reinterpret_cast<uint2*>(a.out.at<T>(b, i, h) + d) = w;
+    const unsigned bh = row / (unsigned)a.Lq, i = row - bh * (unsigned)a.Lq;
+    const unsigned b = bh / (unsigned)a.Hq, h = bh - b * (unsigned)a.Hq;
+    *reinterpret_cast<uint2*>(a.out.at<T>(b, i, h) + d) = make_uint2(
+        pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
   }
-  if (a.lse && lane == 0) a.lse[row] = lse;
+  if (a.lse && lane == 0) a.lse[row] = total == 0.0f ? -INFINITY : top + logf(total);
 }
 
-// Splits of the keys: as many as fill the card's SMs once, each with at least two tiles of keys.
-static int forward_splits(const gs_attention_args& a) {
-  const long long ctas =
-      (long long)a.B * a.Hq * ((a.Lq + 2 * kTileQ - 1) / (2 * kTileQ));
-  const long long tiles = (a.Lk + kTileK - 1) / kTileK;
-  return (int)std::max(1ll, std::min(kSms / std::max(1ll, ctas), tiles / 2));
+struct ForwardPlan {
+  int tiles, splits;
+};
+
+// Query tiles a CTA and splits of the keys (each with at least two tiles of keys, and all in one
+// wave of CTAs), by the time they should take in us: waves of CTAs, each with some 4 us to begin
+// and end and, for a tile of keys, what one and two query tiles take together (measured: 1.35 and
+// 1.65 at D 64, 1.7 and 2.2 at D 128); joining splits takes another launch and the parts' way
+// through memory.
+static ForwardPlan forward_plan(const gs_attention_args& a) {
+  const double heads = (double)a.B * a.Hq;
+  const int q_tiles = (a.Lq + kTileQ - 1) / kTileQ, key_tiles = (a.Lk + kTileK - 1) / kTileK;
+  const double part_us = heads * a.Lq * a.D * 8.0 / 3e6;
+  ForwardPlan best{2, 1};
+  double least = 1e30;
+  for (int tiles = 2; tiles >= 1; --tiles) {
+    const double ctas = heads * ((q_tiles + tiles - 1) / tiles);
+    const double step = a.D <= 64 ? (tiles == 2 ? 1.65 : 1.35) : (tiles == 2 ? 2.2 : 1.7);
+    for (int splits = 1; splits == 1 || (splits <= key_tiles / 2 && ctas * splits <= kSms);
+         ++splits) {
+      const double us = std::ceil(ctas * splits / kSms) *
+                            (4.0 + step * ((key_tiles + splits - 1) / splits)) +
+                        (splits > 1 ? 4.0 + part_us * splits : 0.0);
+      if (us < least) {
+        least = us;
+        best = {tiles, splits};
+      }
+    }
+  }
+  return best;
 }
 
 size_t attention_forward_workspace(const gs_attention_args& a) {
-  const long long splits = forward_splits(a), rows = (long long)a.B * a.Hq * a.Lq;
+  const long long splits = forward_plan(a).splits, rows = (long long)a.B * a.Hq * a.Lq;
   return attention_mask_bytes(a) +
          (splits > 1 ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0);
 }
@@ -426,7 +473,10 @@ static cudaError_t launch_forward(const ForwardParams& p, const CUtensorMap& q,
   const cudaError_t err = cudaFuncSetAttribute(
       kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ForwardShared<DP>::kBytes);
   if (err != cudaSuccess) return err;
-  const dim3 grid((p.a.Lq + 2 * kTileQ - 1) / (2 * kTileQ) * p.a.B * p.a.Hq, p.splits);
+  const int rows = p.tiles * kTileQ;
+  const dim3 grid((p.a.Lq + rows - 1) / rows * p.a.B * p.a.Hq, p.splits);
+  if (p.a.bits)
+    return launch_overlapped(kernel, grid, kFwdThreads, ForwardShared<DP>::kBytes, stream, p, q, k, v);
   kernel<<<grid, kFwdThreads, ForwardShared<DP>::kBytes, stream>>>(p, q, k, v);
   return cudaGetLastError();
 }
@@ -435,8 +485,8 @@ template <typename T>
 static cudaError_t launch_combine(const AttentionParams& a, int splits, const float* out,
                                   const float* lse, cudaStream_t stream) {
   const long long rows = (long long)a.B * a.Hq * a.Lq;
-  combine_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(a, splits, out, lse);
-  return cudaGetLastError();
+  return launch_overlapped(combine_kernel<T>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, a,
+                           splits, out, lse);
 }
 
 cudaError_t attention_combine(const gs_attention_args& args, int splits, const float* out,
@@ -454,7 +504,9 @@ int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t 
   p.scale_log2 = magnitude * 1.4426950408889634f;
   p.lag = std::min(kLag / p.scale_log2, 1e30f);
   p.negate = a.scale < 0.0f;
-  p.splits = forward_splits(a);
+  const ForwardPlan plan = forward_plan(a);
+  p.tiles = plan.tiles;
+  p.splits = plan.splits;
   const size_t mask_bytes = attention_mask_bytes(a);
   if (const int status = attention_pack_mask(a, p.a, workspace, stream)) return status;
   p.part_out = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);

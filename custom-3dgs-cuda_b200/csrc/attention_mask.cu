@@ -3,7 +3,7 @@
 // A thread of those kernels holds one query's scores of 128 keys: as bytes its part of the mask
 // would be 128 loads that no two lanes share, in an order that no alignment helps (a mask of 777
 // keys has rows of 777 bytes); as bits it is one load of 16 bytes. Heads that share a mask share
-// its bits. Packing is bound by HBM (one read of the mask): a warp takes 1,024 keys of a row.
+// its bits. A warp takes 256 keys of a row, its loads all in flight.
 #include "attention.cuh"
 #include "capi_internal.h"
 
@@ -19,24 +19,27 @@ static MaskShape mask_shape(const gs_attention_args& a) {
           a.mask_query_stride ? a.Lq : 1, (a.Lk + 127) / 128 * 4};
 }
 
+constexpr int kMaskWords = 8;  // a warp's
+
 // ALIGNED: rows start on 4-byte boundaries, and a lane reads 4 keys at once.
 template <bool ALIGNED>
 __global__ void __launch_bounds__(256) mask_bits_kernel(const unsigned char* mask, long long sb,
                                                         long long sh, long long sq, MaskShape m,
                                                         int Lk, unsigned* bits) {
+  let_next_start();
   const int lane = threadIdx.x % 32;
-  const int segments = (m.words + 31) / 32;
-  const long long at = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const long long row = at / segments;
-  if (row >= m.b * m.h * m.q) return;
-  const int w0 = (int)(at % segments) * 32;
-  const long long q = row % m.q, h = row / m.q % m.h, b = row / m.q / m.h;
+  const unsigned segments = (m.words + kMaskWords - 1) / kMaskWords;
+  const unsigned at = blockIdx.x * 8 + threadIdx.x / 32, row = at / segments;
+  if (row >= (unsigned)(m.b * m.h * m.q)) return;
+  const int w0 = (int)(at - row * segments) * kMaskWords;
+  const unsigned bh = row / (unsigned)m.q, q = row - bh * (unsigned)m.q;
+  const unsigned b = bh / (unsigned)m.h, h = bh - b * (unsigned)m.h;
   const unsigned char* p = mask + b * sb + h * sh + q * sq;
   unsigned mine = 0;
   if (ALIGNED) {
-    unsigned v[8];
+    unsigned v[kMaskWords / 4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {  // keys w0 32 + 128 k + 4 lane and the next 3
+    for (int k = 0; k < kMaskWords / 4; ++k) {  // keys w0 32 + 128 k + 4 lane and the next 3
       const int j = w0 * 32 + 128 * k + 4 * lane;
       v[k] = 0;
       if (j + 4 <= Lk) {
@@ -47,7 +50,7 @@ __global__ void __launch_bounds__(256) mask_bits_kernel(const unsigned char* mas
       }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < kMaskWords / 4; ++k) {
       // four bytes to four bits, then eight lanes' bits to a word
       const unsigned nz = __vcmpne4(v[k], 0u) & 0x01010101u;
       unsigned word = ((nz * 0x01020408u) >> 24 & 0xfu) << (4 * (lane % 8));
@@ -58,14 +61,19 @@ __global__ void __launch_bounds__(256) mask_bits_kernel(const unsigned char* mas
       if (lane / 4 == k) mine = got;
     }
   } else {
+    unsigned char v[kMaskWords];
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
+    for (int k = 0; k < kMaskWords; ++k) {
       const int j = (w0 + k) * 32 + lane;
-      const unsigned word = __ballot_sync(~0u, j < Lk && p[j]);
+      v[k] = j < Lk ? p[j] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kMaskWords; ++k) {
+      const unsigned word = __ballot_sync(~0u, v[k] != 0);
       if (lane == k) mine = word;
     }
   }
-  if (w0 + lane < m.words) bits[row * m.words + w0 + lane] = mine;
+  if (lane < kMaskWords && w0 + lane < m.words) bits[(long long)row * m.words + w0 + lane] = mine;
 }
 
 size_t attention_mask_bytes(const gs_attention_args& a) {
@@ -83,7 +91,8 @@ int attention_pack_mask(const gs_attention_args& a, AttentionParams& p, void* wo
   p.bits_q = m.q > 1 ? m.words : 0;
   p.bits_h = m.h > 1 ? m.q * m.words : 0;
   p.bits_b = m.b > 1 ? m.h * m.q * m.words : 0;
-  const long long warps = m.b * m.h * m.q * ((m.words + 31) / 32);
+  const long long warps = m.b * m.h * m.q * ((m.words + kMaskWords - 1) / kMaskWords);
+  GS_REQUIRE(m.b * m.h * m.q < (1ll << 31) && warps < (1ll << 32) - 8, "the mask is too large");
   const unsigned blocks = (unsigned)((warps + 7) / 8);
   const bool aligned = (reinterpret_cast<uintptr_t>(a.mask) | (uintptr_t)a.mask_batch_stride |
                         (uintptr_t)a.mask_head_stride | (uintptr_t)a.mask_query_stride) % 4 == 0;

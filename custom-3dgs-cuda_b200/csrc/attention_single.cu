@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
   constexpr int kChunk = 16 * MT;
   constexpr int KL = DP / 32;         // 16-byte loads a lane makes of a row of k
   constexpr int VB = DP / 64;         // blocks of 64 numbers of v
+  let_next_start();
   const AttentionParams& a = p.a;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int shared_heads = a.Hq / a.Hkv;
