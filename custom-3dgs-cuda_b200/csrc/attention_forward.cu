@@ -382,41 +382,71 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   }
 }
 
-// out = sum over splits of exp(lse_s - lse) out_s: a warp for each row, a lane for 4 of its
-// numbers; the weights of 32 splits at a time are formed by one lane each.
-template <typename T>
+// out = sum over splits of exp(lse_s - lse) out_s: WARPS warps for each row, each with every
+// WARPS-th split, a lane for 4 of the row's numbers. 4 warps where there are more than 8 splits.
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(128) combine_kernel(AttentionParams a, int splits,
                                                       const float* part_out,
                                                       const float* part_lse) {
+  __shared__ float s_top[4], s_total[4], s_acc[4][128];
   wait_for_previous();
-  const int lane = threadIdx.x % 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, first = warp % WARPS;
   const unsigned rows = (unsigned)a.B * a.Hq * a.Lq;
-  const unsigned row = blockIdx.x * 4 + threadIdx.x / 32;
-  if (row >= rows) return;
-  float mine = lane < splits ? part_lse[(long long)lane * rows + row] : -INFINITY, top = mine;
-  for (int s = lane + 32; s < splits; s += 32) top = fmaxf(top, part_lse[(long long)s * rows + row]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-  const float shift = top == -INFINITY ? 0.0f : top;
+  const unsigned row = blockIdx.x * (4 / WARPS) + warp / WARPS;
+  if (row >= rows) return;  // whole CTAs where WARPS is 4
   const int d = lane * 4;
-  float total = 0.0f, acc[4] = {};
-  for (int s0 = 0; s0 < splits; s0 += 32) {
-    if (s0) mine = s0 + lane < splits ? part_lse[(long long)(s0 + lane) * rows + row] : -INFINITY;
-    const float w = expf(mine - shift);
+  float top = -INFINITY, total = 0.0f, acc[4] = {};
+  // chunks of 32 splits of this warp, a lane each; the maximum may grow from chunk to chunk
+  for (int s0 = 0; s0 * WARPS + first < splits; s0 += 32) {
+    const int own = (s0 + lane) * WARPS + first;
+    const float lse = own < splits ? part_lse[(long long)own * rows + row] : -INFINITY;
+    float most = lse;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+    most = fmaxf(most, top);
+    if (most > top) {
+      const float f = expf(top - most);
+      total *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] *= f;
+      top = most;
+    }
+    const float w = expf(lse - (top == -INFINITY ? 0.0f : top));
     total += w;
-    const int n = min(32, splits - s0);
-    const float* part = part_out + ((long long)s0 * rows + row) * a.D + d;
-#pragma unroll 4
+    const int n = min(32, (splits - first - s0 * WARPS + WARPS - 1) / WARPS);
+    const float* part = part_out + ((long long)(s0 * WARPS + first) * rows + row) * a.D + d;
+#pragma unroll 8
     for (int s = 0; s < n; ++s) {
       const float ws = __shfl_sync(~0u, w, s);
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (d < a.D) o = *reinterpret_cast<const float4*>(part + (long long)s * rows * a.D);
+      if (d < a.D) o = *reinterpret_cast<const float4*>(part + (long long)s * WARPS * rows * a.D);
       acc[0] = fmaf(ws, o.x, acc[0]), acc[1] = fmaf(ws, o.y, acc[1]);
       acc[2] = fmaf(ws, o.z, acc[2]), acc[3] = fmaf(ws, o.w, acc[3]);
     }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+  if constexpr (WARPS > 1) {
+    if (lane == 0) s_top[warp] = top, s_total[warp] = total;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_acc[warp][d + i] = acc[i];
+    __syncthreads();
+    if (warp) return;
+    top = s_top[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s_top[w]);
+    total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = top == -INFINITY ? 0.0f : expf(s_top[w] - top);
+      total = fmaf(f, s_total[w], total);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, s_acc[w][d + i], acc[i]);
+    }
+  }
+  // a NaN among the parts is in `total`, whatever the maximum
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   if (d < a.D) {
     const unsigned bh = row / (unsigned)a.Lq, i = row - bh * (unsigned)a.Lq;
@@ -485,8 +515,11 @@ template <typename T>
 static cudaError_t launch_combine(const AttentionParams& a, int splits, const float* out,
                                   const float* lse, cudaStream_t stream) {
   const long long rows = (long long)a.B * a.Hq * a.Lq;
-  return launch_overlapped(combine_kernel<T>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, a,
-                           splits, out, lse);
+  if (splits > 8)
+    return launch_overlapped(combine_kernel<T, 4>, dim3((unsigned)rows), 128, 0, stream, a, splits,
+                             out, lse);
+  return launch_overlapped(combine_kernel<T, 1>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream,
+                           a, splits, out, lse);
 }
 
 cudaError_t attention_combine(const gs_attention_args& args, int splits, const float* out,
