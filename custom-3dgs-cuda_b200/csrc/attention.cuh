@@ -1,6 +1,8 @@
 // What the cross-attention kernels share: the operands' description, lengths and masks.
 #pragma once
 
+#include <atomic>
+
 #include "device_errors.h"
 #include "token_types.cuh"
 
@@ -84,6 +86,21 @@ __device__ __forceinline__ void let_next_start() {
 }
 __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the runtime
+// once for each kernel and device.
+template <auto KERNEL>
+cudaError_t allow_shared(int bytes) {
+  static std::atomic<unsigned long long> done{0};  // a bit for each device
+  int dev = 0;
+  if (const cudaError_t err = cudaGetDevice(&dev)) return err;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  const cudaError_t err = cudaFuncSetAttribute(
+      KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_acq_rel);
+  return err;
 }
 
 // Launches a kernel that may start before the previous one in the stream has ended.

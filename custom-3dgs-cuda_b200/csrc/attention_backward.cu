@@ -630,8 +630,8 @@ template <typename T, int DP, bool KEYS>
 static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&m)[4],
                                    bool overlapped, cudaStream_t stream) {
   const auto kernel = attention_backward_kernel<T, DP, KEYS>;
-  const cudaError_t err = cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BackwardShared<DP, KEYS>::kBytes);
+  const cudaError_t err =
+      allow_shared<attention_backward_kernel<T, DP, KEYS>>(BackwardShared<DP, KEYS>::kBytes);
   if (err != cudaSuccess) return err;
   const int rows = KEYS ? p.a.Lk : p.a.Lq, heads = KEYS ? p.a.Hkv : p.a.Hq;
   const dim3 grid((rows + kOuter - 1) / kOuter * p.a.B * heads, p.splits);
@@ -675,25 +675,27 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
         <<<(unsigned)(stat_rows / 32), 256, 0, stream>>>(p.a, p.lq_pad, stats);
     GS_CHECK_LAUNCH();
   }
-  const auto describe = [&](CUtensorMap* map, const gs_token_view& v, int L, int H, unsigned rows) {
+  // Outer and inner tiles have the same box, so one map of each tensor serves both kernels. A map
+  // whose tensor has no rows is never used and stands for any other.
+  static_assert(kOuter == kInner, "one box for both");
+  const auto describe = [&](CUtensorMap* map, const gs_token_view& v, int L, int H) {
     return encode_tokens(map, a.dtype, v.data, a.D, L, H, a.B, v.token_stride, v.head_stride,
-                         v.batch_stride, rows);
+                         v.batch_stride, kOuter);
   };
   const auto items = [&](const gs_token_view& v) { return a.B > 1 && v.batch_stride != 0; };
-  CUtensorMap m[4];
+  CUtensorMap map_q{}, map_g{}, map_k{}, map_v{};
+  GS_REQUIRE((a.Lk == 0 || (describe(&map_k, a.k, a.Lk, a.Hkv) && describe(&map_v, a.v, a.Lk, a.Hkv))) &&
+                 (stat_rows == 0 ||
+                  (describe(&map_q, a.q, a.Lq, a.Hq) && describe(&map_g, dout, a.Lq, a.Hq))),
+             "the driver refused to describe a tensor");
+  if (stat_rows == 0) map_q = map_g = map_k;
+  if (a.Lk == 0) map_k = map_v = map_q;
   if (a.Lk > 0) {
-    GS_REQUIRE(describe(&m[0], a.k, a.Lk, a.Hkv, kOuter) &&
-                   describe(&m[1], a.v, a.Lk, a.Hkv, kOuter),
-               "the driver refused to describe a tensor");
-    m[2] = m[3] = m[0];  // without queries nothing is copied
-    if (stat_rows)
-      GS_REQUIRE(describe(&m[2], a.q, a.Lq, a.Hq, kInner) &&
-                     describe(&m[3], dout, a.Lq, a.Hq, kInner),
-                 "the driver refused to describe a tensor");
     p.x1b = items(a.k), p.x2b = items(a.v), p.y1b = items(a.q), p.y2b = items(dout);
     p.x1h = p.x2h = a.Hkv > 1, p.y1h = p.y2h = a.Hq > 1;
     p.splits = plan.key_splits;
     p.part1 = parts, p.part2 = parts + plan.key_floats;
+    const CUtensorMap m[4] = {map_k, map_v, map_q, map_g};
     GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, true>(p, m, stat_rows > 0, stream))
                       : (launch_backward<T, 128, true>(p, m, stat_rows > 0, stream)));
     count_launches(1u);
@@ -704,17 +706,11 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
     }
   }
   if (!stat_rows) return GS_OK;
-  GS_REQUIRE(describe(&m[0], a.q, a.Lq, a.Hq, kOuter) && describe(&m[1], dout, a.Lq, a.Hq, kOuter),
-             "the driver refused to describe a tensor");
-  m[2] = m[3] = m[0];  // without keys nothing is copied
-  if (a.Lk > 0)
-    GS_REQUIRE(describe(&m[2], a.k, a.Lk, a.Hkv, kInner) &&
-                   describe(&m[3], a.v, a.Lk, a.Hkv, kInner),
-               "the driver refused to describe a tensor");
   p.x1b = items(a.q), p.x2b = items(dout), p.y1b = items(a.k), p.y2b = items(a.v);
   p.x1h = p.x2h = a.Hq > 1, p.y1h = p.y2h = a.Hkv > 1;
   p.splits = plan.query_splits;
   p.part1 = parts, p.part2 = nullptr;
+  const CUtensorMap m[4] = {map_q, map_g, map_k, map_v};
   // dq starts beside the end of dk and dv, unless both use the parts in turn
   const bool beside = a.Lk > 0 && (plan.key_splits == 1 || plan.query_splits == 1);
   GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, false>(p, m, beside, stream))

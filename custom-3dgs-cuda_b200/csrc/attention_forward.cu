@@ -500,8 +500,7 @@ static cudaError_t launch_forward(const ForwardParams& p, const CUtensorMap& q,
                                   const CUtensorMap& k, const CUtensorMap& v,
                                   cudaStream_t stream) {
   const auto kernel = attention_forward_kernel<T, DP>;
-  const cudaError_t err = cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ForwardShared<DP>::kBytes);
+  const cudaError_t err = allow_shared<attention_forward_kernel<T, DP>>(ForwardShared<DP>::kBytes);
   if (err != cudaSuccess) return err;
   const int rows = p.tiles * kTileQ;
   const dim3 grid((p.a.Lq + rows - 1) / rows * p.a.B * p.a.Hq, p.splits);
