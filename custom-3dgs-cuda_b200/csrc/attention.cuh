@@ -4,6 +4,7 @@
 #include <atomic>
 
 #include "device_errors.h"
+#include "overlap.cuh"
 #include "token_types.cuh"
 
 namespace gs {
@@ -78,16 +79,6 @@ __device__ __forceinline__ void clear_rows(unsigned tile, int rows, int left,
   __syncwarp();
 }
 
-// Kernels of one call overlap at their ends (programmatic dependent launch): a kernel lets the next
-// one's CTAs start as soon as all of its own have started, and the next waits for its results
-// where it needs them.
-__device__ __forceinline__ void let_next_start() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void wait_for_previous() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the runtime
 // once for each kernel and device.
 template <auto KERNEL>
@@ -101,23 +92,6 @@ cudaError_t allow_shared(int bytes) {
       KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_acq_rel);
   return err;
-}
-
-// Launches a kernel that may start before the previous one in the stream has ended.
-template <typename... Params, typename... Args>
-cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, unsigned threads,
-                              size_t shared, cudaStream_t stream, const Args&... args) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = shared;
-  config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
 }
 
 constexpr long long kSms = 148;  // streaming multiprocessors of a B200

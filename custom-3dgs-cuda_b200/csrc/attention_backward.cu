@@ -90,6 +90,7 @@ struct ProbabilityScale<__half> {
 template <typename T>
 __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams a, int lq_pad,
                                                                 float* stats) {
+  wait_for_previous();
   let_next_start();
   const int sub = threadIdx.x % 8;
   const long long at = (long long)blockIdx.x * 32 + threadIdx.x / 8;
@@ -671,9 +672,9 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   const long long stat_rows = a.B * a.Hq * plan.lq_pad;
   float* parts = stats + 2 * stat_rows;
   if (stat_rows) {
-    attention_prepare_kernel<T>
-        <<<(unsigned)(stat_rows / 32), 256, 0, stream>>>(p.a, p.lq_pad, stats);
-    GS_CHECK_LAUNCH();
+    GS_CUDA(launch_overlapped(attention_prepare_kernel<T>, dim3((unsigned)(stat_rows / 32)), 256, 0,
+                              stream, p.a, p.lq_pad, stats));
+    count_launches(1u);
   }
   // Outer and inner tiles have the same box, so one map of each tensor serves both kernels. A map
   // whose tensor has no rows is never used and stands for any other.

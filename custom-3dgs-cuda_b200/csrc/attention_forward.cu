@@ -73,6 +73,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const int rows_a_cta = p.tiles * kTileQ, q_blocks = (a.Lq + rows_a_cta - 1) / rows_a_cta;
   const int q0 = blockIdx.x % q_blocks * rows_a_cta, bh = blockIdx.x / q_blocks;
   const int b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hkv);
+  // With a mask this kernel may run beside the one that packs it, which has itself waited for what
+  // came before; only the mask's bits are waited for then.
+  if (!a.bits) wait_for_previous();
   const int n = warp_uniform(key_count(a, b));
   const int tiles = (n + kTileK - 1) / kTileK;
   const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
@@ -152,7 +155,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                  : nullptr;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
-      if (a.bits) wait_for_previous();  // the kernel that packs the mask
+      if (a.bits) wait_for_previous();
       uint4 keep_next = make_uint4(~0u, ~0u, ~0u, ~0u);
       if (keep_row && count > 0) keep_next = keep_row[t0];
       for (int j = 0; j < count; ++j) {
@@ -504,10 +507,7 @@ static cudaError_t launch_forward(const ForwardParams& p, const CUtensorMap& q,
   if (err != cudaSuccess) return err;
   const int rows = p.tiles * kTileQ;
   const dim3 grid((p.a.Lq + rows - 1) / rows * p.a.B * p.a.Hq, p.splits);
-  if (p.a.bits)
-    return launch_overlapped(kernel, grid, kFwdThreads, ForwardShared<DP>::kBytes, stream, p, q, k, v);
-  kernel<<<grid, kFwdThreads, ForwardShared<DP>::kBytes, stream>>>(p, q, k, v);
-  return cudaGetLastError();
+  return launch_overlapped(kernel, grid, kFwdThreads, ForwardShared<DP>::kBytes, stream, p, q, k, v);
 }
 
 template <typename T>

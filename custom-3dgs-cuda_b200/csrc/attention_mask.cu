@@ -26,6 +26,7 @@ template <bool ALIGNED>
 __global__ void __launch_bounds__(256) mask_bits_kernel(const unsigned char* mask, long long sb,
                                                         long long sh, long long sq, MaskShape m,
                                                         int Lk, unsigned* bits) {
+  wait_for_previous();
   let_next_start();
   const int lane = threadIdx.x % 32;
   const unsigned segments = (m.words + kMaskWords - 1) / kMaskWords;
@@ -96,15 +97,10 @@ int attention_pack_mask(const gs_attention_args& a, AttentionParams& p, void* wo
   const unsigned blocks = (unsigned)((warps + 7) / 8);
   const bool aligned = (reinterpret_cast<uintptr_t>(a.mask) | (uintptr_t)a.mask_batch_stride |
                         (uintptr_t)a.mask_head_stride | (uintptr_t)a.mask_query_stride) % 4 == 0;
-  if (aligned)
-    mask_bits_kernel<true><<<blocks, 256, 0, stream>>>(a.mask, a.mask_batch_stride,
-                                                       a.mask_head_stride, a.mask_query_stride, m,
-                                                       a.Lk, bits);
-  else
-    mask_bits_kernel<false><<<blocks, 256, 0, stream>>>(a.mask, a.mask_batch_stride,
-                                                        a.mask_head_stride, a.mask_query_stride, m,
-                                                        a.Lk, bits);
-  GS_CHECK_LAUNCH();
+  GS_CUDA(launch_overlapped(aligned ? mask_bits_kernel<true> : mask_bits_kernel<false>, dim3(blocks),
+                            256, 0, stream, a.mask, a.mask_batch_stride, a.mask_head_stride,
+                            a.mask_query_stride, m, a.Lk, bits));
+  count_launches(1u);
   return GS_OK;
 }
 

@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
   constexpr int kChunk = 16 * MT;
   constexpr int KL = DP / 32;         // 16-byte loads a lane makes of a row of k
   constexpr int VB = DP / 64;         // blocks of 64 numbers of v
+  wait_for_previous();
   let_next_start();
   const AttentionParams& a = p.a;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
@@ -320,10 +321,8 @@ template <typename T, int DP>
 static cudaError_t launch_single(const SingleParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)p.a.B * p.a.Hkv, p.splits);
   if (p.rows <= 8)
-    attention_single_kernel<T, DP, 1><<<grid, kSingleWarps * 32, 0, stream>>>(p);
-  else
-    attention_single_kernel<T, DP, 2><<<grid, kSingleWarps * 32, 0, stream>>>(p);
-  return cudaGetLastError();
+    return launch_overlapped(attention_single_kernel<T, DP, 1>, grid, kSingleWarps * 32, 0, stream, p);
+  return launch_overlapped(attention_single_kernel<T, DP, 2>, grid, kSingleWarps * 32, 0, stream, p);
 }
 
 int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t stream) {

@@ -19,6 +19,7 @@
 
 #include "capi_internal.h"
 #include "gs_common.cuh"
+#include "overlap.cuh"
 #include "token_types.cuh"
 
 namespace gs {
@@ -96,6 +97,8 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_kernel(NormPar
   const T* w = reinterpret_cast<const T*>(p.w);
   float h[CHUNKS][VEC];
   float sum = 0.0f;
+  wait_for_previous();
+  let_next_start();
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int i = (c * ROW + lane) * VEC;
@@ -210,6 +213,8 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_backward_kerne
   extern __shared__ float meet[];
   const int lane = threadIdx.x % ROW, slot = threadIdx.x / ROW;
   const T* w = reinterpret_cast<const T*>(p.w);
+  wait_for_previous();
+  let_next_start();
   float dw[CHUNKS][VEC];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c)
@@ -301,6 +306,8 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const float* partial, int 
   __shared__ float meet[8][32];
   const int col = blockIdx.x * 32 + threadIdx.x % 32, first = threadIdx.x / 32;
   float s = 0.0f;
+  wait_for_previous();
+  let_next_start();
   if (col < width)
     for (int i = first; i < parts; i += 8) s += partial[(long long)i * width + col];
   meet[first][threadIdx.x % 32] = s;
@@ -355,11 +362,13 @@ template <typename T, bool E4M3>
 struct NormLaunch {
   const NormParams& p;
   cudaStream_t stream;
+  cudaError_t* err;
   template <int VEC, int CHUNKS, int ROW>
   void operator()() const {
     constexpr int threads = ROW < 128 ? 128 : ROW;
     const long long blocks = (p.rows + threads / ROW - 1) / (threads / ROW);
-    rms_norm_kernel<T, VEC, CHUNKS, ROW, E4M3><<<(unsigned)blocks, threads, 0, stream>>>(p);
+    *err = launch_overlapped(rms_norm_kernel<T, VEC, CHUNKS, ROW, E4M3>, dim3((unsigned)blocks),
+                             threads, 0, stream, p);
   }
 };
 
@@ -368,9 +377,10 @@ struct NormByType {
   const NormParams& p;
   bool packed;
   cudaStream_t stream;
+  cudaError_t* err;
   template <typename T>
   void operator()() const {
-    with_row_shape<T>(p.width, packed, NormLaunch<T, E4M3>{p, stream});
+    with_row_shape<T>(p.width, packed, NormLaunch<T, E4M3>{p, stream, err});
   }
 };
 
@@ -391,8 +401,8 @@ struct NormBackwardLaunch {
     constexpr int threads = ROW < 128 ? 128 : ROW;
     constexpr size_t meet = (size_t)(threads / ROW - 1) * CHUNKS * VEC * ROW * sizeof(float);
     static_assert(meet <= 48 * 1024, "the rows of dw meet in shared memory");
-    rms_norm_backward_kernel<T, VEC, CHUNKS, ROW><<<blocks, threads, meet, stream>>>(p);
-    *err = cudaGetLastError();
+    *err = launch_overlapped(rms_norm_backward_kernel<T, VEC, CHUNKS, ROW>, dim3((unsigned)blocks),
+                             threads, meet, stream, p);
   }
 };
 
@@ -407,8 +417,8 @@ struct NormBackwardByType {
   void operator()() const {
     with_row_shape<T>(p.width, packed, NormBackwardLaunch<T>{p, blocks, stream, err});
     if (*err != cudaSuccess) return;
-    norm_dw_kernel<T><<<(p.width + 31) / 32, 256, 0, stream>>>(p.partial, blocks, p.width, dw);
-    *err = cudaGetLastError();
+    *err = launch_overlapped(norm_dw_kernel<T>, dim3((unsigned)(p.width + 31) / 32), 256, 0, stream,
+                             p.partial, blocks, p.width, dw);
   }
 };
 
@@ -429,8 +439,10 @@ extern "C" int gs_rms_norm_forward(int dtype, long long rows, int width, const v
   GS_REQUIRE(!h || residual, "the residual stream is written only where a residual is added");
   const NormParams p{x, residual, weight, y, h, rstd, nullptr, rows, width, width, eps};
   const bool packed = packs(dtype, width, {x, residual, weight, y, h});
-  with_type(dtype, NormByType<false>{p, packed, (cudaStream_t)stream});
-  GS_CHECK_LAUNCH();
+  cudaError_t err = cudaSuccess;
+  with_type(dtype, NormByType<false>{p, packed, (cudaStream_t)stream, &err});
+  GS_CUDA(err);
+  gs::count_launches(1u);
   return GS_OK;
   GS_API_END();
 }
@@ -453,8 +465,10 @@ extern "C" int gs_rms_norm_e4m3(int dtype, long long rows, int width, int group,
   const NormParams p{x, residual, weight, q, h, nullptr, scales, rows, width,
                      group ? group : width, eps};
   // a group as wide as the row is a row
-  with_type(dtype, NormByType<true>{p, packed, (cudaStream_t)stream});
-  GS_CHECK_LAUNCH();
+  cudaError_t err = cudaSuccess;
+  with_type(dtype, NormByType<true>{p, packed, (cudaStream_t)stream, &err});
+  GS_CUDA(err);
+  gs::count_launches(1u);
   return GS_OK;
   GS_API_END();
 }

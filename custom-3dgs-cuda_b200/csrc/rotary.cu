@@ -21,6 +21,7 @@
 
 #include "capi_internal.h"
 #include "gs_common.cuh"
+#include "overlap.cuh"
 #include "token_types.cuh"
 
 namespace gs {
@@ -93,6 +94,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
       }
     }
   };
+  wait_for_previous();
+  let_next_start();
   load(lane_h);  // in flight while the angles are formed
 
   float c[VEC], s[VEC];
@@ -135,40 +138,40 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
 }
 
 template <typename T, int VEC, bool INTERLEAVED, typename P>
-static void launch_rotary(const RotaryParams& p, unsigned blocks, cudaStream_t stream) {
+static cudaError_t launch_rotary(const RotaryParams& p, unsigned blocks, cudaStream_t stream) {
   if (p.flight == 4)
-    rotary_kernel<T, VEC, INTERLEAVED, P, 4><<<blocks, p.threads, 0, stream>>>(p);
-  else
-    rotary_kernel<T, VEC, INTERLEAVED, P, 1><<<blocks, p.threads, 0, stream>>>(p);
+    return launch_overlapped(rotary_kernel<T, VEC, INTERLEAVED, P, 4>, dim3(blocks), p.threads, 0,
+                             stream, p);
+  return launch_overlapped(rotary_kernel<T, VEC, INTERLEAVED, P, 1>, dim3(blocks), p.threads, 0, stream, p);
 }
 
 template <typename T, int VEC, bool INTERLEAVED>
-static void launch_rotary(const RotaryParams& p, int position_type, unsigned blocks,
+static cudaError_t launch_rotary(const RotaryParams& p, int position_type, unsigned blocks,
                           cudaStream_t stream) {
   if (position_type == GS_FP32)
-    launch_rotary<T, VEC, INTERLEAVED, float>(p, blocks, stream);
+    return launch_rotary<T, VEC, INTERLEAVED, float>(p, blocks, stream);
   else
-    launch_rotary<T, VEC, INTERLEAVED, int>(p, blocks, stream);
+    return launch_rotary<T, VEC, INTERLEAVED, int>(p, blocks, stream);
 }
 
 template <typename T, int VEC>
-static void launch_rotary(const RotaryParams& p, int position_type, unsigned blocks,
+static cudaError_t launch_rotary(const RotaryParams& p, int position_type, unsigned blocks,
                           cudaStream_t stream) {
   if (p.interleaved)
-    launch_rotary<T, VEC, true>(p, position_type, blocks, stream);
+    return launch_rotary<T, VEC, true>(p, position_type, blocks, stream);
   else
-    launch_rotary<T, VEC, false>(p, position_type, blocks, stream);
+    return launch_rotary<T, VEC, false>(p, position_type, blocks, stream);
 }
 
 template <typename T>
-static void launch_rotary(const RotaryParams& p, int vec, int position_type, unsigned blocks,
+static cudaError_t launch_rotary(const RotaryParams& p, int vec, int position_type, unsigned blocks,
                           cudaStream_t stream) {
   if (vec == 4)
-    launch_rotary<T, 4>(p, position_type, blocks, stream);
+    return launch_rotary<T, 4>(p, position_type, blocks, stream);
   else if (vec == 2)
-    launch_rotary<T, 2>(p, position_type, blocks, stream);
+    return launch_rotary<T, 2>(p, position_type, blocks, stream);
   else
-    launch_rotary<T, 1>(p, position_type, blocks, stream);
+    return launch_rotary<T, 1>(p, position_type, blocks, stream);
 }
 
 }  // namespace gs
@@ -246,13 +249,11 @@ extern "C" int gs_rotary_axes(int dtype, int B, int L, int H, int D, const gs_to
     p.head_lanes = (p.head_lanes + 1) / 2;
   p.tokens_per_block = std::max(1, cta / (p.items * p.head_lanes));
   const unsigned blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-  if (dtype == GS_FP32)
-    launch_rotary<float>(p, vec, position_type, blocks, (cudaStream_t)stream);
-  else if (dtype == GS_FP16)
-    launch_rotary<__half>(p, vec, position_type, blocks, (cudaStream_t)stream);
-  else
-    launch_rotary<__nv_bfloat16>(p, vec, position_type, blocks, (cudaStream_t)stream);
-  GS_CHECK_LAUNCH();
+  const cudaStream_t st = (cudaStream_t)stream;
+  GS_CUDA(dtype == GS_FP32   ? launch_rotary<float>(p, vec, position_type, blocks, st)
+          : dtype == GS_FP16 ? launch_rotary<__half>(p, vec, position_type, blocks, st)
+                             : launch_rotary<__nv_bfloat16>(p, vec, position_type, blocks, st));
+  gs::count_launches(1u);
   return GS_OK;
   GS_API_END();
 }
