@@ -9,8 +9,8 @@
 // q = e4m3(y / s), so that y ~ q s (448 is e4m3's largest number); s = 0 where y is all zero.
 //
 // Bound by HBM: each input is read once and each output written once, the row staying in
-// registers between the sum of squares and the scaling. ROW threads hold one row, CHUNKS packs of
-// VEC elements each; the smallest of a warp, 4 warps and 32 warps that holds the row takes it.
+// registers between the sum of squares and the scaling. ROW threads hold one row, up to CHUNKS
+// packs of VEC elements each; the shape that fits the width best takes it (with_row_shape).
 // dw is summed by a fixed set of CTAs over their own rows into partial rows, which a second
 // kernel adds in a fixed order: the same bits on every run.
 #include <cuda_fp8.h>
@@ -26,7 +26,7 @@ namespace gs {
 
 constexpr float kE4m3Max = 448.0f;
 constexpr int kNormMaxWidth = 32768;
-constexpr int kNormMaxBlocks = 148 * 4;  // CTAs (and partial rows of dw) of the backward
+constexpr int kNormMaxBlocks = 148 * 2;  // CTAs (and partial rows of dw) of the backward
 
 struct NormParams {
   const void* x;
@@ -41,35 +41,46 @@ struct NormParams {
   float eps;
 };
 
-template <int ROW>
+// Waits for the ROW threads of a row: the whole CTA, or the row's own part of one that holds several.
+template <int ROW, int THREADS>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (ROW == THREADS)
+    __syncthreads();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / ROW), "n"(ROW) : "memory");
+}
+
+template <int ROW, int THREADS>
 __device__ __forceinline__ float row_sum(float v, float* shared) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   if constexpr (ROW > 32) {
     constexpr int W = ROW / 32;
-    __syncthreads();  // the previous use of `shared` is over
-    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
-    __syncthreads();
+    float* mine = shared + threadIdx.x / ROW * W;
+    row_sync<ROW, THREADS>();  // the previous use of `shared` is over
+    if (threadIdx.x % 32 == 0) mine[threadIdx.x % ROW / 32] = v;
+    row_sync<ROW, THREADS>();
     v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) v += shared[i];
+    for (int i = 0; i < W; ++i) v += mine[i];
   }
   return v;
 }
 
 // NaN where the row holds one, so that its scale says so.
-template <int ROW>
+template <int ROW, int THREADS>
 __device__ __forceinline__ float row_max(float v, float* shared) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
   if constexpr (ROW > 32) {
     constexpr int W = ROW / 32;
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = shared[0];
+    float* mine = shared + threadIdx.x / ROW * W;
+    row_sync<ROW, THREADS>();
+    if (threadIdx.x % 32 == 0) mine[threadIdx.x % ROW / 32] = v;
+    row_sync<ROW, THREADS>();
+    v = mine[0];
 #pragma unroll
-    for (int i = 1; i < W; ++i) v = max_nan(v, shared[i]);
+    for (int i = 1; i < W; ++i) v = max_nan(v, mine[i]);
   }
   return v;
 }
@@ -83,11 +94,13 @@ __device__ __forceinline__ void store_e4m3(unsigned char* p, const float (&v)[VE
   *reinterpret_cast<Pack<unsigned char, VEC>*>(p) = a;
 }
 
-// CTAs of max(ROW, 128) threads. Each row's threads take packs at stride ROW, so a warp's accesses
-// are consecutive.
+// CTAs of one row, or of four rows of a warp each. Each row's threads take packs at stride ROW, so a
+// warp's accesses are consecutive.
+constexpr int forward_threads(int row) { return row == 32 ? 128 : row; }
+
 template <typename T, int VEC, int CHUNKS, int ROW, bool E4M3>
-__global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_kernel(NormParams p) {
-  constexpr int kThreads = ROW < 128 ? 128 : ROW;
+__global__ void __launch_bounds__(forward_threads(ROW)) rms_norm_kernel(NormParams p) {
+  constexpr int kThreads = forward_threads(ROW);
   __shared__ float shared[32];
   const int lane = threadIdx.x % ROW;
   const long long row = (long long)blockIdx.x * (kThreads / ROW) + threadIdx.x / ROW;
@@ -130,7 +143,7 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_kernel(NormPar
   for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
     for (int k = 0; k < VEC; ++k) sum = fmaf(h[c][k], h[c][k], sum);
-  sum = row_sum<ROW>(sum, shared);
+  sum = row_sum<ROW, kThreads>(sum, shared);
   const float rstd = rsqrtf(sum / (float)p.width + p.eps);
   if (p.rstd && lane == 0) p.rstd[row] = rstd;
 #pragma unroll
@@ -152,7 +165,7 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_kernel(NormPar
       for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) top = max_nan(top, fabsf(h[c][k]));
-      top = row_max<ROW>(top, shared);
+      top = row_max<ROW, kThreads>(top, shared);
       const float s = top / kE4m3Max;
       const float inv = s > 0.0f ? 1.0f / s : 0.0f;
       if (lane == 0) p.scales[row] = s;
@@ -203,10 +216,14 @@ struct NormBackwardParams {
   int width;
 };
 
+// CTAs of 512 threads, two an SM, as many rows at a time as fit: enough bytes on their way, and few
+// partial rows.
+constexpr int backward_threads(int row) { return row < 512 ? 512 : row; }
+
 template <typename T, int VEC, int CHUNKS, int ROW>
-__global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_backward_kernel(
-    NormBackwardParams p) {
-  constexpr int kThreads = ROW < 128 ? 128 : ROW;
+__global__ void __launch_bounds__(backward_threads(ROW), ROW <= 512 && CHUNKS * VEC <= 8 ? 2 : 1)
+    rms_norm_backward_kernel(NormBackwardParams p) {
+  constexpr int kThreads = backward_threads(ROW);
   constexpr int kRows = kThreads / ROW;
   __shared__ float shared[32];
   // the CTA's rows of dw meet here, CHUNKS * VEC * ROW floats for each of kRows - 1 rows
@@ -252,7 +269,7 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_backward_kerne
         }
       }
     }
-    dot = row_sum<ROW>(dot, shared) / (float)p.width;
+    dot = row_sum<ROW, kThreads>(dot, shared) / (float)p.width;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int i = (c * ROW + lane) * VEC;
@@ -271,7 +288,7 @@ __global__ void __launch_bounds__(ROW < 128 ? 128 : ROW) rms_norm_backward_kerne
   }
   if constexpr (kRows > 1) {
     constexpr int kPer = CHUNKS * VEC * ROW;
-    if (slot) {
+    if (slot > 0) {
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
@@ -321,23 +338,39 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const float* partial, int 
 }
 
 // Calls f with the (VEC, CHUNKS, ROW) that holds a row: 16-byte packs where width and pointers
-// allow them, else single elements.
-template <typename T, typename F>
+// allow them, else single elements. MOST packs a thread, more only where 1,024 threads do not hold
+// the row otherwise: 4 forward; backward, which keeps three inputs and its part of dw, 8 elements,
+// for which 64 registers do (65,280 rows of 1,024 bfloat16: 103 us at 8 elements a thread, 143 at
+// 16). Narrow rows take a warp each, whose sums need no barrier.
+template <typename T, int MOST, typename F>
 static void with_row_shape(int width, bool packed, F&& f) {
   constexpr int V = 16 / (int)sizeof(T);
-  if (packed) {
-    if (width <= 32 * 4 * V)
-      f.template operator()<V, 4, 32>();
-    else if (width <= 128 * 4 * V)
-      f.template operator()<V, 4, 128>();
-    else
-      f.template operator()<V, 32 / V, 1024>();
-  } else {
-    if (width <= 32 * 32)
-      f.template operator()<1, 32, 32>();
+  if (!packed) {
+    if (width <= 1024)
+      f.template operator()<1, 8, 128>();
     else
       f.template operator()<1, 32, 1024>();
+    return;
   }
+  const int n = width / V;
+  if (n <= 32)
+    f.template operator()<V, 1, 32>();
+  else if (n <= 64)
+    f.template operator()<V, 2, 32>();
+  else if (n <= 32 * MOST)
+    f.template operator()<V, MOST, 32>();
+  else if (n <= 64 * MOST)
+    f.template operator()<V, MOST, 64>();
+  else if (n <= 128 * MOST)
+    f.template operator()<V, MOST, 128>();
+  else if (n <= 256 * MOST)
+    f.template operator()<V, MOST, 256>();
+  else if (n <= 512 * MOST)
+    f.template operator()<V, MOST, 512>();
+  else if (n <= 1024 * MOST)
+    f.template operator()<V, MOST, 1024>();
+  else
+    f.template operator()<V, 32 / V, 1024>();
 }
 
 template <typename F>
@@ -365,7 +398,7 @@ struct NormLaunch {
   cudaError_t* err;
   template <int VEC, int CHUNKS, int ROW>
   void operator()() const {
-    constexpr int threads = ROW < 128 ? 128 : ROW;
+    constexpr int threads = forward_threads(ROW);
     const long long blocks = (p.rows + threads / ROW - 1) / (threads / ROW);
     *err = launch_overlapped(rms_norm_kernel<T, VEC, CHUNKS, ROW, E4M3>, dim3((unsigned)blocks),
                              threads, 0, stream, p);
@@ -380,13 +413,12 @@ struct NormByType {
   cudaError_t* err;
   template <typename T>
   void operator()() const {
-    with_row_shape<T>(p.width, packed, NormLaunch<T, E4M3>{p, stream, err});
+    with_row_shape<T, 4>(p.width, packed, NormLaunch<T, E4M3>{p, stream, err});
   }
 };
 
-static int norm_blocks(long long rows, int width) {
-  // a row takes a warp up to 512 (fp32) or 1024 elements; the count only has to be a bound
-  (void)width;
+// CTAs of the backward: a bound that holds for every shape, since a CTA takes one row at least.
+static int norm_blocks(long long rows) {
   return (int)std::max(1ll, std::min(rows, (long long)kNormMaxBlocks));
 }
 
@@ -398,7 +430,7 @@ struct NormBackwardLaunch {
   cudaError_t* err;
   template <int VEC, int CHUNKS, int ROW>
   void operator()() const {
-    constexpr int threads = ROW < 128 ? 128 : ROW;
+    constexpr int threads = backward_threads(ROW);
     constexpr size_t meet = (size_t)(threads / ROW - 1) * CHUNKS * VEC * ROW * sizeof(float);
     static_assert(meet <= 48 * 1024, "the rows of dw meet in shared memory");
     *err = launch_overlapped(rms_norm_backward_kernel<T, VEC, CHUNKS, ROW>, dim3((unsigned)blocks),
@@ -415,7 +447,7 @@ struct NormBackwardByType {
   cudaError_t* err;
   template <typename T>
   void operator()() const {
-    with_row_shape<T>(p.width, packed, NormBackwardLaunch<T>{p, blocks, stream, err});
+    with_row_shape<T, sizeof(T) == 4 ? 2 : 1>(p.width, packed, NormBackwardLaunch<T>{p, blocks, stream, err});
     if (*err != cudaSuccess) return;
     *err = launch_overlapped(norm_dw_kernel<T>, dim3((unsigned)(p.width + 31) / 32), 256, 0, stream,
                              p.partial, blocks, p.width, dw);
@@ -475,7 +507,7 @@ extern "C" int gs_rms_norm_e4m3(int dtype, long long rows, int width, int group,
 
 extern "C" size_t gs_rms_norm_backward_workspace_size(long long rows, int width) {
   if (rows <= 0 || width <= 0 || width > kNormMaxWidth) return 0;
-  return (size_t)norm_blocks(rows, width) * width * sizeof(float);
+  return (size_t)norm_blocks(rows) * width * sizeof(float);
 }
 
 extern "C" int gs_rms_norm_backward(int dtype, long long rows, int width, const void* dy,
@@ -499,7 +531,7 @@ extern "C" int gs_rms_norm_backward(int dtype, long long rows, int width, const 
                              width};
   const bool packed = packs(dtype, width, {dy, dh, h, weight, dx});
   cudaError_t err = cudaSuccess;
-  with_type(dtype, NormBackwardByType{p, packed, norm_blocks(rows, width), dw,
+  with_type(dtype, NormBackwardByType{p, packed, norm_blocks(rows), dw,
                                       (cudaStream_t)stream, &err});
   GS_CUDA(err);
   gs::count_launches(2u);
