@@ -87,11 +87,16 @@ __device__ __forceinline__ float row_max(float v, float* shared) {
 
 template <int VEC>
 __device__ __forceinline__ void store_e4m3(unsigned char* p, const float (&v)[VEC]) {
-  Pack<unsigned char, VEC> a;
+  if constexpr (VEC == 1) {
+    *p = (unsigned char)__nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+  } else {
+    Pack<unsigned short, VEC / 2> a;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    a.v[i] = (unsigned char)__nv_cvt_float_to_fp8(v[i], __NV_SATFINITE, __NV_E4M3);
-  *reinterpret_cast<Pack<unsigned char, VEC>*>(p) = a;
+    for (int i = 0; i < VEC / 2; ++i)
+      a.v[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE,
+                                        __NV_E4M3);
+    *reinterpret_cast<Pack<unsigned short, VEC / 2>*>(p) = a;
+  }
 }
 
 // CTAs of one row, or of four rows of a warp each. Each row's threads take packs at stride ROW, so a
