@@ -56,25 +56,31 @@ __device__ __forceinline__ void hide32(unsigned keep, unsigned* s) {
     if (!(keep >> k & 1u)) s[k] = kMinusInf;
 }
 
-// Zeroes, in a swizzled tile of `rows` keys (BOXES boxes of 128 bytes a row) at shared address
-// `tile`, the rows from `left` on and those whose bit in `bits` is 0 (or null): whole rows, so
-// the swizzle inside them does not matter. One warp; the matrix engine sees it afterwards.
-template <int BOXES>
-__device__ __forceinline__ void clear_rows(unsigned tile, int rows, int left,
-                                           const unsigned* bits) {
+// Zeroes, in a swizzled tile of ROWS keys (BOXES boxes of 128 bytes a row) at shared address `tile`,
+// the rows from `left` on and those whose bit in `bits` is 0 (or null): whole rows, so the swizzle
+// inside them does not matter. One warp; the matrix engine sees it afterwards.
+template <int BOXES, int ROWS>
+__device__ __forceinline__ void clear_rows(unsigned tile, int left, const unsigned* bits) {
   const int lane = threadIdx.x % 32;
-  for (int w = 0; w < rows / 32; ++w) {
-    unsigned out = ~(below(left, w) & (bits ? bits[w] : ~0u));
-    while (out) {
-      const int k = w * 32 + __ffs(out) - 1;
-      out &= out - 1;
+  for (int x = 0; x < BOXES; ++x)
+#pragma unroll 4
+    for (int at = left * 128 + lane * 16; at < ROWS * 128; at += 512)
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + x * ROWS * 128 + at),
+                   "r"(0)
+                   : "memory");
+  if (bits)
+    for (int w = 0; w < ROWS / 32; ++w) {
+      unsigned out = below(left, w) & ~bits[w];
+      while (out) {
+        const int k = w * 32 + __ffs(out) - 1;
+        out &= out - 1;
 #pragma unroll
-      for (int x = 0; x < BOXES; ++x)
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile + (x * rows + k) * 128 + lane * 4),
-                     "r"(0)
-                     : "memory");
+        for (int x = 0; x < BOXES; ++x)
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile + (x * ROWS + k) * 128 + lane * 4),
+                       "r"(0)
+                       : "memory");
+      }
     }
-  }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }

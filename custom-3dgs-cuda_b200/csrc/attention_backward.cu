@@ -222,20 +222,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int count = (int)((long long)tiles * (blockIdx.y + 1) / p.splits) - t0;
   const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
 
+  if (threadIdx.x == 288) {
+    prefetch_map(&map_x1);
+    prefetch_map(&map_x2);
+    prefetch_map(&map_y1);
+    prefetch_map(&map_y2);
+  }
   if (threadIdx.x == 0) {
     gave_up = 0;
-    mbar_init(&x_full, 1);
-    mbar_init(&acc_full, 1);
+    mbar_set(&x_full, 1);
+    mbar_set(&acc_full, 1);
     for (int i = 0; i < S::kStages1; ++i) {
-      mbar_init(&y1_full[i], 1);
-      mbar_init(&y1_free[i], 1);
+      mbar_set(&y1_full[i], 1);
+      mbar_set(&y1_free[i], 1);
     }
     for (int i = 0; i < S::kStages2; ++i) {
-      mbar_init(&y2_full[i], 1);
-      mbar_init(&y2_free[i], 1);
+      mbar_set(&y2_full[i], 1);
+      mbar_set(&y2_free[i], 1);
     }
-    for (uint64_t* bar : {&s_full, &dp_full, &acc_done}) mbar_init(bar, 1);
-    for (uint64_t* bar : {&s_read, &p_ready, &ds_ready}) mbar_init(bar, 8);
+    for (uint64_t* bar : {&s_full, &dp_full, &acc_done}) mbar_set(bar, 1);
+    for (uint64_t* bar : {&s_read, &p_ready, &ds_ready}) mbar_set(bar, 8);
+    mbar_ready();
   }
   if (warp == 8) tc_alloc(&tmem_slot, 512);
   // dk and dv need the rows' statistics and with them the packed mask; the CTAs of dq that start
@@ -371,38 +378,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const TokenView& view = KEYS ? (first ? a.dk : a.dv) : a.dq;
     const long long rows = (long long)a.B * outer_heads * outer_rows;
     float* part = first ? p.part1 : p.part2;
-    for (int d = KEYS ? 0 : wg * (DP / 2); d < (KEYS ? DP : (wg + 1) * (DP / 2)); d += 16) {
-      if (d >= a.D) break;
-      unsigned o[16];
-#pragma unroll
-      for (int k = 0; k < 16; ++k) o[k] = 0u;
-      if (ok && count > 0) {
-        tc_ld16((first ? tm_acc1 : tm_acc2) + lanes + d, o);
-        tc_wait_ld();
-      }
-      if (x >= outer_rows) continue;
-      float f[16];
-#pragma unroll
-      for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(o[k]) * factor;
-      if (p.splits == 1) {
-        T* out = view.at<T>(b, x, ho) + d;
-#pragma unroll
-        for (int k = 0; k < 16; k += 8) {
-          if (d + k >= a.D) break;
-          uint4 w;
-          w.x = pack2<T>(f[k], f[k + 1]), w.y = pack2<T>(f[k + 2], f[k + 3]);
-          w.z = pack2<T>(f[k + 4], f[k + 5]), w.w = pack2<T>(f[k + 6], f[k + 7]);
-          *reinterpret_cast<uint4*>(out + k) = w;
-        }
-      } else {
-        float* out = part + (blockIdx.y * rows + (long long)bh * outer_rows + x) * a.D + d;
-#pragma unroll
-        for (int k = 0; k < 16; k += 4) {
-          if (d + k >= a.D) break;
-          *reinterpret_cast<float4*>(out + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
-        }
-      }
-    }
+    const int d = KEYS ? 0 : wg * (DP / 2), r0 = x - lane;
+    // the outer tiles in shared memory have done their work
+    constexpr int kCols = KEYS ? DP : DP / 2;
+    const bool wide = p.splits > 1;
+    char* to = wide ? reinterpret_cast<char*>(
+                          part +
+                          (blockIdx.y * rows + (long long)bh * outer_rows + r0) * a.D + d)
+                    : reinterpret_cast<char*>(view.at<T>(b, r0, ho) + d);
+    store_rows<T, kCols>((first ? tm_acc1 : tm_acc2) + lanes + d, ok && count > 0, true, factor,
+                         a.D - d, wide, (wg ? sm_x2 : sm_x1) + warp % 4 * (kCols * 64), to,
+                         wide ? a.D * 4ll : view.l * 2, outer_rows - r0);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
     if (warp == 9) {
@@ -473,7 +459,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           // would be added
           const int key = (t0 + j) * kInner;
           if (n - key < kInner || key_mask)
-            clear_rows<S::kBoxes>(sm_y1 + st * S::kInnerBytes, kInner, n - key,
+            clear_rows<S::kBoxes, kInner>(sm_y1 + st * S::kInnerBytes, n - key,
                                   key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
         }
         return true;

@@ -75,6 +75,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const int b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hkv);
   // With a mask this kernel may run beside the one that packs it, which has itself waited for what
   // came before; only the mask's bits are waited for then.
+  if (threadIdx.x == 288) {
+    prefetch_map(&map_q);
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
   if (!a.bits) wait_for_previous();
   const int n = warp_uniform(key_count(a, b));
   const int tiles = (n + kTileK - 1) / kTileK;
@@ -99,22 +104,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   };
   if (warp == 9 && threadIdx.x % 32 == 0) {
     gave_up = 0;
-    mbar_init(&q_full, 1);
+    mbar_set(&q_full, 1);
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_free[i], both ? 2 : 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_clean[i], 1);
-      mbar_init(&v_free[i], both ? 2 : 1);
+      mbar_set(&k_full[i], 1);
+      mbar_set(&k_free[i], both ? 2 : 1);
+      mbar_set(&v_full[i], 1);
+      mbar_set(&v_clean[i], 1);
+      mbar_set(&v_free[i], both ? 2 : 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_read[i], 4);
-      mbar_init(&p_ready[i], 4);
-      mbar_init(&o_done[i], 1);
-      mbar_init(&o_full[i], 1);
-      mbar_init(&turn[i], 4);
+      mbar_set(&s_full[i], 1);
+      mbar_set(&s_read[i], 4);
+      mbar_set(&p_ready[i], 4);
+      mbar_set(&o_done[i], 1);
+      mbar_set(&o_full[i], 1);
+      mbar_set(&turn[i], 4);
     }
+    mbar_ready();
     if (count > 0) {  // the first copies start while the other warps get ready
       const int bq = b * p.qb, hq = h * p.qh;
       mbar_arrive_expect_tx(&q_full, (both ? 2 : 1) * S::kTileBytes);
@@ -255,37 +261,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       const float lse = l == 0.0f ? -INFINITY : m * p.scale_log2 * 0.6931471805599453f + logf(l);
       const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
       const long long rows = (long long)a.B * a.Hq * a.Lq;
-      for (int c = 0; c < DP; c += 16) {
-        if (c >= a.D) break;
-        unsigned o[16];
-        if (ok && count > 0) {
-          tc_ld16(my_o + c, o);
-          tc_wait_ld();
-        }
-        float f[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) f[k] = l == 0.0f ? 0.0f : __uint_as_float(o[k]) * inv;
-        if (i < a.Lq) {
-          if (p.splits == 1) {
-            T* out = a.out.at<T>(b, i, h) + c;
-#pragma unroll
-            for (int k = 0; k < 16; k += 8) {
-              if (c + k >= a.D) break;
-              uint4 w;
-              w.x = pack2<T>(f[k], f[k + 1]), w.y = pack2<T>(f[k + 2], f[k + 3]);
-              w.z = pack2<T>(f[k + 4], f[k + 5]), w.w = pack2<T>(f[k + 6], f[k + 7]);
-              *reinterpret_cast<uint4*>(out + k) = w;
-            }
-          } else {
-            float* out = p.part_out + (blockIdx.y * rows + row) * a.D + c;
-#pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              if (c + k >= a.D) break;
-              *reinterpret_cast<float4*>(out + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
-            }
-          }
-        }
-      }
+      // the tile's queries in shared memory have done their work
+      const int i0 = i - (int)threadIdx.x % 32;
+      const bool wide = p.splits > 1;
+      char* to = wide ? reinterpret_cast<char*>(
+                            p.part_out +
+                            (blockIdx.y * rows + row - (int)threadIdx.x % 32) * a.D)
+                      : reinterpret_cast<char*>(a.out.at<T>(b, i0, h));
+      store_rows<T, DP>(my_o, ok && count > 0, l != 0.0f, inv, a.D, wide,
+                        sm_q + t * S::kTileBytes + warp % 4 * (DP * 64), to,
+                        wide ? a.D * 4ll : a.out.l * 2, a.Lq - i0);
       if (i < a.Lq) {
         if (p.splits > 1)
           p.part_lse[blockIdx.y * rows + row] = lse;
@@ -315,7 +300,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const int st = j % S::kStages, key = (t0 + j) * kTileK;
         if (!tc_wait_warp(&v_full[st], j / S::kStages & 1)) { gave_up = 1; break; }
         if (n - key < kTileK || key_mask)
-          clear_rows<S::kBoxes>(sm_v + st * S::kTileBytes, kTileK, n - key,
+          clear_rows<S::kBoxes, kTileK>(sm_v + st * S::kTileBytes, n - key,
                                 key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
         mbar_arrive_warp(&v_clean[st]);
       }

@@ -46,6 +46,19 @@ __device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, unsigned parity) {
   return __all_sync(~0u, tc_wait(bar, parity));
 }
 
+// A barrier's first state, to be seen by the other threads and engines after mbar_ready and a
+// __syncthreads.
+__device__ __forceinline__ void mbar_set(uint64_t* bar, unsigned arrivals) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(arrivals)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_ready() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // True in one lane of the (converged) warp. The products and commits below are issued under it
 // rather than under `lane == 0`: the compiler then knows that one thread runs them (105 clocks to
 // issue a product under `lane == 0`, under 64 so).
@@ -204,6 +217,68 @@ __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float lo, float hi) {
   unsigned r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// Writes COLS columns from `addr` on of the warp's 32 accumulator rows, times `factor`, as far as
+// `left` columns go (a multiple of 8): rounded to T, or in 32 bits (`wide`), to rows `pitch` bytes
+// apart from `to` on, of which the first `rows` exist. Where there is nothing to read (`have` false,
+// for the whole warp) or the lane's row counts for nothing (`live` false) zeros are written. The rows
+// pass through COLS * 64 bytes of shared memory at `stage`, of this warp alone, so that neighbouring
+// lanes write neighbouring 16 bytes: a lane writing its own row would touch 32 lines at a time. The
+// loop that writes is kept short: it runs once a CTA, from a cold instruction cache.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_rows(unsigned addr, bool have, bool live, float factor,
+                                           int left, bool wide, unsigned stage, char* to,
+                                           long long pitch, int rows) {
+  constexpr int kPieces = COLS / 8, kSwizzle = (kPieces < 8 ? kPieces : 8) - 1;
+  const int lane = threadIdx.x % 32;
+  float f[COLS];
+  if (have) {
+    unsigned o[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32) tc_ld32(addr + c, o + c);
+    tc_wait_ld();
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) f[c] = live ? __uint_as_float(o[c]) * factor : 0.0f;
+  } else {
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) f[c] = 0.0f;
+  }
+  const unsigned mine = stage + lane * kPieces * 16;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (half && !wide) break;
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      uint4 w;
+      if (wide) {
+        const float* x = f + half * (COLS / 2) + c * 4;
+        w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                       __float_as_uint(x[3]));
+      } else {
+        const float* x = f + c * 8;
+        w = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+                       pack2<T>(x[6], x[7]));
+      }
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                       mine + ((c ^ (lane & kSwizzle)) << 4)),
+                   "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                   : "memory");
+    }
+    __syncwarp();
+    const int c = lane % kPieces, column = wide ? half * (COLS / 2) + c * 4 : c * 8;
+    char* out = to + column * (wide ? 4 : 2);
+#pragma unroll 2
+    for (int r = lane / kPieces; r < 32; r += 32 / kPieces) {
+      uint4 w;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                   : "r"(stage + r * kPieces * 16 + ((c ^ (r & kSwizzle)) << 4))
+                   : "memory");
+      if (r < rows && column < left) *reinterpret_cast<uint4*>(out + r * pitch) = w;
+    }
+    __syncwarp();
+  }
 }
 
 // 2^x by the special-function unit: relative error below 2^-22, 0 for -inf, results below 2^-126
