@@ -209,26 +209,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                  sm_y2 = sm_y1 + S::kStages1 * S::kInnerBytes,
                  sm_stats = sm_y2 + S::kStages2 * S::kInnerBytes;
   const int warp = warp_uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
-  const AttentionParams& a = p.a;
-  const int shared_heads = a.Hq / a.Hkv;
-  const int outer_rows = KEYS ? a.Lk : a.Lq, outer_heads = KEYS ? a.Hkv : a.Hq;
-  const int outer_tiles = (outer_rows + kOuter - 1) / kOuter;
-  const int x0 = blockIdx.x % outer_tiles * kOuter, bh = blockIdx.x / outer_tiles;
-  const int b = bh / outer_heads, ho = bh % outer_heads;
-  const int n = warp_uniform(key_count(a, b));
-  const int q_tiles = p.lq_pad / kInner;
-  const int tiles = KEYS ? (x0 < n ? q_tiles * shared_heads : 0) : (n + kInner - 1) / kInner;
-  const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
-  const int count = (int)((long long)tiles * (blockIdx.y + 1) / p.splits) - t0;
-  const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
-
-  if (threadIdx.x == 288) {
+  if (threadIdx.x == 288) {  // of warp 9
     prefetch_map(&map_x1);
     prefetch_map(&map_x2);
     prefetch_map(&map_y1);
     prefetch_map(&map_y2);
-  }
-  if (threadIdx.x == 0) {
     gave_up = 0;
     mbar_set(&x_full, 1);
     mbar_set(&acc_full, 1);
@@ -244,15 +229,35 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (uint64_t* bar : {&s_read, &p_ready, &ds_ready}) mbar_set(bar, 8);
     mbar_ready();
   }
-  if (warp == 8) tc_alloc(&tmem_slot, 512);
+  __syncwarp();
+  const AttentionParams& a = p.a;
+  const int shared_heads = a.Hq / a.Hkv;
+  const int outer_rows = KEYS ? a.Lk : a.Lq, outer_heads = KEYS ? a.Hkv : a.Hq;
+  const int outer_tiles = (outer_rows + kOuter - 1) / kOuter;
+  const int x0 = blockIdx.x % outer_tiles * kOuter, bh = blockIdx.x / outer_tiles;
+  const int b = bh / outer_heads, ho = bh % outer_heads;
+  const int n = warp_uniform(key_count(a, b));
+  const int q_tiles = p.lq_pad / kInner;
+  const int tiles = KEYS ? (x0 < n ? q_tiles * shared_heads : 0) : (n + kInner - 1) / kInner;
+  // at most 2^24 tiles times kSms splits fit 32 bits
+  const unsigned splits = (unsigned)p.splits;
+  const int t0 = (int)((unsigned)tiles * blockIdx.y / splits);
+  const int count = (int)((unsigned)tiles * (blockIdx.y + 1) / splits) - t0;
+  const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
+
   // dk and dv need the rows' statistics and with them the packed mask; the CTAs of dq that start
   // beside the last of dk's and dv's then find both, and only end after them
   if (KEYS) wait_for_previous();
   let_next_start();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const unsigned tmem = (unsigned)warp_uniform((int)tmem_slot);
+  if (warp == 9) {  // goes on to the first copies while the others get ready
+    ready_arrive<kBwdThreads>();
+  } else {
+    if (warp == 8) tc_alloc(&tmem_slot, 512);
+    tc_fence_before();
+    ready_wait<kBwdThreads>();
+    tc_fence_after();
+  }
+  const unsigned tmem = warp == 9 ? 0u : (unsigned)warp_uniform((int)tmem_slot);
   // Tensor memory: S, dP, the sums, P and dS (in S's and dP's columns unless kOwnP). The 16-bit
   // numbers of warpgroup w's 64 inner columns take 32 columns from w * kHalf on.
   constexpr unsigned kHalf = S::kOwnP ? 32 : 64;

@@ -73,36 +73,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const int rows_a_cta = p.tiles * kTileQ, q_blocks = (a.Lq + rows_a_cta - 1) / rows_a_cta;
   const int q0 = blockIdx.x % q_blocks * rows_a_cta, bh = blockIdx.x / q_blocks;
   const int b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hkv);
-  // With a mask this kernel may run beside the one that packs it, which has itself waited for what
-  // came before; only the mask's bits are waited for then.
-  if (threadIdx.x == 288) {
+  const bool both = p.tiles == 2 && q0 + kTileQ < a.Lq;
+  if (threadIdx.x == 288) {  // of warp 9
     prefetch_map(&map_q);
     prefetch_map(&map_k);
     prefetch_map(&map_v);
-  }
-  if (!a.bits) wait_for_previous();
-  const int n = warp_uniform(key_count(a, b));
-  const int tiles = (n + kTileK - 1) / kTileK;
-  const int t0 = (int)((long long)tiles * blockIdx.y / p.splits);
-  const int t1 = (int)((long long)tiles * (blockIdx.y + 1) / p.splits);
-  const int count = t1 - t0;
-  const bool both = p.tiles == 2 && q0 + kTileQ < a.Lq;
-
-  const auto load_k = [&](int j) {
-    const int st = j % S::kStages;
-    mbar_arrive_expect_tx(&k_full[st], S::kTileBytes);
-    for (int x = 0; x < S::kBoxes; ++x)
-      tma_load_4d(sm_k + st * S::kTileBytes + x * 16384, &map_k, x * 64, (t0 + j) * kTileK,
-                  hk * p.kh, b * p.kb, &k_full[st]);
-  };
-  const auto load_v = [&](int j) {
-    const int st = j % S::kStages;
-    mbar_arrive_expect_tx(&v_full[st], S::kTileBytes);
-    for (int x = 0; x < S::kBoxes; ++x)
-      tma_load_4d(sm_v + st * S::kTileBytes + x * 16384, &map_v, x * 64, (t0 + j) * kTileK,
-                  hk * p.vh, b * p.vb, &v_full[st]);
-  };
-  if (warp == 9 && threadIdx.x % 32 == 0) {
     gave_up = 0;
     mbar_set(&q_full, 1);
     for (int i = 0; i < S::kStages; ++i) {
@@ -121,7 +96,36 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       mbar_set(&turn[i], 4);
     }
     mbar_ready();
-    if (count > 0) {  // the first copies start while the other warps get ready
+  }
+  __syncwarp();
+  // With a mask this kernel may run beside the one that packs it, which has itself waited for what
+  // came before; only the mask's bits are waited for then.
+  if (!a.bits) wait_for_previous();
+  const int n = warp_uniform(key_count(a, b));
+  const int tiles = (n + kTileK - 1) / kTileK;
+  // fewer than 2^24 tiles times at most kSms splits fit 32 bits
+  const unsigned splits = (unsigned)p.splits;
+  const int t0 = (int)((unsigned)tiles * blockIdx.y / splits);
+  const int count = (int)((unsigned)tiles * (blockIdx.y + 1) / splits) - t0;
+
+  const auto load_k = [&](int j) {
+    const int st = j % S::kStages;
+    mbar_arrive_expect_tx(&k_full[st], S::kTileBytes);
+    for (int x = 0; x < S::kBoxes; ++x)
+      tma_load_4d(sm_k + st * S::kTileBytes + x * 16384, &map_k, x * 64, (t0 + j) * kTileK,
+                  hk * p.kh, b * p.kb, &k_full[st]);
+  };
+  const auto load_v = [&](int j) {
+    const int st = j % S::kStages;
+    mbar_arrive_expect_tx(&v_full[st], S::kTileBytes);
+    for (int x = 0; x < S::kBoxes; ++x)
+      tma_load_4d(sm_v + st * S::kTileBytes + x * 16384, &map_v, x * 64, (t0 + j) * kTileK,
+                  hk * p.vh, b * p.vb, &v_full[st]);
+  };
+  let_next_start();
+  if (warp == 9) {  // goes on to the first copies while the others get ready
+    ready_arrive<kFwdThreads>();
+    if (threadIdx.x % 32 == 0 && count > 0) {
       const int bq = b * p.qb, hq = h * p.qh;
       mbar_arrive_expect_tx(&q_full, (both ? 2 : 1) * S::kTileBytes);
       for (int t = 0; t < (both ? 2 : 1); ++t)
@@ -133,13 +137,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         load_v(j);
       }
     }
+  } else {
+    if (warp == 8) tc_alloc(&tmem_slot, 512);
+    tc_fence_before();
+    ready_wait<kFwdThreads>();
+    tc_fence_after();
   }
-  let_next_start();
-  if (warp == 8) tc_alloc(&tmem_slot, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const unsigned tmem = (unsigned)warp_uniform((int)tmem_slot);
+  const unsigned tmem = warp == 9 ? 0u : (unsigned)warp_uniform((int)tmem_slot);
   // Tensor memory, 512 columns: S of both tiles 256, O of both 2 DP. Up to D = 64 there is room
   // for P beside S; above, P takes the first half of S's own columns.
   constexpr bool kAhead = DP == 64;

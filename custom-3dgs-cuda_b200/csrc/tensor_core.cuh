@@ -55,6 +55,16 @@ __device__ __forceinline__ void mbar_set(uint64_t* bar, unsigned arrivals) {
 __device__ __forceinline__ void mbar_ready() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
+// Named barrier 1 over THREADS threads: a warp that only arrives goes on at once, what it wrote
+// before is seen by those that wait.
+template <int THREADS>
+__device__ __forceinline__ void ready_arrive() {
+  asm volatile("bar.arrive 1, %0;" ::"n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void ready_wait() {
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }

@@ -240,3 +240,77 @@ def test_runs_on_the_current_stream(cuda_device):
     s.synchronize()
     assert_within(o, *ref["out"], "other stream")
     assert_within(one, ref["out"][0][:, :1], ref["out"][1][:, :1], "other stream, one query")
+
+
+def test_calls_recorded_in_a_graph(cuda_device):
+    """Every kernel of the token operators, the masked and split ones and those that overlap the end
+    of the one before included, replays in a CUDA graph on new inputs."""
+    from gs3d_b200.attention import cross_attention
+    from gs3d_b200.norm import rms_norm, rms_norm_8bit
+    from gs3d_b200.rotary import rotary_axes
+
+    q, k, v, _ = draw(cuda_device, torch.bfloat16, 2, 150, 900, 4, 2, 64, seed=12)
+    mask = masks(cuda_device, 2, 4, 150, 900, "query")
+    lengths = torch.tensor([900, 411], dtype=torch.int32, device=cuda_device)
+    w = torch.ones(64, device=cuda_device, dtype=torch.bfloat16)
+    pos = torch.rand(2, 150, 1, device=cuda_device) * 30
+
+    def chain():
+        x, h = rms_norm(q, w, residual=q)
+        x = rotary_axes(x, pos, (64,))
+        o = cross_attention(x, k, v, lengths=lengths, mask=mask)
+        one = cross_attention(o[:, :1], k, v, lengths=lengths)
+        q8, s = rms_norm_8bit(o, w)
+        return x, h, o, one, q8, s
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            chain()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for seed in (13, 14):
+        fresh = draw(cuda_device, torch.bfloat16, 2, 150, 900, 4, 2, 64, seed=seed)
+        for old, new in zip((q, k, v), fresh):
+            old.copy_(new)
+        lengths.copy_(torch.tensor([900 - seed, 300 + seed], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, chain()):
+            assert torch.equal(a.float(), b.float())
+
+
+def test_back_to_back_calls_do_not_overtake_one_another(cuda_device):
+    """Kernels that may start before the one in front has ended still see its results: a chain of
+    dependent calls, its buffers reused by the allocator, gives the same bits as one that waits
+    after every call."""
+    from gs3d_b200.attention import cross_attention
+    from gs3d_b200.norm import rms_norm
+    from gs3d_b200.rotary import rotary_axes
+
+    q, k, v, _ = draw(cuda_device, torch.bfloat16, 1, 300, 700, 4, 2, 64, seed=15)
+    w = torch.ones(64, device=cuda_device, dtype=torch.bfloat16)
+    pos = torch.rand(1, 300, 1, device=cuda_device) * 30
+    mask = masks(cuda_device, 1, 4, 300, 700, "query")
+
+    def chain(wait):
+        x, n = q, torch.full((1,), 700, dtype=torch.int32, device=cuda_device)
+        for i in range(12):
+            x = rotary_axes(x, pos, (64,), inverse=bool(i % 2))
+            wait()
+            x = cross_attention(x, k, v, lengths=n, mask=mask if i % 3 else None)
+            wait()
+            x, _ = rms_norm(x, w, residual=q)
+            wait()
+            one = cross_attention(x[:, :2], k, v, lengths=n)
+            wait()
+            x = torch.cat((one, x[:, 2:]), 1)
+            n = n - 13
+        return x
+
+    apart = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        assert torch.equal(chain(lambda: None), apart)
