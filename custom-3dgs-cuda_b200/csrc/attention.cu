@@ -66,8 +66,9 @@ extern "C" int gs_cross_attention_forward(const gs_attention_args* a, void* work
     fault = view_fault(*v, keys ? a->Lk : a->Lq, keys ? a->Hkv : a->Hq);
     GS_REQUIRE(!*fault, fault);
   }
-  GS_REQUIRE(workspace_bytes >= gs_cross_attention_workspace_size(a), "workspace too small");
-  GS_REQUIRE(workspace || !gs_cross_attention_workspace_size(a), "null pointer");
+  const size_t needed = gs_cross_attention_workspace_size(a);
+  GS_REQUIRE(workspace_bytes >= needed, "workspace too small");
+  GS_REQUIRE(workspace || !needed, "null pointer");
   return attention_is_single(*a) ? attention_single(*a, workspace, (cudaStream_t)stream)
                                  : attention_forward(*a, workspace, (cudaStream_t)stream);
   GS_API_END();

@@ -3,9 +3,15 @@
 // A CTA holds two tiles of 128 query rows of one head and walks over tiles of 128 keys. For each
 // pair of tiles S = q k^T is a product into tensor memory; a warpgroup with one thread for each
 // query row reads its row of S, keeps the running maximum and sum, writes P = exp(S - max) back
-// over S in 16 bits, and P v is added to the row's accumulator, also in tensor memory. Four
-// warps serve the first query tile, four the second, one warp issues the products, one the
-// copies. While one tile's softmax runs, the other tile's products do.
+// into tensor memory in 16 bits, and P v is added to the row's accumulator, also there. Four warps
+// serve the first query tile, four the second; two issue their products, on schedulers of their own
+// (one for both held the tensor pipe up: 204 -> 293 us in the first case below), one the copies, one
+// clears v's rows past the keys' end. While one tile's softmax runs, the other tile's products do.
+//
+// What bounds it, at D 64, is the exponentials: 1,024 clocks of the special-function unit for a pair
+// of tiles whose two products take 512 (measured: that unit 69% busy, the tensor pipe 34%); at D 128
+// both take 1,024. One item of 4,096 queries, bfloat16: 16 heads of 64 x 8,160 keys 197 us, 700
+// TFLOP/s; 16 heads of 128 x 4,096 keys 147 us, 940 TFLOP/s.
 //
 // The maximum that P is formed with may lag behind the true one by up to kLag powers of two: the
 // accumulator (128 rows x D numbers through registers) is rescaled only when a row's maximum has
@@ -14,7 +20,10 @@
 // nothing is lost. The row sum adds P before that rounding, in 32 bits.
 //
 // With few query tiles the keys are split over CTAs: each writes its normalised output in 32
-// bits and its lse, and combine_kernel joins them with weights exp(lse_split - lse).
+// bits and its lse, and combine_kernel joins them with weights exp(lse_split - lse). With few queries,
+// heads that share a key head share a tile of rows too, so that k and v are read and multiplied once
+// for all of them (2 x 1 query x 65,280 keys, 24 heads on each of 8 of 128: 2,533 -> 106 us; 4 x 40 x
+// 3,600, 4 on each of 4 of 64: 24.3 -> 17.3).
 #include <algorithm>
 #include <cmath>
 
@@ -39,6 +48,8 @@ struct ForwardParams {
   float lag;         // kLag in units of unscaled scores
   int negate;        // scale < 0: scores change sign first
   int tiles;   // query tiles a CTA holds, 1 or 2
+  int pack;    // query heads a tile holds: above 1 it holds all queries of each
+  int groups, shared, q_blocks;  // Hq / pack, Hq / Hkv, CTAs a group of heads
   int splits;
   int kb, kh, vb, vh, qb, qh;  // 0 where all batch items (heads) share the tensor, else 1
   float* part_out;  // [splits, B, Hq, Lq, D] where splits > 1
@@ -70,10 +81,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                  sm_v = sm_k + S::kStages * S::kTileBytes;
   const int warp = warp_uniform(threadIdx.x / 32);
   const AttentionParams& a = p.a;
-  const int rows_a_cta = p.tiles * kTileQ, q_blocks = (a.Lq + rows_a_cta - 1) / rows_a_cta;
-  const int q0 = blockIdx.x % q_blocks * rows_a_cta, bh = blockIdx.x / q_blocks;
-  const int b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hkv);
-  const bool both = p.tiles == 2 && q0 + kTileQ < a.Lq;
+  const int queries = p.pack * a.Lq;
+  const unsigned bh = blockIdx.x / (unsigned)p.q_blocks, block = blockIdx.x - bh * p.q_blocks;
+  const int q0 = block * p.tiles * kTileQ, b = bh / (unsigned)p.groups,
+            h0 = (bh - b * p.groups) * p.pack, hk = (unsigned)h0 / (unsigned)p.shared;
+  const bool both = p.tiles == 2 && q0 + kTileQ < queries;
   if (threadIdx.x == 288) {  // of warp 9
     prefetch_map(&map_q);
     prefetch_map(&map_k);
@@ -126,8 +138,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (warp == 9) {  // goes on to the first copies while the others get ready
     ready_arrive<kFwdThreads>();
     if (threadIdx.x % 32 == 0 && count > 0) {
-      const int bq = b * p.qb, hq = h * p.qh;
-      mbar_arrive_expect_tx(&q_full, (both ? 2 : 1) * S::kTileBytes);
+      const int bq = b * p.qb, hq = h0 * p.qh;
+      mbar_arrive_expect_tx(&q_full, p.pack > 1 ? queries * S::kBoxes * 128
+                                                : (both ? 2 : 1) * S::kTileBytes);
       for (int t = 0; t < (both ? 2 : 1); ++t)
         for (int x = 0; x < S::kBoxes; ++x)
           tma_load_4d(sm_q + t * S::kTileBytes + x * 16384, &map_q, x * 64, q0 + t * kTileQ, hq, bq,
@@ -139,6 +152,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     }
   } else {
     if (warp == 8) tc_alloc(&tmem_slot, 512);
+    // rows that no query is copied to: as good as a query of zeros
+    if (warp == 11 && p.pack > 1) clear_rows<S::kBoxes, kTileQ>(sm_q, queries, nullptr);
     tc_fence_before();
     ready_wait<kFwdThreads>();
     tc_fence_after();
@@ -155,14 +170,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---- softmax: one thread for each query row ----
     const int t = warp / 4;
-    const int i = q0 + t * kTileQ + threadIdx.x % 128;
+    // the thread's row, one of `queries`, and what it is of: query i of head h0 + s
+    const int row_q = q0 + t * kTileQ + threadIdx.x % 128;
+    const bool live = row_q < queries;
+    int i = min(row_q, queries - 1), h = h0;
+    if (p.pack > 1) {
+      const int s = (unsigned)i / (unsigned)a.Lq;
+      h += s;
+      i -= s * a.Lq;
+    }
     if (t == 0 || both) {
       const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
       const unsigned my_s = tm_s + t * 128 + lanes, my_o = tm_o + t * kStepO + lanes,
                      my_p = tm_p + t * kStepP + lanes;
       const uint4* keep_row =
           a.bits ? reinterpret_cast<const uint4*>(a.bits + b * a.bits_b + h * a.bits_h +
-                                                  (long long)min(i, a.Lq - 1) * a.bits_q)
+                                                  (long long)i * a.bits_q)
                  : nullptr;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
@@ -263,19 +286,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const float lse = l == 0.0f ? -INFINITY : m * p.scale_log2 * 0.6931471805599453f + logf(l);
-      const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
+      const long long row = ((long long)b * a.Hq + h0) * a.Lq + row_q;
       const long long rows = (long long)a.B * a.Hq * a.Lq;
-      // the tile's queries in shared memory have done their work
-      const int i0 = i - (int)threadIdx.x % 32;
       const bool wide = p.splits > 1;
-      char* to = wide ? reinterpret_cast<char*>(
-                            p.part_out +
-                            (blockIdx.y * rows + row - (int)threadIdx.x % 32) * a.D)
-                      : reinterpret_cast<char*>(a.out.at<T>(b, i0, h));
+      // rows of several heads follow one another in the parts, but not in `out`
+      const int lane = threadIdx.x % 32;
+      char* to;
+      if (wide)
+        to = reinterpret_cast<char*>(p.part_out + (blockIdx.y * rows + row - lane) * a.D);
+      else if (p.pack > 1)
+        to = reinterpret_cast<char*>(a.out.at<T>(b, i, h));
+      else
+        to = reinterpret_cast<char*>(a.out.at<T>(b, row_q - lane, h0));
+      // the tile's queries in shared memory have done their work
       store_rows<T, DP>(my_o, ok && count > 0, l != 0.0f, inv, a.D, wide,
                         sm_q + t * S::kTileBytes + warp % 4 * (DP * 64), to,
-                        wide ? a.D * 4ll : a.out.l * 2, a.Lq - i0);
-      if (i < a.Lq) {
+                        wide ? a.D * 4ll : p.pack > 1 ? 0 : a.out.l * 2,
+                        queries - row_q + lane);
+      if (live) {
         if (p.splits > 1)
           p.part_lse[blockIdx.y * rows + row] = lse;
         else if (a.lse)
@@ -386,7 +414,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 }
 
 // out = sum over splits of exp(lse_s - lse) out_s: WARPS warps for each row, each with every
-// WARPS-th split, a lane for 4 of the row's numbers. 4 warps where there are more than 8 splits.
+// WARPS-th split, a lane for 4 of the row's numbers. 4 warps where there are more than 8 splits:
+// with the forward before it 256 x 30,000 of 2 heads of 64 then takes 19.8 us instead of 25.0 with
+// one warp, but 1,000 x 8,160 (up to 8 splits) 17.7 with one and 19.2 with four.
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(128) combine_kernel(AttentionParams a, int splits,
                                                       const float* part_out,
@@ -461,34 +491,46 @@ __global__ void __launch_bounds__(128) combine_kernel(AttentionParams a, int spl
 }
 
 struct ForwardPlan {
-  int tiles, splits;
+  int pack, tiles, splits;
 };
 
-// Query tiles a CTA and splits of the keys (each with at least two tiles of keys, and all in one
-// wave of CTAs), by the time they should take in us: waves of CTAs, each with some 4 us to begin
+// How many query heads that share a key head go into one tile (1, or as many as fit with all their
+// queries), query tiles a CTA and splits of the keys (each with at least two tiles of keys, and all in
+// one wave of CTAs), by the time they should take in us: waves of CTAs, each with some 4 us to begin
 // and end and, for a tile of keys, what one and two query tiles take together (measured: 1.35 and
 // 1.65 at D 64, 1.7 and 2.2 at D 128); joining splits takes another launch and the parts' way
 // through memory.
 static ForwardPlan forward_plan(const gs_attention_args& a) {
-  const double heads = (double)a.B * a.Hq;
-  const int q_tiles = (a.Lq + kTileQ - 1) / kTileQ, key_tiles = (a.Lk + kTileK - 1) / kTileK;
-  const double part_us = heads * a.Lq * a.D * 8.0 / 3e6;
-  ForwardPlan best{2, 1};
+  const int shared = a.Hq / a.Hkv, key_tiles = (a.Lk + kTileK - 1) / kTileK;
+  const double part_us = (double)a.B * a.Hq * a.Lq * a.D * 8.0 / 3e6;
+  int most = shared;
+  while (most > 1 && (shared % most || (long long)most * a.Lq > kTileQ)) --most;
+  ForwardPlan best{1, 2, 1};
   double least = 1e30;
-  for (int tiles = 2; tiles >= 1; --tiles) {
-    const double ctas = heads * ((q_tiles + tiles - 1) / tiles);
-    const double step = a.D <= 64 ? (tiles == 2 ? 1.65 : 1.35) : (tiles == 2 ? 2.2 : 1.7);
-    for (int splits = 1; splits == 1 || (splits <= key_tiles / 2 && ctas * splits <= kSms);
-         ++splits) {
-      const double us = std::ceil(ctas * splits / kSms) *
-                            (4.0 + step * ((key_tiles + splits - 1) / splits)) +
-                        (splits > 1 ? 4.0 + part_us * splits : 0.0);
-      if (us < least) {
-        least = us;
-        best = {tiles, splits};
+  for (int tiles = 2; tiles >= 1; --tiles)
+    for (int pack = 1;; pack = most) {
+      const int q_tiles = (int)(((long long)pack * a.Lq + kTileQ - 1) / kTileQ);
+      const double ctas = (double)a.B * (a.Hq / pack) * ((q_tiles + tiles - 1) / tiles);
+      const double step = a.D <= 64 ? (tiles == 2 ? 1.65 : 1.35) : (tiles == 2 ? 2.2 : 1.7);
+      const auto consider = [&](int splits) {
+        const double us = std::ceil(ctas * splits / kSms) *
+                              (4.0 + step * ((key_tiles + splits - 1) / splits)) +
+                          (splits > 1 ? 4.0 + part_us * splits : 0.0);
+        if (us < least) {
+          least = us;
+          best = {pack, tiles, splits};
+        }
+      };
+      consider(1);
+      // more splits than that take longer to join than they save
+      const double enough = std::sqrt(step * key_tiles / part_us);
+      const int splits = (int)std::min({enough + 1.0, (double)(key_tiles / 2), kSms / ctas});
+      if (splits > 1) {
+        const int longest = (key_tiles + splits - 1) / splits;
+        consider((key_tiles + longest - 1) / longest);  // the fewest with tiles that long
       }
+      if (pack == most) break;
     }
-  }
   return best;
 }
 
@@ -505,8 +547,7 @@ static cudaError_t launch_forward(const ForwardParams& p, const CUtensorMap& q,
   const auto kernel = attention_forward_kernel<T, DP>;
   const cudaError_t err = allow_shared<attention_forward_kernel<T, DP>>(ForwardShared<DP>::kBytes);
   if (err != cudaSuccess) return err;
-  const int rows = p.tiles * kTileQ;
-  const dim3 grid((p.a.Lq + rows - 1) / rows * p.a.B * p.a.Hq, p.splits);
+  const dim3 grid(p.q_blocks * p.a.B * p.groups, p.splits);
   return launch_overlapped(kernel, grid, kFwdThreads, ForwardShared<DP>::kBytes, stream, p, q, k, v);
 }
 
@@ -537,8 +578,11 @@ int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t 
   p.lag = std::min(kLag / p.scale_log2, 1e30f);
   p.negate = a.scale < 0.0f;
   const ForwardPlan plan = forward_plan(a);
+  p.pack = plan.pack;
   p.tiles = plan.tiles;
   p.splits = plan.splits;
+  p.groups = a.Hq / p.pack, p.shared = a.Hq / a.Hkv;
+  p.q_blocks = (int)(((long long)p.pack * a.Lq + p.tiles * kTileQ - 1) / (p.tiles * kTileQ));
   const size_t mask_bytes = attention_mask_bytes(a);
   if (const int status = attention_pack_mask(a, p.a, workspace, stream)) return status;
   p.part_out = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);
@@ -549,7 +593,7 @@ int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t 
   p.vb = a.B > 1 && a.v.batch_stride != 0, p.vh = a.Hkv > 1;
   CUtensorMap q, k, v;
   GS_REQUIRE(encode_tokens(&q, a.dtype, a.q.data, a.D, a.Lq, a.Hq, a.B, a.q.token_stride,
-                           a.q.head_stride, a.q.batch_stride, kTileQ),
+                           a.q.head_stride, a.q.batch_stride, plan.pack > 1 ? a.Lq : kTileQ, plan.pack),
              "the driver refused to describe q");
   k = v = q;  // without keys nothing is copied
   if (a.Lk > 0) {

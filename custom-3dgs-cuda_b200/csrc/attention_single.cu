@@ -1,7 +1,9 @@
-// Cross attention forward for single queries: up to 16 rows share the keys of a (batch item, key
-// head), counting the query heads that share the key head and the queries of each.
+// Cross attention forward for single queries: up to 16 rows (D above 64: 8) share the keys of a
+// (batch item, key head), counting the query heads that share the key head and the queries of each.
 //
-// Bound by HBM: every key and value is read once, for 1 to 16 rows of work on it. So nothing is
+// Bound by HBM: every key and value is read once, for a few rows of work on it. 2 x 65,280 keys, 32
+// query heads on 8 of 128, half: 96 us, 5.6 TB/s; 4 x 3,600 keys of 16 heads of 64: 17 us, of which
+// the loads' latency is the larger part (five rounds of them a warp). So nothing is
 // staged: each lane loads 16 bytes of a row of k or v straight into the registers in which the
 // warp-wide product (16 x 8 x 16) takes them. The product's contraction index may be numbered
 // freely as long as both operands agree, which turns a lane's 8 consecutive numbers into the
@@ -299,8 +301,12 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
   }
 }
 
+// Against the kernel with tiles of 128 rows, in us with the joining of the splits: up to 8 rows 93
+// against 106 (2 x 65,280 keys, 8 heads of 128) and 18 against 26 (4 x 3,600, 16 of 64), 9 to 16 rows
+// at D up to 64 66 against 76 (2 x 65,280, 8 heads) and 24 against 26 (4 x 3,600, 16 heads); above,
+// where two groups of rows leave 2 CTAs an SM, it loses: 126 against 106, 40 against 35.
 bool attention_is_single(const gs_attention_args& a) {
-  return a.Hkv > 0 && (long long)a.Lq * (a.Hq / a.Hkv) <= 16;
+  return a.Hkv > 0 && (long long)a.Lq * (a.Hq / a.Hkv) <= (a.D <= 64 ? 16 : 8);
 }
 
 // Splits of the keys: one wave of CTAs, each with at least two chunks for every warp.
@@ -320,9 +326,11 @@ size_t attention_single_workspace(const gs_attention_args& a) {
 template <typename T, int DP>
 static cudaError_t launch_single(const SingleParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)p.a.B * p.a.Hkv, p.splits);
-  if (p.rows <= 8)
-    return launch_overlapped(attention_single_kernel<T, DP, 1>, grid, kSingleWarps * 32, 0, stream, p);
-  return launch_overlapped(attention_single_kernel<T, DP, 2>, grid, kSingleWarps * 32, 0, stream, p);
+  if constexpr (DP == 64)
+    if (p.rows > 8)
+      return launch_overlapped(attention_single_kernel<T, DP, 2>, grid, kSingleWarps * 32, 0, stream,
+                               p);
+  return launch_overlapped(attention_single_kernel<T, DP, 1>, grid, kSingleWarps * 32, 0, stream, p);
 }
 
 int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t stream) {

@@ -231,9 +231,9 @@ __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float lo, float hi) {
 
 // Writes COLS columns from `addr` on of the warp's 32 accumulator rows, times `factor`, as far as
 // `left` columns go (a multiple of 8): rounded to T, or in 32 bits (`wide`), to rows `pitch` bytes
-// apart from `to` on, of which the first `rows` exist. Where there is nothing to read (`have` false,
-// for the whole warp) or the lane's row counts for nothing (`live` false) zeros are written. The rows
-// pass through COLS * 64 bytes of shared memory at `stage`, of this warp alone, so that neighbouring
+// apart from `to` on or, with a pitch of 0, each lane's row to its own `to`; the first `rows` rows
+// exist. Where there is nothing to read (`have` false, for the whole
+// warp) or the lane's row counts for nothing (`live` false) zeros are written. The rows pass through COLS * 64 bytes of shared memory at `stage`, of this warp alone, so that neighbouring
 // lanes write neighbouring 16 bytes: a lane writing its own row would touch 32 lines at a time. The
 // loop that writes is kept short: it runs once a CTA, from a cold instruction cache.
 template <typename T, int COLS>
@@ -277,7 +277,6 @@ __device__ __forceinline__ void store_rows(unsigned addr, bool have, bool live, 
     }
     __syncwarp();
     const int c = lane % kPieces, column = wide ? half * (COLS / 2) + c * 4 : c * 8;
-    char* out = to + column * (wide ? 4 : 2);
 #pragma unroll 2
     for (int r = lane / kPieces; r < 32; r += 32 / kPieces) {
       uint4 w;
@@ -285,7 +284,10 @@ __device__ __forceinline__ void store_rows(unsigned addr, bool have, bool live, 
                    : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                    : "r"(stage + r * kPieces * 16 + ((c ^ (r & kSwizzle)) << 4))
                    : "memory");
-      if (r < rows && column < left) *reinterpret_cast<uint4*>(out + r * pitch) = w;
+      char* row = to + r * pitch;
+      if (!pitch)
+        row = reinterpret_cast<char*>(__shfl_sync(~0u, reinterpret_cast<uintptr_t>(to), r));
+      if (r < rows && column < left) *reinterpret_cast<uint4*>(row + column * (wide ? 4 : 2)) = w;
     }
     __syncwarp();
   }
@@ -321,12 +323,12 @@ __device__ __forceinline__ Two add2(Two a, Two b) {
 }
 
 // Host: describes a [B, L, H, D] tensor of 16-bit numbers as (D, L, H, B), innermost first, copied
-// in boxes of 64 numbers x `rows` tokens of one head, 128-byte-swizzled; what lies past D or L
+// in boxes of 64 numbers x `rows` tokens x `heads` heads, 128-byte-swizzled; what lies past D or L
 // reads as zero. Axes of one element, and a batch stride of 0 (all items alike), are encoded as
 // one element: the caller passes coordinate 0 there.
 inline bool encode_tokens(CUtensorMap* map, int dtype, const void* base, int D, int L, int H,
                           int B, long long stride_l, long long stride_h, long long stride_b,
-                          unsigned rows) {
+                          unsigned rows, unsigned heads = 1) {
   const EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return false;
   const auto one = [](long long n, long long stride) { return n <= 1 || stride == 0; };
@@ -337,7 +339,7 @@ inline bool encode_tokens(CUtensorMap* map, int dtype, const void* base, int D, 
   const cuuint64_t strides[3] = {one(L, stride_l) ? row : (cuuint64_t)stride_l * 2,
                                  one(H, stride_h) ? row : (cuuint64_t)stride_h * 2,
                                  one(B, stride_b) ? row : (cuuint64_t)stride_b * 2};
-  const cuuint32_t box[4] = {64, rows, 1, 1};
+  const cuuint32_t box[4] = {64, rows, heads, 1};
   const cuuint32_t elem[4] = {1, 1, 1, 1};
   return fn(map,
             dtype == GS_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,

@@ -314,3 +314,20 @@ def test_back_to_back_calls_do_not_overtake_one_another(cuda_device):
     apart = chain(torch.cuda.synchronize)
     for _ in range(5):
         assert torch.equal(chain(lambda: None), apart)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(2, 1, 900, 48, 2, 64), (1, 1, 2000, 128, 1, 128),
+                                  (1, 5, 700, 16, 4, 80), (2, 10, 1333, 24, 2, 64),
+                                  (1, 30, 5000, 12, 2, 64), (40, 64, 257, 4, 1, 128),
+                                  (1, 1, 600, 130, 1, 64), (1, 3, 290, 43, 1, 64),
+                                  (30, 9, 70, 16, 2, 96), (1, 12, 1000, 2, 2, 128)])
+def test_few_queries_of_many_shared_heads(cuda_device, dtype, size):
+    """More rows for each key head than the single-query form takes, fewer queries than a tile."""
+    B, Lq, Lk, Hq, Hkv, D = size
+    q, k, v, g = draw(cuda_device, dtype, *size, seed=8)
+    apart = q.transpose(1, 2).contiguous().transpose(1, 2)  # heads outside of queries
+    check(apart, k, v, g)
+    t = torch.arange(B, device=cuda_device, dtype=torch.int32) * 131 % (Lk + 1)
+    for kind in ("key", "query", "head", "full"):
+        check(q, k, v, lengths=t, mask=masks(cuda_device, B, Hq, Lq, Lk, kind))
