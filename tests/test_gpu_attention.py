@@ -331,3 +331,12 @@ def test_few_queries_of_many_shared_heads(cuda_device, dtype, size):
     t = torch.arange(B, device=cuda_device, dtype=torch.int32) * 131 % (Lk + 1)
     for kind in ("key", "query", "head", "full"):
         check(q, k, v, lengths=t, mask=masks(cuda_device, B, Hq, Lq, Lk, kind))
+
+
+def test_no_second_derivative(cuda_device):
+    from gs3d_b200.attention import cross_attention
+
+    q, k, v, _ = draw(cuda_device, torch.bfloat16, 1, 4, 6, 1, 1, 8)
+    q.requires_grad_()
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(cross_attention(q, k, v).sum(), q, create_graph=True)

@@ -174,3 +174,30 @@ def test_only_one_output_used(cuda_device):
     ref, _ = norm_backward64(dy, None, h.detach(), w, 1e-6)
     torch.testing.assert_close(dx.double(), ref, rtol=1e-4, atol=1e-5)
     assert torch.equal(dx, dr)
+
+
+@pytest.mark.parametrize("group", (0, 128))
+def test_8bit_rows_of_tiny_numbers(cuda_device, group):
+    """max|y| / 448 below the smallest normal number, whose reciprocal would be infinite."""
+    from gs3d_b200.norm import rms_norm_8bit
+
+    x = torch.randn(3, 256, device=cuda_device)
+    x[:, ::3] = 0.0
+    w = torch.full((256,), 2.0 ** -124, device=cuda_device)
+    q, s = rms_norm_8bit(x, w, group=group)
+    assert bool((s >= 2.0 ** -126).all())
+    assert not q.float().isnan().any() and not q.float()[:, ::3].any()
+    y = (x.double() * torch.rsqrt((x.double() ** 2).mean(-1, keepdim=True) + 1e-6)) * w.double()
+    got = (q.double().view(3, -1, 256 if group == 0 else 128) * s.double().unsqueeze(-1)).view(3, 256)
+    # 4 bits of precision: half a step of 2^-3 relative, or of 2^-9 of the scale near zero
+    assert bool(((got - y).abs() <= y.abs() * (2.0 ** -4 + 2.0 ** -18)
+                 + 2.0 ** -10 * s.double().amax(-1, keepdim=True)).all())
+
+
+def test_no_second_derivative(cuda_device):
+    from gs3d_b200.norm import rms_norm
+
+    x = torch.randn(4, 64, device=cuda_device, requires_grad=True)
+    w = torch.ones(64, device=cuda_device, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(rms_norm(x, w).sum(), x, create_graph=True)
