@@ -340,3 +340,31 @@ def test_no_second_derivative(cuda_device):
     q.requires_grad_()
     with pytest.raises(RuntimeError, match="no second derivative"):
         torch.autograd.grad(cross_attention(q, k, v).sum(), q, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(3, 300, 900, 28, 7, 64), (2, 600, 800, 30, 5, 128),
+                                  (32, 257, 500, 5, 5, 40), (1, 5000, 700, 8, 2, 80)])
+def test_more_blocks_of_queries_than_run_at_once(cuda_device, dtype, size):
+    """Between one and three waves of CTAs, with every kind of mask."""
+    B, Lq, Lk, Hq, Hkv, D = size
+    q, k, v, g = draw(cuda_device, dtype, *size, seed=9)
+    check(q, k, v, g)
+    t = torch.arange(B, device=cuda_device, dtype=torch.int32) * 131 % (Lk + 1)
+    for kind in ("key", "query", "head"):
+        check(q, k, v, lengths=t if B > 1 else None,
+              mask=masks(cuda_device, B, Hq, Lq, Lk, kind))
+
+
+@pytest.mark.parametrize("D", (64, 128))
+def test_one_item_much_longer_than_the_others(cuda_device, D):
+    """Items without keys beside one with many, infinities past the ends."""
+    lengths = [0, 1, 4000, 0, 130, 128, -3, 129, 1] + [1] * 10 + [0]
+    B, Lk = len(lengths), 4000
+    q, k, v, _ = draw(cuda_device, torch.bfloat16, B, 257, Lk, 4, 2, D, seed=10)
+    for b, n in enumerate(lengths):
+        k[b, max(n, 0):] = float("nan") if b % 2 else float("inf")
+        v[b, max(n, 0):] = float("inf") if b % 2 else float("nan")
+    t = torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    check(q, k, v, lengths=t)
+    check(q, k, v, lengths=t.clamp(max=1), mask=masks(cuda_device, B, 4, 257, Lk, "key"))
