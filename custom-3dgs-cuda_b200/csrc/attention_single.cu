@@ -2,8 +2,8 @@
 // (batch item, key head), counting the query heads that share the key head and the queries of each.
 //
 // Bound by HBM: every key and value is read once, for a few rows of work on it. 2 x 65,280 keys, 32
-// query heads on 8 of 128, half: 96 us, 5.6 TB/s; 4 x 3,600 keys of 16 heads of 64: 17 us, of which
-// the loads' latency is the larger part (five rounds of them a warp). So nothing is
+// query heads on 8 of 128, half: 96 us, 5.6 TB/s; 4 x 3,600 keys of 16 heads of 64: 17.7 us,
+// of which the loads' latency is the larger part (five rounds of them a warp). So nothing is
 // staged: each lane loads 16 bytes of a row of k or v straight into the registers in which the
 // warp-wide product (16 x 8 x 16) takes them. The product's contraction index may be numbered
 // freely as long as both operands agree, which turns a lane's 8 consecutive numbers into the
@@ -13,7 +13,8 @@
 //   and interleaves pairs of them by byte permutes; P^T is S^T's fragment transposed in 8 x 8.
 // Rows are columns of both results, so the running maximum of a row is rescaled in place.
 // A warp walks over chunks of 16 keys (D above 64) or 32, the next chunk's loads in flight while
-// it works on this one; CTAs of 4 warps split the keys, and combine_kernel joins them.
+// it works on this one; CTAs of 4 warps split the keys, and a cluster joins its CTAs' parts or, where
+// there are more than 8, combine_kernel.
 #include <algorithm>
 #include <cmath>
 
@@ -24,6 +25,7 @@
 namespace gs {
 
 constexpr int kSingleWarps = 4;
+constexpr int kClusterSplits = 8;  // at most, of those that a cluster joins
 // resident CTAs an SM, by groups of 8 rows: 168 registers a thread hold one, 255 two
 constexpr int single_ctas(int groups) { return groups == 1 ? 3 : 2; }
 
@@ -31,6 +33,7 @@ struct SingleParams {
   AttentionParams a;
   float scale_log2;  // scale * log2 e
   int splits, rows;  // rows = Lq * Hq / Hkv
+  int cluster;       // the splits of a key head are a cluster, which joins them itself
   float* part_out;
   float* part_lse;
 };
@@ -76,6 +79,32 @@ __device__ __forceinline__ uint4 load16(const void* p, bool in) {
 
 __device__ __forceinline__ unsigned part(const uint4& v, int u) {
   return u == 0 ? v.x : u == 1 ? v.y : u == 2 ? v.z : v.w;
+}
+
+// The barrier of a cluster's threads, and shared memory of its CTA `rank` where this CTA's p is.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ unsigned cluster_address(const void* p, int rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float cluster_load(const float* p, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_address(p, rank))
+               : "memory");
+  return v;
 }
 
 // DP: head size rounded up to 64 or 128. NT: groups of 8 rows.
@@ -248,7 +277,9 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
   }
 
   // the warps' results meet: M = max m, weights 2^(m - M)
-  __shared__ float s_m[kSingleWarps][8], s_l[kSingleWarps][8], s_o[kSingleWarps][8][DP];
+  __shared__ float s_m[kSingleWarps][8], s_l[kSingleWarps][8];
+  __shared__ __align__(16) float s_o[kSingleWarps][8][DP], s_part[NT * 8][DP];
+  __shared__ float s_lse[NT * 8];  // to base 2
   const long long all_rows = (long long)a.B * a.Hq * a.Lq;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -285,7 +316,12 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = l == 0.0f ? 0.0f : acc[i] * inv;
-      const float lse = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+      const float lse2 = l == 0.0f ? -INFINITY : top + log2f(l), lse = lse2 * 0.6931471805599453f;
+      if (p.cluster) {
+        *reinterpret_cast<float4*>(&s_part[r][d]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (d == 0) s_lse[r] = lse2;
+        continue;
+      }
       const int i = r / shared_heads, h = head_of(r);
       const long long row = ((long long)b * a.Hq + h) * a.Lq + i;
       if (p.splits > 1) {
@@ -299,6 +335,40 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
       }
     }
   }
+  if (!p.cluster) return;
+  // out = sum over splits of 2^(lse_s - lse) out_s, from the shared memory of the cluster's CTAs, each
+  // of which takes its share of the numbers
+  cluster_arrive();
+  cluster_wait();
+  for (int k = threadIdx.x * p.splits + blockIdx.y; k < p.rows * (DP / 4);
+       k += kSingleWarps * 32 * p.splits) {
+    const int r = k / (DP / 4), d = k % (DP / 4) * 4;
+    if (d >= a.D) continue;
+    float top = -INFINITY, total = 0.0f, acc[4] = {}, w[kClusterSplits];
+    float4 v[kClusterSplits];
+#pragma unroll
+    for (int s = 0; s < kClusterSplits; ++s) {
+      w[s] = s < p.splits ? cluster_load(&s_lse[r], s) : -INFINITY;
+      v[s] = s < p.splits ? cluster_load4(&s_part[r][d], s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      top = max_nan(top, w[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < kClusterSplits; ++s) {
+      const float f = top == -INFINITY ? 0.0f : fast_exp2(w[s] - top);
+      total += f;
+      acc[0] = fmaf(f, v[s].x, acc[0]), acc[1] = fmaf(f, v[s].y, acc[1]);
+      acc[2] = fmaf(f, v[s].z, acc[2]), acc[3] = fmaf(f, v[s].w, acc[3]);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const int i = r / shared_heads, h = head_of(r);
+    *reinterpret_cast<uint2*>(a.out.at<T>(b, i, h) + d) =
+        make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+    if (d == 0 && a.lse)
+      a.lse[((long long)b * a.Hq + h) * a.Lq + i] =
+          total == 0.0f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
+  }
+  cluster_arrive();  // the others may still be reading this CTA's memory
+  cluster_wait();
 }
 
 // Against the kernel with tiles of 128 rows, in us with the joining of the splits: up to 8 rows 93
@@ -309,28 +379,35 @@ bool attention_is_single(const gs_attention_args& a) {
   return a.Hkv > 0 && (long long)a.Lq * (a.Hq / a.Hkv) <= (a.D <= 64 ? 16 : 8);
 }
 
-// Splits of the keys: one wave of CTAs, each with at least two chunks for every warp.
+// Splits of the keys: one wave of CTAs, each with at least two chunks for every warp. Up to 8 of them
+// are a cluster, which joins its parts through shared memory (4 x 3,600 keys of 16 heads of 64: 17.7 us,
+// 20.0 with a second kernel), so there are 8 rather than a few more, and where a warp has at most
+// 4 chunks with 8 (2 x 3,600, 16 heads of 64: 13.6 us with 8, 15.0 with 13; 3 x 8,160: 24.6 with 8, 26.5
+// with 9; but 2 x 16,320: 34.0 with 8, 31.0 with 13).
 static int single_splits(const gs_attention_args& a) {
   const long long pairs = (long long)a.B * a.Hkv;
   const long long chunk = a.D <= 64 ? 32 : 16;
   const long long most = a.Lk / (2 * kSingleWarps * chunk);
   const long long wave = kSms * single_ctas((long long)a.Lq * (a.Hq / a.Hkv) <= 8 ? 1 : 2);
-  return (int)std::max(1ll, std::min(wave / std::max(1ll, pairs), most));
+  const long long splits = std::max(1ll, std::min(wave / std::max(1ll, pairs), most));
+  const bool short_enough = a.Lk <= 4 * kClusterSplits * kSingleWarps * chunk;
+  return (int)(splits > kClusterSplits && (splits <= 10 || short_enough) ? kClusterSplits : splits);
 }
 
 size_t attention_single_workspace(const gs_attention_args& a) {
   const long long splits = single_splits(a), rows = (long long)a.B * a.Hq * a.Lq;
-  return splits > 1 ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0;
+  return splits > kClusterSplits ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0;
 }
 
 template <typename T, int DP>
 static cudaError_t launch_single(const SingleParams& p, cudaStream_t stream) {
-  const dim3 grid((unsigned)p.a.B * p.a.Hkv, p.splits);
+  const dim3 grid((unsigned)p.a.B * p.a.Hkv, p.splits), cluster(1, p.cluster ? p.splits : 1);
   if constexpr (DP == 64)
     if (p.rows > 8)
-      return launch_overlapped(attention_single_kernel<T, DP, 2>, grid, kSingleWarps * 32, 0, stream,
-                               p);
-  return launch_overlapped(attention_single_kernel<T, DP, 1>, grid, kSingleWarps * 32, 0, stream, p);
+      return launch_overlapped_clusters(attention_single_kernel<T, DP, 2>, grid, cluster,
+                                        kSingleWarps * 32, 0, stream, p);
+  return launch_overlapped_clusters(attention_single_kernel<T, DP, 1>, grid, cluster,
+                                    kSingleWarps * 32, 0, stream, p);
 }
 
 int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t stream) {
@@ -339,6 +416,7 @@ int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t s
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.rows = a.Lq * (a.Hq / a.Hkv);
   p.splits = single_splits(a);
+  p.cluster = p.splits > 1 && p.splits <= kClusterSplits;
   const long long rows = (long long)a.B * a.Hq * a.Lq;
   p.part_out = static_cast<float*>(workspace);
   p.part_lse = p.part_out + p.splits * rows * a.D;
@@ -349,7 +427,7 @@ int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t s
     GS_CUDA(a.D <= 64 ? (launch_single<__nv_bfloat16, 64>(p, stream))
                       : (launch_single<__nv_bfloat16, 128>(p, stream)));
   count_launches(1u);
-  if (p.splits > 1) {
+  if (p.splits > kClusterSplits) {
     GS_CUDA(attention_combine(a, p.splits, p.part_out, p.part_lse, stream));
     count_launches(1u);
   }

@@ -16,21 +16,30 @@ __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Launches a kernel that may start before the previous one in the stream has ended.
+// Launches a kernel that may start before the previous one in the stream has ended, in clusters of
+// `cluster` CTAs.
 template <typename... Params, typename... Args>
-cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, unsigned threads,
-                              size_t shared, cudaStream_t stream, const Args&... args) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch_overlapped_clusters(void (*kernel)(Params...), dim3 grid, dim3 cluster,
+                                       unsigned threads, size_t shared, cudaStream_t stream,
+                                       const Args&... args) {
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim = {cluster.x, cluster.y, cluster.z};
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = shared;
   config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, unsigned threads,
+                              size_t shared, cudaStream_t stream, const Args&... args) {
+  return launch_overlapped_clusters(kernel, grid, dim3(1), threads, shared, stream, args...);
 }
 
 }  // namespace gs
