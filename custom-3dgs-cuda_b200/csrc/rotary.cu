@@ -13,9 +13,9 @@
 //
 // Bound by HBM: every element is read once and written once. The angles depend on the token and
 // the pair but not on the head, so a thread keeps VEC pairs' sines and cosines and walks over
-// heads, the loads of FLIGHT heads in flight at once. 5.6 TB/s at 65,280 tokens of 16 heads of 64
-// bfloat16 with neighbouring pairs, 5.0 TB/s with pairs half a block apart, whose accesses split
-// 32-byte sectors. (Staging whole rows in shared memory to mend that took 115 us instead of 54.)
+// heads, the loads of FLIGHT heads in flight at once. 65,280 tokens of 16 heads of 64 bfloat16 take
+// 54 us (5.0 TB/s) with neighbouring pairs and 59 with pairs half a block apart, 55 in the kernel
+// below that reads and writes those in whole lines. (Staging whole rows in shared memory took 115.)
 #include <algorithm>
 #include <cmath>
 
@@ -50,6 +50,22 @@ struct RotaryParams {
   int axis_start[kRotaryMaxAxes + 1];  // first pair of each axis; [n_axes] = turned
   float freq_hi[kRotaryMaxPairs], freq_lo[kRotaryMaxPairs];  // turns per unit of position
 };
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(unsigned v);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(unsigned v) {
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ unsigned pack_pair(float lo, float hi) {
+  return (unsigned)__builtin_bit_cast(unsigned short, from_f32<T>(lo)) |
+         (unsigned)__builtin_bit_cast(unsigned short, from_f32<T>(hi)) << 16;
+}
 
 template <typename T, int VEC, bool INTERLEAVED, typename P, int FLIGHT>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__
@@ -135,6 +151,118 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
       *reinterpret_cast<Pack<T, VEC>*>(y + h * p.yh + off_v) = v[k];
     }
   }
+}
+
+// Pairs half a block apart, 16-bit numbers, blocks of multiples of 8 numbers: a lane holds 8 numbers of
+// a head that follow one another, in groups of 4, and gets their partners from the lanes that hold
+// them, so that whole lines are read and written, with half as many accesses; the next heads' loads
+// are in flight beside this ones' arithmetic. A lane forms the angles of 4 pairs. Against the kernel
+// above at 16 heads a thread, in us: 65,280 tokens of 16 heads of 64 55 and 59, 32,640 of them 33 and 35,
+// 65,280 of 8 heads of 128 58 and 59; at fewer heads a thread it loses (16,320 tokens: 19 and 17).
+template <typename T, typename P>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_rows_kernel(const __grid_constant__
+                                                                     RotaryParams p) {
+  constexpr int kFlight = 4;
+  __shared__ float s_hi[kRotaryMaxPairs], s_lo[kRotaryMaxPairs];
+  for (int i = threadIdx.x; i < p.turned; i += blockDim.x) {
+    s_hi[i] = p.freq_hi[i];
+    s_lo[i] = p.freq_lo[i];
+  }
+  __syncthreads();
+  const int lanes = p.pairs / 4, in_warp = 32 / lanes;  // of a head, and heads a warp holds
+  const int lane = threadIdx.x % 32, slot = lane / lanes, i = lane - slot * lanes, lane0 = slot * lanes;
+  const unsigned at = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * in_warp + slot;
+  const unsigned token = at / (unsigned)p.head_lanes;
+  const int lane_h = at - token * p.head_lanes;
+  const int H = slot < in_warp && token < p.tokens ? p.H : 0;  // no heads for the lanes left over
+  const unsigned b = token / (unsigned)p.L, l = token - b * p.L;
+  const T* x = reinterpret_cast<const T*>(p.x) + b * p.xb + l * p.xl + 8 * i;
+  T* y = reinterpret_cast<T*>(p.y) + b * p.yb + l * p.yl + 8 * i;
+  uint4 w[kFlight], ahead[kFlight];
+  const auto load = [&](uint4 (&w)[kFlight], int h0) {
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      w[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (h < H) w[k] = *reinterpret_cast<const uint4*>(x + h * p.xh);
+    }
+  };
+  wait_for_previous();
+  let_next_start();
+  load(w, lane_h);  // in flight while the angles are formed
+
+  const auto axis_of = [&](int pair) {
+    int axis = 0;
+#pragma unroll
+    for (int a = 1; a < kRotaryMaxAxes; ++a)
+      if (a < p.n_axes && pair >= p.axis_start[a]) axis = a;
+    return axis;
+  };
+  float c[4] = {}, s[4] = {};
+  if (4 * i < p.turned && H) {
+    const P raw = reinterpret_cast<const P*>(p.pos)[b * p.pos_b + l * p.pos_l + axis_of(4 * i)];
+    const float pos = p.sign * (float)raw;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float hi = s_hi[4 * i + k];
+      const float t = pos * hi;
+      const float err = fmaf(pos, hi, -t) + pos * s_lo[4 * i + k];
+      sincospif(2.0f * ((t - rintf(t)) + err), &s[k], &c[k]);
+    }
+  }
+  // this lane's numbers are 4 q, 4 q + 4 of its axis's block, whose pairs are `half` groups apart
+  const bool turned = 4 * i < p.turned;
+  const int axis = axis_of(4 * i), first = turned ? p.axis_start[axis] / 4 : i;
+  const int half = turned ? p.axis_start[axis + 1] / 4 - first : 1, q = 2 * (i - first);
+  int from[2];
+  float cs[2][4], sn[2][4];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const bool second = q + e >= half;
+    const int pair = second ? q + e - half : q + e;
+    from[e] = lane0 + first + (second ? pair : pair + half) / 2;
+    if (!turned) from[e] = lane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      cs[e][k] = __shfl_sync(~0u, c[k], lane0 + first + pair);
+      sn[e][k] = __shfl_sync(~0u, s[k], lane0 + first + pair);
+      if (!second) sn[e][k] = -sn[e][k];
+    }
+  }
+  const bool swap = half & 1;
+  for (int h0 = lane_h; __any_sync(~0u, h0 < H); h0 += kFlight * p.head_lanes) {
+    load(ahead, h0 + kFlight * p.head_lanes);
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      const unsigned own[2][2] = {{w[k].x, w[k].y}, {w[k].z, w[k].w}};
+      unsigned out[2][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const unsigned partner = __shfl_sync(~0u, swap ? own[1 - e][d] : own[e][d], from[e]);
+          const float2 a = unpack2<T>(own[e][d]), z = unpack2<T>(partner);
+          const float lo = fmaf(a.x, cs[e][2 * d], z.x * sn[e][2 * d]);
+          const float hi = fmaf(a.y, cs[e][2 * d + 1], z.y * sn[e][2 * d + 1]);
+          out[e][d] = turned ? pack_pair<T>(lo, hi) : own[e][d];
+        }
+      if (h < H)
+        *reinterpret_cast<uint4*>(y + h * p.yh) = make_uint4(out[0][0], out[0][1], out[1][0], out[1][1]);
+    }
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k) w[k] = ahead[k];
+  }
+}
+
+template <typename T>
+static cudaError_t launch_rotary_rows(const RotaryParams& p, int position_type,
+                                      cudaStream_t stream) {
+  const long long heads_a_cta = 4 * (32 / (p.pairs / 4));
+  const dim3 blocks((unsigned)(((long long)p.tokens * p.head_lanes + heads_a_cta - 1) / heads_a_cta));
+  return position_type == GS_FP32
+             ? launch_overlapped(rotary_rows_kernel<T, float>, blocks, 128, 0, stream, p)
+             : launch_overlapped(rotary_rows_kernel<T, int>, blocks, 128, 0, stream, p);
 }
 
 template <typename T, int VEC, bool INTERLEAVED, typename P>
@@ -245,11 +373,22 @@ extern "C" int gs_rotary_axes(int dtype, int B, int L, int H, int D, const gs_to
   p.threads = cta;
   p.flight = std::min(heads, 4);
   p.head_lanes = (H + heads - 1) / heads;
+  const cudaStream_t st = (cudaStream_t)stream;
+  // whole lines where there is work for 16 heads a thread (rotary_rows_kernel)
+  bool rows = heads == 16 && size == 2 && !interleaved && D % 8 == 0;
+  for (int a = 0; a < n_axes; ++a) rows = rows && axis_dims[a] % 8 == 0;
+  for (const long long stride : {p.xb, p.xl, p.xh, p.yb, p.yl, p.yh}) rows = rows && stride % 8 == 0;
+  rows = rows && (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y)) % 16 == 0;
+  if (rows) {
+    GS_CUDA(dtype == GS_FP16 ? launch_rotary_rows<__half>(p, position_type, st)
+                             : launch_rotary_rows<__nv_bfloat16>(p, position_type, st));
+    gs::count_launches(1u);
+    return GS_OK;
+  }
   while (p.head_lanes > 1 && p.items * p.head_lanes > cta)
     p.head_lanes = (p.head_lanes + 1) / 2;
   p.tokens_per_block = std::max(1, cta / (p.items * p.head_lanes));
   const unsigned blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-  const cudaStream_t st = (cudaStream_t)stream;
   GS_CUDA(dtype == GS_FP32   ? launch_rotary<float>(p, vec, position_type, blocks, st)
           : dtype == GS_FP16 ? launch_rotary<__half>(p, vec, position_type, blocks, st)
                              : launch_rotary<__nv_bfloat16>(p, vec, position_type, blocks, st));

@@ -107,3 +107,27 @@ def test_runs_on_the_current_stream(cuda_device):
     s.synchronize()
     ref, mag = rotary64(x * 2.0, pos, (64,), (10000.0,))
     assert_within(y, ref, 2.0 ** -20 * mag, "other stream")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", (False, True))
+@pytest.mark.parametrize("B,L,H,D,dims", [
+    (1, 20000, 17, 64, (16, 24, 24)), (1, 9000, 33, 80, (8, 16, 40, 16)),
+    (2, 3000, 16, 256, (64, 128)), (1, 160000, 16, 8, (8,)), (1, 20000, 17, 64, (20, 44))])
+def test_many_tokens(cuda_device, dtype, interleaved, B, L, H, D, dims):
+    """Work enough for 16 heads a thread; heads outside of tokens; NaN and infinities in what no
+    axis owns."""
+    g = torch.Generator(cuda_device).manual_seed(L + D)
+    x = torch.randn(B, H, L, D, generator=g, device=cuda_device).to(dtype).transpose(1, 2)
+    pos = torch.randint(-300, 300, (B, L, len(dims)), generator=g, device=cuda_device)
+    check(x, pos.to(torch.int32), dims, 100.0, interleaved)
+    y = check(x.contiguous(), pos.float() + 0.5, dims, 100.0, interleaved, True)
+    if sum(dims) < D:
+        bad = x.clone()
+        bad[..., sum(dims)::2], bad[..., sum(dims) + 1::2] = float("nan"), float("inf")
+        from gs3d_b200.rotary import rotary_axes
+
+        out = rotary_axes(bad, pos.float() + 0.5, dims, base=100.0, interleaved=interleaved,
+                          inverse=True)
+        assert torch.equal(out[..., :sum(dims)], y[..., :sum(dims)])
+        assert torch.equal(out[..., sum(dims):].isnan(), bad[..., sum(dims):].isnan())
