@@ -10,7 +10,7 @@
 //
 // What bounds it, at D 64, is the exponentials: 1,024 clocks of the special-function unit for a pair
 // of tiles whose two products take 512 (measured: that unit 69% busy, the tensor pipe 34%); at D 128
-// both take 1,024. One item of 4,096 queries, bfloat16: 16 heads of 64 x 8,160 keys 197 us, 700
+// both take 1,024. One item of 4,096 queries, bfloat16: 16 heads of 64 x 8,160 keys 193 us, 710
 // TFLOP/s; 16 heads of 128 x 4,096 keys 147 us, 940 TFLOP/s.
 //
 // The maximum that P is formed with may lag behind the true one by up to kLag powers of two: the
@@ -19,8 +19,9 @@
 // 16-bit types' range; its rounding to 16 bits (the products' operand type) is relative, so
 // nothing is lost. The row sum adds P before that rounding, in 32 bits.
 //
-// With few query tiles the keys are split over CTAs: each writes its normalised output in 32
-// bits and its lse, and combine_kernel joins them with weights exp(lse_split - lse). With few queries,
+// With few query tiles the keys are split over CTAs: each has its normalised output in 32 bits and
+// its lse, and the splits of a block, as a cluster through shared memory, or combine_kernel join them
+// with weights exp(lse_split - lse). With few queries,
 // heads that share a key head share a tile of rows too, so that k and v are read and multiplied once
 // for all of them (2 x 1 query x 65,280 keys, 24 heads on each of 8 of 128: 2,533 -> 106 us; 4 x 40 x
 // 3,600, 4 on each of 4 of 64: 24.3 -> 17.3).
@@ -51,6 +52,7 @@ struct ForwardParams {
   int pack;    // query heads a tile holds: above 1 it holds all queries of each
   int groups, shared, q_blocks;  // Hq / pack, Hq / Hkv, CTAs a group of heads
   int splits;
+  int cluster;  // the splits of a block are a cluster, which joins them itself
   int kb, kh, vb, vh, qb, qh;  // 0 where all batch items (heads) share the tensor, else 1
   float* part_out;  // [splits, B, Hq, Lq, D] where splits > 1
   float* part_lse;  // [splits, B, Hq, Lq]
@@ -74,6 +76,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t q_full, k_full[S::kStages], k_free[S::kStages], v_full[S::kStages],
       v_clean[S::kStages], v_free[S::kStages], s_full[2], s_read[2], p_ready[2], o_done[2], o_full[2], turn[2];
+  __shared__ float lse_part[2 * kTileQ];
   __shared__ unsigned tmem_slot;
   __shared__ volatile int gave_up;
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -298,16 +301,42 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         to = reinterpret_cast<char*>(a.out.at<T>(b, i, h));
       else
         to = reinterpret_cast<char*>(a.out.at<T>(b, row_q - lane, h0));
-      // the tile's queries in shared memory have done their work
-      store_rows<T, DP>(my_o, ok && count > 0, l != 0.0f, inv, a.D, wide,
-                        sm_q + t * S::kTileBytes + warp % 4 * (DP * 64), to,
-                        wide ? a.D * 4ll : p.pack > 1 ? 0 : a.out.l * 2,
-                        queries - row_q + lane);
-      if (live) {
-        if (p.splits > 1)
-          p.part_lse[blockIdx.y * rows + row] = lse;
-        else if (a.lse)
-          a.lse[row] = lse;
+      if (p.cluster) {
+        // the keys and values have done their work once both query tiles are through: the parts of the
+        // block take their place, rows of DP numbers in 16-byte pieces, swizzled
+        if (both)
+          asm volatile("bar.sync 2, 256;" ::: "memory");
+        else
+          asm volatile("bar.sync 2, 128;" ::: "memory");
+        const int r = t * kTileQ + threadIdx.x % 128;
+        for (int c = 0; c < DP; c += 32) {
+          unsigned o[32];
+          if (ok && count > 0) tc_ld32(my_o + c, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            float f[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) f[d] = l != 0.0f ? __uint_as_float(o[k + d]) * inv : 0.0f;
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             sm_k + r * (DP * 4) + (((c + k) / 4 ^ (r & 7)) << 4)),
+                         "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3])
+                         : "memory");
+          }
+        }
+        lse_part[r] = lse;
+      } else {
+        // the tile's queries in shared memory have done their work
+        store_rows<T, DP>(my_o, ok && count > 0, l != 0.0f, inv, a.D, wide,
+                          sm_q + t * S::kTileBytes + warp % 4 * (DP * 64), to,
+                          wide ? a.D * 4ll : p.pack > 1 ? 0 : a.out.l * 2,
+                          queries - row_q + lane);
+        if (live) {
+          if (p.splits > 1)
+            p.part_lse[blockIdx.y * rows + row] = lse;
+          else if (a.lse)
+            a.lse[row] = lse;
+        }
       }
     }
   } else {
@@ -411,6 +440,40 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     tc_fence_after();
     tc_free(tmem, 512);
   }
+  if (!p.cluster) return;
+  // out = sum over splits of exp(lse_s - lse) out_s from the shared memory of the cluster's CTAs, each
+  // of which takes every splits-th row
+  cluster_arrive();
+  cluster_wait();
+  const int rows = min(queries - q0, both ? 2 * kTileQ : kTileQ);
+  for (int at = threadIdx.x;; at += kFwdThreads) {
+    const int r = at / (DP / 4) * p.splits + blockIdx.y, c = at % (DP / 4);
+    if (r >= rows) break;
+    if (c * 4 >= a.D) continue;
+    float top = -INFINITY, total = 0.0f, acc[4] = {};
+    for (int s = 0; s < p.splits; ++s) top = max_nan(top, cluster_load(&lse_part[r], s));
+    for (int s = 0; s < p.splits; ++s) {
+      const float f = top == -INFINITY ? 0.0f : expf(cluster_load(&lse_part[r], s) - top);
+      const float4 v = cluster_load4(sm_k + r * (DP * 4) + ((c ^ (r & 7)) << 4), s);
+      total += f;
+      acc[0] = fmaf(f, v.x, acc[0]), acc[1] = fmaf(f, v.y, acc[1]);
+      acc[2] = fmaf(f, v.z, acc[2]), acc[3] = fmaf(f, v.w, acc[3]);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    int i = q0 + r, h = h0;
+    if (p.pack > 1) {
+      const int s = (unsigned)i / (unsigned)a.Lq;
+      h += s;
+      i -= s * a.Lq;
+    }
+    *reinterpret_cast<uint2*>(a.out.at<T>(b, i, h) + c * 4) =
+        make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+    if (c == 0 && a.lse)
+      a.lse[((long long)b * a.Hq + h0) * a.Lq + q0 + r] =
+          total == 0.0f ? -INFINITY : top + logf(total);
+  }
+  cluster_arrive();  // the others may still be reading this CTA's memory
+  cluster_wait();
 }
 
 // out = sum over splits of exp(lse_s - lse) out_s: WARPS warps for each row, each with every
@@ -534,10 +597,24 @@ static ForwardPlan forward_plan(const gs_attention_args& a) {
   return best;
 }
 
+// Whether a cluster joins the splits, rather than a second kernel: up to 4 of them, and where all
+// clusters still run at once, a cluster's CTAs having to lie in one part of the chip (pairs always find
+// their SMs; with 144 CTAs in threes some waited for a second round, 39 us instead of 25 at 3 x 128 x
+// 3,600, 16 heads of 64). It saves 1 to 4 us: 2 x 999 x 3,600, 8 heads of 64 in pairs 41 -> 37,
+// 2 x 128 x 3,600, 16 heads of 64 in fours 20.7 -> 19.4.
+static bool in_clusters(const gs_attention_args& a, const ForwardPlan& plan) {
+  const long long rows = plan.tiles * kTileQ;
+  const long long ctas = ((long long)plan.pack * a.Lq + rows - 1) / rows * a.B * (a.Hq / plan.pack);
+  return plan.splits == 2 ||
+         (plan.splits > 2 && plan.splits <= 4 && ctas * plan.splits <= 128);
+}
+
 size_t attention_forward_workspace(const gs_attention_args& a) {
-  const long long splits = forward_plan(a).splits, rows = (long long)a.B * a.Hq * a.Lq;
-  return attention_mask_bytes(a) +
-         (splits > 1 ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0);
+  const ForwardPlan plan = forward_plan(a);
+  const long long rows = (long long)a.B * a.Hq * a.Lq;
+  return attention_mask_bytes(a) + (plan.splits > 1 && !in_clusters(a, plan)
+                                        ? (size_t)(plan.splits * rows) * (a.D + 1) * sizeof(float)
+                                        : 0);
 }
 
 template <typename T, int DP>
@@ -548,7 +625,8 @@ static cudaError_t launch_forward(const ForwardParams& p, const CUtensorMap& q,
   const cudaError_t err = allow_shared<attention_forward_kernel<T, DP>>(ForwardShared<DP>::kBytes);
   if (err != cudaSuccess) return err;
   const dim3 grid(p.q_blocks * p.a.B * p.groups, p.splits);
-  return launch_overlapped(kernel, grid, kFwdThreads, ForwardShared<DP>::kBytes, stream, p, q, k, v);
+  return launch_overlapped_clusters(kernel, grid, dim3(1, p.cluster ? p.splits : 1), kFwdThreads,
+                                    ForwardShared<DP>::kBytes, stream, p, q, k, v);
 }
 
 template <typename T>
@@ -581,6 +659,7 @@ int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t 
   p.pack = plan.pack;
   p.tiles = plan.tiles;
   p.splits = plan.splits;
+  p.cluster = in_clusters(a, plan);
   p.groups = a.Hq / p.pack, p.shared = a.Hq / a.Hkv;
   p.q_blocks = (int)(((long long)p.pack * a.Lq + p.tiles * kTileQ - 1) / (p.tiles * kTileQ));
   const size_t mask_bytes = attention_mask_bytes(a);
@@ -611,7 +690,7 @@ int attention_forward(const gs_attention_args& a, void* workspace, cudaStream_t 
     GS_CUDA(a.D <= 64 ? (launch_forward<__nv_bfloat16, 64>(p, q, k, v, stream))
                       : (launch_forward<__nv_bfloat16, 128>(p, q, k, v, stream)));
   count_launches(1u);
-  if (p.splits > 1) {
+  if (p.splits > 1 && !p.cluster) {
     GS_CUDA(attention_combine(a, p.splits, p.part_out, p.part_lse, stream));
     count_launches(1u);
   }

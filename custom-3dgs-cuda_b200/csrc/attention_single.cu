@@ -81,32 +81,6 @@ __device__ __forceinline__ unsigned part(const uint4& v, int u) {
   return u == 0 ? v.x : u == 1 ? v.y : u == 2 ? v.z : v.w;
 }
 
-// The barrier of a cluster's threads, and shared memory of its CTA `rank` where this CTA's p is.
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ unsigned cluster_address(const void* p, int rank) {
-  unsigned r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float cluster_load(const float* p, int rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address(p, rank)) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(cluster_address(p, rank))
-               : "memory");
-  return v;
-}
-
 // DP: head size rounded up to 64 or 128. NT: groups of 8 rows.
 template <typename T, int DP, int NT>
 __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
@@ -349,7 +323,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
 #pragma unroll
     for (int s = 0; s < kClusterSplits; ++s) {
       w[s] = s < p.splits ? cluster_load(&s_lse[r], s) : -INFINITY;
-      v[s] = s < p.splits ? cluster_load4(&s_part[r][d], s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      v[s] = s < p.splits ? cluster_load4(smem_u32(&s_part[r][d]), s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       top = max_nan(top, w[s]);
     }
 #pragma unroll

@@ -293,6 +293,32 @@ __device__ __forceinline__ void store_rows(unsigned addr, bool have, bool live, 
   }
 }
 
+// The barrier of a cluster's threads, and shared memory of its CTA `rank` where this CTA's p is.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ unsigned cluster_address(unsigned p, int rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float cluster_load(const float* p, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_address(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(unsigned p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_address(p, rank))
+               : "memory");
+  return v;
+}
+
 // 2^x by the special-function unit: relative error below 2^-22, 0 for -inf, results below 2^-126
 // are flushed to 0.
 __device__ __forceinline__ float fast_exp2(float x) {
