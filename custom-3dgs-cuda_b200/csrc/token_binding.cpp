@@ -6,6 +6,7 @@
 // custom_rasterizer_cuda._lib has loaded (bind).
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -75,6 +76,20 @@ void check_tokens(const Tensor& t, const char* name, int64_t dims) {
   TORCH_CHECK(t.dim() == dims, name, " must have ", dims, " dimensions");
 }
 
+// What is told apart by neither requires_grad() nor the pointers: a trace would record the empty
+// output and not the kernel, and a tangent (forward mode) would be dropped without a word.
+void check_untraced(const char* op) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), op, " cannot be traced");
+}
+
+bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
+void check_no_tangent(const char* op, std::initializer_list<const Tensor*> inputs) {
+  check_untraced(op);
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!has_tangent(*t), op, " has no forward-mode derivative");
+}
+
 void* stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
@@ -125,6 +140,8 @@ Tensor rotate(const Tensor& x_in, const Tensor& positions, const RotaryArgs& a) 
   return y;
 }
 
+Tensor differentiable_rotate(const Tensor& x, const Tensor& positions, const RotaryArgs& a);
+
 struct RotaryAxes : torch::autograd::Function<RotaryAxes> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& positions,
                         const RotaryArgs& a) {
@@ -143,16 +160,25 @@ struct RotaryAxes : torch::autograd::Function<RotaryAxes> {
     for (int i = 0; i < 4; ++i) a.dims[i] = (int)ints[1 + i], a.bases[i] = bases[i];
     a.inverse = !ints[5];
     a.interleaved = ints[6];
-    const Tensor& dy = grads[0];
-    // linear: a second derivative is the rotation again
-    return {dy.requires_grad() && at::GradMode::is_enabled() ? apply(dy, positions, a)
-                                                             : rotate(dy, positions, a),
-            Tensor(), Tensor()};
+    return {differentiable_rotate(grads[0], positions, a), Tensor(), Tensor()};
   }
 };
 
+// The map is linear: its gradient, a second derivative and the tangent (forward mode) are rotations.
+Tensor differentiable_rotate(const Tensor& x, const Tensor& positions, const RotaryArgs& a) {
+  if (has_tangent(x)) {
+    const auto [value, tangent] = at::_unpack_dual(x, /*level=*/0);
+    return at::_make_dual(differentiable_rotate(value, positions, a),
+                          differentiable_rotate(tangent, positions, a), /*level=*/0);
+  }
+  return x.requires_grad() && at::GradMode::is_enabled()
+             ? RotaryAxes::apply(x, positions.detach(), a)
+             : rotate(x, positions, a);
+}
+
 Tensor rotary_axes(const Tensor& x, Tensor positions, const std::vector<int64_t>& axis_dims,
                    const std::vector<double>& bases, bool interleaved, bool inverse) {
+  check_untraced("rotary_axes");
   check_tokens(x, "x", 4);
   check_tokens(positions, "positions", 3);
   TORCH_CHECK(type_of(x) >= 0, "x must be float32, float16 or bfloat16");
@@ -185,9 +211,7 @@ Tensor rotary_axes(const Tensor& x, Tensor positions, const std::vector<int64_t>
   }
   TORCH_CHECK(fine, "base must be one positive number, or one for each axis");
   if (positions.stride(2) != 1) positions = positions.contiguous();
-  if (at::GradMode::is_enabled() && x.requires_grad())
-    return RotaryAxes::apply(x, positions.detach(), a);
-  return rotate(x, positions, a);
+  return differentiable_rotate(x, positions, a);
 }
 
 // ---- norms -----------------------------------------------------------------------------------
@@ -237,6 +261,7 @@ NormOut norm_forward(const Tensor& x, const Tensor& weight, const OptTensor& res
 std::pair<Tensor, Tensor> norm_backward(Tensor dy, const Tensor& dh_in, const Tensor& h,
                                         const Tensor& weight, const Tensor& rstd) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "rms_norm has no second derivative");
+  check_no_tangent("rms_norm's gradient", {&dy, dh_in.defined() ? &dh_in : &dy});
   const int64_t width = h.size(-1), rows = h.numel() / width;
   dy = dy.contiguous();
   const Tensor dh = dh_in.defined() ? dh_in.contiguous() : dh_in;
@@ -282,6 +307,7 @@ struct RMSNormResidual : torch::autograd::Function<RMSNormResidual> {
 };
 
 py::object rms_norm(Tensor x, Tensor weight, OptTensor residual, double eps) {
+  check_no_tangent("rms_norm", {&x, &weight, residual ? &*residual : &x});
   check_norm(x, weight, residual, eps);
   Tensor y, h;
   {
@@ -306,6 +332,7 @@ py::object rms_norm(Tensor x, Tensor weight, OptTensor residual, double eps) {
 }
 
 py::object rms_norm_8bit(Tensor x, Tensor weight, OptTensor residual, double eps, int64_t group) {
+  check_no_tangent("rms_norm_8bit", {&x, &weight, residual ? &*residual : &x});
   check_norm(x, weight, residual, eps);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad() ||
                                                (residual && residual->requires_grad())),
@@ -394,6 +421,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return variable_list(6);
     TORCH_CHECK(!at::GradMode::is_enabled(), "cross_attention has no second derivative");
+    check_no_tangent("cross_attention's gradient", {&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4];
     const auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; };
@@ -414,6 +442,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 
 py::object cross_attention(Tensor q, Tensor k, Tensor v, OptTensor lengths, OptTensor mask,
                            c10::optional<double> scale_in, bool return_lse) {
+  check_no_tangent("cross_attention", {&q, &k, &v});
   check_tokens(q, "q", 4);
   check_tokens(k, "k", 4);
   check_tokens(v, "v", 4);

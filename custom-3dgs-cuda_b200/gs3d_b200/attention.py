@@ -16,7 +16,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     `lengths` (int32 [B]): the keys of each batch item; later ones are not looked at. `mask` (bool,
     [B or 1, Hq or 1, Lq or 1, Lk]): False leaves a key out. A query that keeps no key gives zeros.
     `scale` is 1 / sqrt(D) unless given. With `return_lse`, (out, lse[B, Hq, Lq] float32): log sum
-    exp of the scaled scores, -inf for a query without keys; no gradient flows through it.
+    exp of the scaled scores, -inf for a query without keys; no gradient flows through it. First
+    derivatives backwards only: a tangent (forward mode) is refused.
 
     Tensors whose last axis is contiguous are used in place, whatever the other strides, if address
     and strides are multiples of 16 bytes; others are copied first. Under a mask that differs

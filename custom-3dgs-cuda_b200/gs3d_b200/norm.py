@@ -12,7 +12,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
              eps: float = 1e-6):
     """y = h / sqrt(mean(h^2) + eps) * weight over the last axis (at most 32,768 elements), with
     h = x + residual where a residual is given: then (y, h) is returned, h being the new residual
-    stream, else y alone. float32, float16 or bfloat16, all of one type."""
+    stream, else y alone. float32, float16 or bfloat16, all of one type. First derivatives
+    backwards only: a tangent (forward mode) is refused."""
     return native.rms_norm(x, weight, residual, eps)
 
 

@@ -19,7 +19,7 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, axis_dims, base=10000.
     float32). `axis_dims` gives the (even) number of a head's numbers that each axis owns, from
     the first on; what is left over is copied. Pair j of an axis with d numbers turns by
     position * base^(-2 j / d); pairs are (j, j + d / 2) of the axis's block, or neighbours when
-    `interleaved`. `base` is one number or one for each axis. `inverse` turns back. No gradient
-    reaches the positions."""
+    `interleaved`. `base` is one number or one for each axis. `inverse` turns back. Differentiable in
+    x, forward mode included; the positions count as constants in both modes."""
     bases = base if isinstance(base, (tuple, list)) else (base,) * len(axis_dims)
     return native.rotary_axes(x, positions, axis_dims, bases, interleaved, inverse)
