@@ -32,8 +32,14 @@
 // P and dS are rounded to the products' 16-bit type, a relative error for bfloat16 down to 2^-126,
 // where the exponential's results and the products' operands end. Both are formed 2^32 times
 // larger and the sums scaled back, so that probabilities down to 2^-158 still count. Half has few
-// exponents: P is formed 2^15 times larger there, and dS as it is, since it has no bound: half's
-// gradients lose bits where dS is below 2^-14 unless the loss is scaled.
+// exponents: P is formed 2^15 times larger there, and dS by a power of two for each (item, key head),
+// whose query heads dk adds up: |dS| = P |dP - delta| is at most |dO| |v| / 2, so with the largest
+// norms of a row of dO and of a kept row of v the largest dS ends up below 2^15, and those down to
+// 2^-29 of it keep all their bits. (As it is, dS of 999 x 3,600 lies among half's subnormals
+// from a dO of deviation 1e-3 down: 6 times the error of the results' own rounding.) Reading v once more
+// for its norms, and clearing them first, costs 4 us of 111 there, forward included, and 13 of 398 at
+// 4,096 x 4,096, 16 heads of 64. The power is at least 1: where dO is so large that dS may pass 65,504, the loss is scaled too far up, as with any
+// half gradient.
 #include <algorithm>
 #include <cmath>
 
@@ -58,6 +64,7 @@ struct BackwardParams {
   int lq_pad;           // Lq rounded up to kInner
   int splits;           // of the inner tiles
   int x1b, x1h, x2b, x2h, y1b, y1h, y2b, y2h;  // 0 where items or heads share the tensor, else 1
+  const float* norms;   // half only: see attention_prepare_kernel
   float* part1;  // [splits, outer rows, D] where splits > 1: dq or dk
   float* part2;  // dv
 };
@@ -77,27 +84,77 @@ struct BackwardShared {
                                 kStages1 * kStatBytes;
 };
 
-// P is formed 2^kLog2 times larger; kDs brings dS back where its type cannot hold that, kAcc1 and
-// kAcc2 the accumulators of dS and P.
+// P is formed 2^kLog2 times larger, kAcc brings its sums back. kOwnDs: dS has a scale of its own
+// (ds_scale), else it is P's.
 template <typename T>
 struct ProbabilityScale {
-  static constexpr float kLog2 = 32.0f, kDs = 1.0f;
-  static constexpr float kAcc1 = 1.0f / 4294967296.0f, kAcc2 = kAcc1;
+  static constexpr float kLog2 = 32.0f, kAcc = 1.0f / 4294967296.0f;
+  static constexpr bool kOwnDs = false;
 };
 template <>
 struct ProbabilityScale<__half> {
-  static constexpr float kLog2 = 15.0f, kDs = 1.0f / 32768.0f;
-  static constexpr float kAcc1 = 1.0f, kAcc2 = kDs;
+  static constexpr float kLog2 = 15.0f, kAcc = 1.0f / 32768.0f;
+  static constexpr bool kOwnDs = true;
 };
 
+// The power of two that dS of a key head is formed times larger, from the squares of the largest norms
+// of its rows of dO and v: the largest |dO| |v| / 2 comes to lie in [2^14, 2^15], where that is up.
+__device__ __forceinline__ float ds_scale(const float* norms) {
+  const float bound = 0.5f * sqrtf(norms[0]) * sqrtf(norms[1]);
+  const int exponent = (int)(__float_as_uint(bound) >> 23) - 126;  // bound < 2^exponent
+  return bound > 0.0f ? __uint_as_float((unsigned)(127 + min(max(15 - exponent, 0), 60)) << 23) : 1.0f;
+}
+
+// Raises norms[0] to the largest of the CTA's values, whose 8 lanes a row agree; rows that hold a NaN or
+// an infinity do not count: either no result sees them or all that do are NaN. Not negative, so
+// the largest integer is the largest number, and the order of the CTAs does not matter.
+__device__ __forceinline__ void raise_norm(float square, float* norm) {
+  __shared__ float shared[8];
+  square = square < INFINITY ? square : 0.0f;
+#pragma unroll
+  for (int w = 8; w < 32; w <<= 1) square = fmaxf(square, __shfl_xor_sync(~0u, square, w));
+  if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = square;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) square = fmaxf(square, shared[k]);
+    atomicMax(reinterpret_cast<int*>(norm), __float_as_int(square));
+  }
+}
+
 // delta and lse in powers of two of every query row, 8 lanes a row; the rows, padded to a multiple
-// of kInner for each head, fill the grid exactly.
+// of kInner for each head, fill the first `query_blocks` of the grid exactly. For half also the squares
+// of the largest norms of the rows of dO and of v, [B, Hkv, 2], zero before; the CTAs past the queries'
+// read v, 32 keys each.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams a, int lq_pad,
-                                                                float* stats) {
+                                                                unsigned query_blocks, float* stats,
+                                                                float* norms) {
+  constexpr bool kNorms = ProbabilityScale<T>::kOwnDs;
   wait_for_previous();
   let_next_start();
   const int sub = threadIdx.x % 8;
+  float square = 0.0f;
+  if (kNorms && blockIdx.x >= query_blocks) {
+    const unsigned key_blocks = (unsigned)(a.Lk + 31) / 32, at = blockIdx.x - query_blocks;
+    const unsigned bh = at / key_blocks;
+    const int j = (int)(at - bh * key_blocks) * 32 + threadIdx.x / 8;
+    const int b = bh / (unsigned)a.Hkv, h = bh - b * (unsigned)a.Hkv;
+    const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
+    if (j < key_count(a, b) && (!key_mask || (a.bits[b * a.bits_b + j / 32] >> (j % 32) & 1u))) {
+      const T* v = a.v.at<T>(b, j, h);
+      for (int d = sub * 8; d < a.D; d += 64) {
+        float x[8];
+        load_pack<T, 8>(v + d, x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) square = fmaf(x[k], x[k], square);
+      }
+    }
+#pragma unroll
+    for (int w = 4; w; w >>= 1) square += __shfl_xor_sync(~0u, square, w);
+    raise_norm(square, norms + 2ll * bh + 1);
+    return;
+  }
   const long long at = (long long)blockIdx.x * 32 + threadIdx.x / 8;
   const int i = (int)(at % lq_pad), h = (int)(at / lq_pad % a.Hq), b = (int)(at / lq_pad / a.Hq);
   float delta = 0.0f, lse = INFINITY;
@@ -110,6 +167,9 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams 
       load_pack<T, 8>(g + d, y);
 #pragma unroll
       for (int k = 0; k < 8; ++k) delta = fmaf(x[k], y[k], delta);
+      if (kNorms)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) square = fmaf(y[k], y[k], square);
     }
     lse = a.lse[((long long)b * a.Hq + h) * a.Lq + i];
     lse = lse == -INFINITY ? INFINITY
@@ -121,6 +181,12 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams 
     float* tile = stats + at / kInner * (2 * kInner) + at % kInner;
     tile[0] = lse;
     tile[kInner] = delta;
+  }
+  if constexpr (kNorms) {
+    if (lse == INFINITY) square = 0.0f;  // keeps no key
+#pragma unroll
+    for (int w = 4; w; w >>= 1) square += __shfl_xor_sync(~0u, square, w);
+    raise_norm(square, norms + 2 * ((long long)b * a.Hkv + h / (a.Hq / a.Hkv)));
   }
 }
 
@@ -275,6 +341,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int wg = warp / 4, row = threadIdx.x % 128, x = x0 + row;
     const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
     const float c = p.scale_log2;
+    // dS's scale, the row's part of it beside P's, and dS's back to 1
+    float ds_up = 1.0f, ds_back = PS::kAcc;
+    if (PS::kOwnDs && count > 0) {
+      const float up =
+          ds_scale(p.norms + 2 * ((long long)b * a.Hkv + (KEYS ? ho : ho / shared_heads)));
+      ds_up = up * PS::kAcc;
+      ds_back = 1.0f / up;
+    }
     float2 mine = make_float2(INFINITY, 0.0f);
     const unsigned* keep_row = nullptr;
     // KEYS: the warp's 32 keys that are below the length, and that a key mask leaves
@@ -347,7 +421,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             tc_fence_after();
           }
           if (KEYS) store_packed<T>(my_p + h / 2, pr + h);
-          differences<KEYS>(pr + h, dp + h, stat + kInner * 4 + h * 4, mine.y, PS::kDs);
+          differences<KEYS>(pr + h, dp + h, stat + kInner * 4 + h * 4, mine.y, ds_up);
           store_packed<T>(my_ds + h / 2, pr + h);
         }
         if (!ok) break;
@@ -371,7 +445,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (hidden) hide(keep, c < 0.0f, nullptr, dp);
 #pragma unroll
         for (int h = 0; h < 64; h += 32) {
-          differences<KEYS>(pr + h, dp + h, stat + kInner * 4 + h * 4, mine.y, PS::kDs);
+          differences<KEYS>(pr + h, dp + h, stat + kInner * 4 + h * 4, mine.y, ds_up);
           store_packed<T>(my_ds + h / 2, pr + h);
         }
       }
@@ -384,7 +458,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tc_fence_after();
     // KEYS: the first warpgroup writes dk, the second dv; else they take half of dq's columns each
     const bool first = !KEYS || wg == 0;
-    const float factor = first ? a.scale * PS::kAcc1 : PS::kAcc2;
+    const float factor = first ? a.scale * ds_back : PS::kAcc;
     const TokenView& view = KEYS ? (first ? a.dk : a.dv) : a.dq;
     const long long rows = (long long)a.B * outer_heads * outer_rows;
     float* part = first ? p.part1 : p.part2;
@@ -593,7 +667,7 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, int s
 
 struct BackwardPlan {
   int key_splits = 1, query_splits = 1;
-  long long lq_pad = 0, key_floats = 0, query_floats = 0;
+  long long lq_pad = 0, norm_floats = 0, key_floats = 0, query_floats = 0;
   size_t bytes = 0;
 };
 
@@ -613,8 +687,10 @@ static BackwardPlan backward_plan(const gs_attention_args& a) {
     plan.key_floats = (long long)plan.key_splits * a.B * a.Hkv * a.Lk * a.D;
   if (plan.query_splits > 1)
     plan.query_floats = (long long)plan.query_splits * a.B * a.Hq * a.Lq * a.D;
+  if (a.dtype == GS_FP16 && plan.lq_pad && a.Hq > 0)
+    plan.norm_floats = ((long long)a.B * a.Hkv * 2 + 3) / 4 * 4;
   // dk, dv and dq in turn use the same parts
-  plan.bytes = (size_t)(a.B * a.Hq * plan.lq_pad) * 2 * sizeof(float) +
+  plan.bytes = (size_t)(a.B * a.Hq * plan.lq_pad * 2 + plan.norm_floats) * sizeof(float) +
                (size_t)std::max(2 * plan.key_floats, plan.query_floats) * sizeof(float);
   return plan;
 }
@@ -662,14 +738,21 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   p.scale_log2 = (a.scale == 0.0f ? 1e-30f : a.scale) * 1.4426950408889634f;
   p.lq_pad = (int)plan.lq_pad;
   const size_t mask_bytes = attention_mask_bytes(a);
-  if (const int status = attention_pack_mask(a, p.a, workspace, stream)) return status;
   float* stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);
   p.stats = stats;
   const long long stat_rows = a.B * a.Hq * plan.lq_pad;
-  float* parts = stats + 2 * stat_rows;
+  float* norms = stats + 2 * stat_rows;
+  p.norms = norms;
+  float* parts = norms + plan.norm_floats;
+  // before the mask's kernel, beside whose end the next one may then start
+  if (plan.norm_floats)
+    GS_CUDA(cudaMemsetAsync(norms, 0, plan.norm_floats * sizeof(float), stream));
+  if (const int status = attention_pack_mask(a, p.a, workspace, stream)) return status;
   if (stat_rows) {
-    GS_CUDA(launch_overlapped(attention_prepare_kernel<T>, dim3((unsigned)(stat_rows / 32)), 256, 0,
-                              stream, p.a, p.lq_pad, stats));
+    const unsigned query_blocks = (unsigned)(stat_rows / 32);
+    const long long key_blocks = plan.norm_floats ? (long long)a.B * a.Hkv * ((a.Lk + 31) / 32) : 0;
+    GS_CUDA(launch_overlapped(attention_prepare_kernel<T>, dim3((unsigned)(query_blocks + key_blocks)),
+                              256, 0, stream, p.a, p.lq_pad, query_blocks, stats, norms));
     count_launches(1u);
   }
   // Outer and inner tiles have the same box, so one map of each tensor serves both kernels. A map
