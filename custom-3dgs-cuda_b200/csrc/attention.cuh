@@ -49,6 +49,9 @@ __device__ __forceinline__ unsigned below(int left, int w) {
 
 constexpr unsigned kMinusInf = 0xff800000u;
 
+// 2^kHalfLog2 is half's largest power of two.
+constexpr float kHalfLog2 = 15.0f;
+
 // Sets the scores s of 32 keys to -inf where their bit in `keep` is 0.
 __device__ __forceinline__ void hide32(unsigned keep, unsigned* s) {
 #pragma unroll

@@ -15,9 +15,11 @@
 //
 // The maximum that P is formed with may lag behind the true one by up to kLag powers of two: the
 // accumulator (128 rows x D numbers through registers) is rescaled only when a row's maximum has
-// grown by more, which after the first tiles is rare. P is at most 2^kLag then, far inside both
-// 16-bit types' range; its rounding to 16 bits (the products' operand type) is relative, so
-// nothing is lost. The row sum adds P before that rounding, in 32 bits.
+// grown by more, which after the first tiles is rare. P is rounded to 16 bits, the products' operand
+// type, while the row sum adds it before that, in 32 bits. For bfloat16 the rounding is relative
+// all the way down. Half has few exponents, so P is formed with what the lag leaves of them, 2^(15 -
+// kLag) times larger: relative down to 2^-21 of the (lagging) maximum, and 65,000 keys below that
+// are still off by less than 2^-16 of it together.
 //
 // With few query tiles the keys are split over CTAs: each has its normalised output in 32 bits and
 // its lse, and the splits of a block, as a cluster through shared memory, or combine_kernel join them
@@ -38,6 +40,11 @@ constexpr int kTileQ = 128;   // query rows of one warpgroup
 constexpr int kTileK = 128;   // keys of one tile
 constexpr float kLag = 8.0f;  // powers of two
 constexpr int kFwdThreads = 384;
+// P is formed 2^kUp times larger.
+template <typename T>
+constexpr float kUp = 0.0f;
+template <>
+constexpr float kUp<__half> = kHalfLog2 - kLag;
 // Registers of a softmax thread and of the others: 2 x 128 x 200 + 128 x 104 = 384 x 168, what the
 // CTA is launched with.
 constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           if (!ok) break;
         }
         // m - m is 0, or NaN where the row holds an infinite score
-        const float off = m == -INFINITY ? 0.0f : fmaf(m, p.scale_log2, m - m);
+        const float off = m == -INFINITY ? 0.0f : fmaf(m, p.scale_log2, (m - m) - kUp<T>);
         const Two scale2 = two(p.scale_log2, p.scale_log2), off2 = two(-off, -off);
         Two sum[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
 #pragma unroll
@@ -288,7 +295,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (!ok) gave_up = 1;
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const float lse = l == 0.0f ? -INFINITY : m * p.scale_log2 * 0.6931471805599453f + logf(l);
+      const float lse = l == 0.0f ? -INFINITY
+                                  : m * p.scale_log2 * 0.6931471805599453f +
+                                        logf(l * (1.0f / (1 << (int)kUp<T>)));
       const long long row = ((long long)b * a.Hq + h0) * a.Lq + row_q;
       const long long rows = (long long)a.B * a.Hq * a.Lq;
       const bool wide = p.splits > 1;

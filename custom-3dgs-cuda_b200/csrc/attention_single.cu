@@ -11,7 +11,9 @@
 //   S^T[16 keys, 8 rows] = k q^T: A from k, lane (g = lane / 4, t = lane % 4) holds keys g, g + 8;
 //   O^T[16 numbers, 8 rows] += v^T P^T: A from v, the lane holds keys 2t, 2t + 1, 2t + 8, 2t + 9
 //   and interleaves pairs of them by byte permutes; P^T is S^T's fragment transposed in 8 x 8.
-// Rows are columns of both results, so the running maximum of a row is rescaled in place.
+// Rows are columns of both results, so the running maximum of a row is rescaled in place. P is rounded
+// to 16 bits for the second product; half, which has few exponents, takes it 2^15 times larger, so
+// that weights down to 2^-29 of the largest keep all their bits.
 // A warp walks over chunks of 16 keys (D above 64) or 32, the next chunk's loads in flight while
 // it works on this one; CTAs of 4 warps split the keys, and a cluster joins its CTAs' parts or, where
 // there are more than 8, combine_kernel.
@@ -25,6 +27,11 @@
 namespace gs {
 
 constexpr int kSingleWarps = 4;
+// P is formed 2^kUp times larger.
+template <typename T>
+constexpr float kUp = 0.0f;
+template <>
+constexpr float kUp<__half> = kHalfLog2;
 constexpr int kClusterSplits = 8;  // at most, of those that a cluster joins
 // resident CTAs an SM, by groups of 8 rows: 168 registers a thread hold one, 255 two
 constexpr int single_ctas(int groups) { return groups == 1 ? 3 : 2; }
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float top_e = m_row[nt][e & 1];
-          s[nt][m][e] = fast_exp2(s[nt][m][e] - (top_e == -INFINITY ? 0.0f : top_e));
+          s[nt][m][e] = fast_exp2(s[nt][m][e] - (top_e == -INFINITY ? 0.0f : top_e) + kUp<T>);
           l_row[nt][e & 1] += s[nt][m][e];
         }
         pt[nt][m][0] = transpose8x8(pack2<T>(s[nt][m][0], s[nt][m][1]));
@@ -290,7 +297,8 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = l == 0.0f ? 0.0f : acc[i] * inv;
-      const float lse2 = l == 0.0f ? -INFINITY : top + log2f(l), lse = lse2 * 0.6931471805599453f;
+      const float lse2 = l == 0.0f ? -INFINITY : top + log2f(l * (1.0f / (1 << (int)kUp<T>))),
+                  lse = lse2 * 0.6931471805599453f;
       if (p.cluster) {
         *reinterpret_cast<float4*>(&s_part[r][d]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         if (d == 0) s_lse[r] = lse2;

@@ -88,3 +88,42 @@ def test_upstream_gradients_of_any_size_stay_finite(cuda_device):
     ref = attention64(q, k, v, dout=g)
     for name, got in zip(("dq", "dk", "dv"), gradients(q, k, v, g)):
         assert_close_in_norm(got, ref[name][0], name)
+
+
+@pytest.mark.parametrize("Lq,Hq,Hkv,D", [(1, 2, 2, 64), (1, 4, 1, 128), (12, 1, 1, 64), (40, 4, 2, 64),
+                                         (130, 2, 2, 64), (300, 1, 1, 128)])
+@pytest.mark.parametrize("at", (0, 30000, 60000))
+def test_many_keys_of_little_weight(cuda_device, Lq, Hq, Hkv, D, at):
+    """One key has nearly all the weight, 60,000 others 2^-25.3 of it each: together 1.5e-3 of the sum,
+    and all of the result, since the values are 0 at the one and 1 at the others. The weights are
+    rounded to half at 2^7 times their size or more (the largest is 2^8, and half ends at 2^16), where
+    half's steps are 2^-24: an error of at most 2^-32 each."""
+    from gs3d_b200.attention import cross_attention
+
+    Lk, dev = 60001, cuda_device
+    q = torch.zeros(1, Lq, Hq, D, device=dev).half()
+    k, v = (torch.zeros(1, Lk, Hkv, D, device=dev).half() for _ in range(2))
+    q[..., 0], k[..., 0], v[:] = 1.0, -17.54, 1.0
+    k[:, at], v[:, at] = 0.0, 0.0
+    out, lse = cross_attention(q, k, v, scale=1.0, return_lse=True)
+    w = 60000 * torch.exp(k[0, (at + 1) % Lk, 0, 0].double())
+    ref = float(w / (1.0 + w))
+    worst = float((out.double() - ref).abs().max())
+    assert worst <= 60000 * 2.0 ** -32 + 2.0 ** -10 * ref, (worst, ref)
+    assert float((lse.double() - torch.log1p(w)).abs().max()) <= 2.0 ** -18
+
+
+def test_many_keys_of_little_weight_in_one_piece(cuda_device):
+    """The same where one CTA takes all keys of a key head: many items that share their keys."""
+    from gs3d_b200.attention import cross_attention
+
+    B, Lk, D, dev = 500, 20000, 64, cuda_device
+    q = torch.zeros(B, 1, 1, D, device=dev).half()
+    k, v = (torch.zeros(1, Lk, 1, D, device=dev).half() for _ in range(2))
+    q[..., 0], k[..., 0], v[:] = 1.0, -17.54, 1.0
+    k[:, 0], v[:, 0] = 0.0, 0.0
+    out = cross_attention(q, k.expand(B, Lk, 1, D), v.expand(B, Lk, 1, D), scale=1.0)
+    w = (Lk - 1) * torch.exp(k[0, 1, 0, 0].double())
+    ref = float(w / (1.0 + w))
+    worst = float((out.double() - ref).abs().max())
+    assert worst <= Lk * 2.0 ** -32 + 2.0 ** -10 * ref, (worst, ref)
