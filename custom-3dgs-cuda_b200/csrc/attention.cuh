@@ -33,6 +33,11 @@ struct AttentionParams {
   // the mask as bits, rows of 4 words for each 128 keys; strides in words, 0 where shared; or null
   const unsigned* bits;
   long long bits_b, bits_h, bits_q;
+  // rows of such words whose OR says which keys any query and head of a key head keeps: kept_rows of
+  // them for each batch item and key head, 4 words for each 128 keys; strides in words
+  const unsigned* kept;
+  long long kept_b, kept_h;
+  int kept_rows, kept_row, kept_tile;
   float* lse;  // [B, Hq, Lq] or null
 };
 
@@ -47,6 +52,31 @@ __device__ __forceinline__ unsigned below(int left, int w) {
   return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u;
 }
 
+// The keys of tile `tile` (of 128) that any query of key head hk keeps, in two steps so that the loads can
+// be in flight meanwhile; for a whole warp, whose lanes then all have it. All loads are in flight at
+// once, lanes without a row read the last one (a loop with a trip count of each lane's own takes its
+// odd trips one after another: 306 -> 641 us at 3 x 6,000 x 10,000, 4 heads of 64).
+constexpr int kKeptMost = 256;  // rows, at most
+__device__ __forceinline__ uint4 kept_begin(const AttentionParams& p, int b, int hk, int tile) {
+  const unsigned* at = p.kept + b * p.kept_b + hk * p.kept_h + (long long)tile * p.kept_tile;
+  uint4 w[kKeptMost / 32], any = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int k = 0; k < kKeptMost / 32; ++k) {
+    w[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (32 * k < p.kept_rows)
+      w[k] = *reinterpret_cast<const uint4*>(
+          at + (long long)min(32 * k + (int)(threadIdx.x % 32), p.kept_rows - 1) * p.kept_row);
+  }
+#pragma unroll
+  for (int k = 0; k < kKeptMost / 32; ++k)
+    any.x |= w[k].x, any.y |= w[k].y, any.z |= w[k].z, any.w |= w[k].w;
+  return any;
+}
+__device__ __forceinline__ uint4 kept_end(const uint4& any) {
+  return make_uint4(__reduce_or_sync(~0u, any.x), __reduce_or_sync(~0u, any.y),
+                    __reduce_or_sync(~0u, any.z), __reduce_or_sync(~0u, any.w));
+}
+
 constexpr unsigned kMinusInf = 0xff800000u;
 
 // 2^kHalfLog2 is half's largest power of two.
@@ -59,33 +89,38 @@ __device__ __forceinline__ void hide32(unsigned keep, unsigned* s) {
     if (!(keep >> k & 1u)) s[k] = kMinusInf;
 }
 
-// Zeroes, in a swizzled tile of ROWS keys (BOXES boxes of 128 bytes a row) at shared address `tile`,
-// the rows from `left` on and those whose bit in `bits` is 0 (or null): whole rows, so the swizzle
-// inside them does not matter. One warp; the matrix engine sees it afterwards.
-template <int BOXES, int ROWS>
-__device__ __forceinline__ void clear_rows(unsigned tile, int left, const unsigned* bits) {
+// Zeroes, in a swizzled tile of 128 rows (BOXES boxes of 128 bytes a row) at shared address `tile`, the
+// rows from `left` on and those whose bit in `keep` is 0: whole rows, so the swizzle inside them does
+// not matter. One warp; the matrix engine sees it afterwards.
+template <int BOXES>
+__device__ __forceinline__ void clear_rows(unsigned tile, int left, const uint4& keep) {
+  constexpr int kRows = 128;
   const int lane = threadIdx.x % 32;
   for (int x = 0; x < BOXES; ++x)
 #pragma unroll 4
-    for (int at = left * 128 + lane * 16; at < ROWS * 128; at += 512)
-      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + x * ROWS * 128 + at),
+    for (int at = left * 128 + lane * 16; at < kRows * 128; at += 512)
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + x * kRows * 128 + at),
                    "r"(0)
                    : "memory");
-  if (bits)
-    for (int w = 0; w < ROWS / 32; ++w) {
-      unsigned out = below(left, w) & ~bits[w];
-      while (out) {
-        const int k = w * 32 + __ffs(out) - 1;
-        out &= out - 1;
 #pragma unroll
-        for (int x = 0; x < BOXES; ++x)
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile + (x * ROWS + k) * 128 + lane * 4),
-                       "r"(0)
-                       : "memory");
-      }
+  for (int w = 0; w < kRows / 32; ++w) {
+    const unsigned kept = w == 0 ? keep.x : w == 1 ? keep.y : w == 2 ? keep.z : keep.w;
+    unsigned out = below(left, w) & ~kept;
+    while (out) {
+      const int k = w * 32 + __ffs(out) - 1;
+      out &= out - 1;
+#pragma unroll
+      for (int x = 0; x < BOXES; ++x)
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile + (x * kRows + k) * 128 + lane * 4), "r"(0)
+                     : "memory");
     }
+  }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
+}
+// Whether clear_rows would find anything to clear.
+__device__ __forceinline__ bool has_hidden_rows(int left, const uint4& keep) {
+  return left < 128 || (keep.x & keep.y & keep.z & keep.w) != ~0u;
 }
 
 // Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the runtime

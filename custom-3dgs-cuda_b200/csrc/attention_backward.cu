@@ -85,7 +85,7 @@ struct BackwardShared {
 };
 
 // P is formed 2^kLog2 times larger, kAcc brings its sums back. kOwnDs: dS has a scale of its own
-// (ds_scale), else it is P's.
+// (ds_log2), else it is P's.
 template <typename T>
 struct ProbabilityScale {
   static constexpr float kLog2 = 32.0f, kAcc = 1.0f / 4294967296.0f;
@@ -97,12 +97,12 @@ struct ProbabilityScale<__half> {
   static constexpr bool kOwnDs = true;
 };
 
-// The power of two that dS of a key head is formed times larger, from the squares of the largest norms
-// of its rows of dO and v: the largest |dO| |v| / 2 comes to lie in [2^14, 2^15], where that is up.
-__device__ __forceinline__ float ds_scale(const float* norms) {
+// How many powers of two dS of a key head is formed larger, from the squares of the largest norms of its
+// rows of dO and v: the largest |dO| |v| / 2 comes to lie in [2^14, 2^15], where that is up.
+__device__ __forceinline__ int ds_log2(const float* norms) {
   const float bound = 0.5f * sqrtf(norms[0]) * sqrtf(norms[1]);
   const int exponent = (int)(__float_as_uint(bound) >> 23) - 126;  // bound < 2^exponent
-  return bound > 0.0f ? __uint_as_float((unsigned)(127 + min(max(15 - exponent, 0), 60)) << 23) : 1.0f;
+  return bound > 0.0f ? min(max(15 - exponent, 0), 60) : 0;
 }
 
 // Raises norms[0] to the largest of the CTA's values, whose 8 lanes a row agree; rows that hold a NaN or
@@ -140,8 +140,15 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams 
     const unsigned bh = at / key_blocks;
     const int j = (int)(at - bh * key_blocks) * 32 + threadIdx.x / 8;
     const int b = bh / (unsigned)a.Hkv, h = bh - b * (unsigned)a.Hkv;
-    const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
-    if (j < key_count(a, b) && (!key_mask || (a.bits[b * a.bits_b + j / 32] >> (j % 32) & 1u))) {
+    unsigned keep = ~0u;  // the CTA's 32 keys that any query keeps
+    if (a.bits) {
+      keep = 0;
+      const unsigned* rows = a.kept + b * a.kept_b + h * a.kept_h +
+                             (long long)(j / 128) * a.kept_tile + j / 32 % 4;
+      for (int r = threadIdx.x % 32; r < a.kept_rows; r += 32) keep |= rows[(long long)r * a.kept_row];
+      keep = __reduce_or_sync(~0u, keep);
+    }
+    if (j < key_count(a, b) && (keep >> (j % 32) & 1u)) {
       const T* v = a.v.at<T>(b, j, h);
       for (int d = sub * 8; d < a.D; d += 64) {
         float x[8];
@@ -272,7 +279,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   using PS = ProbabilityScale<T>;
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t x_full, y1_full[S::kStages1], y1_free[S::kStages1], y2_full[S::kStages2],
-      y2_free[S::kStages2], s_full, s_read, dp_full, p_ready, ds_ready, acc_done, acc_full;
+      y2_free[S::kStages2], y1_clean[S::kStages1], s_full, s_read, dp_full, p_ready, ds_ready, acc_done, acc_full;
   __shared__ unsigned tmem_slot;
   __shared__ volatile int gave_up;
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -290,6 +297,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_set(&acc_full, 1);
     for (int i = 0; i < S::kStages1; ++i) {
       mbar_set(&y1_full[i], 1);
+      mbar_set(&y1_clean[i], 1);
       mbar_set(&y1_free[i], 1);
     }
     for (int i = 0; i < S::kStages2; ++i) {
@@ -341,13 +349,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int wg = warp / 4, row = threadIdx.x % 128, x = x0 + row;
     const unsigned lanes = (unsigned)(warp % 4 * 32) << 16;
     const float c = p.scale_log2;
-    // dS's scale, the row's part of it beside P's, and dS's back to 1
-    float ds_up = 1.0f, ds_back = PS::kAcc;
+    // dS's scale over P's, and dS's back to 1; dq, which needs P for dS alone, forms P with dS's scale
+    float ds_up = 1.0f, ds_back = PS::kAcc, p_log2 = 0.0f;
     if (PS::kOwnDs && count > 0) {
-      const float up =
-          ds_scale(p.norms + 2 * ((long long)b * a.Hkv + (KEYS ? ho : ho / shared_heads)));
-      ds_up = up * PS::kAcc;
-      ds_back = 1.0f / up;
+      const int k = ds_log2(p.norms + 2 * ((long long)b * a.Hkv + (KEYS ? ho : ho / shared_heads)));
+      ds_back = __uint_as_float((unsigned)(127 - k) << 23);
+      if (KEYS)
+        ds_up = PS::kAcc / ds_back;
+      else
+        p_log2 = (float)k - PS::kLog2;
     }
     float2 mine = make_float2(INFINITY, 0.0f);
     const unsigned* keep_row = nullptr;
@@ -359,7 +369,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     } else {
       if (x < a.Lq) {
         const float* tile = p.stats + (((long long)b * a.Hq + ho) * p.lq_pad + x0) * 2 + row;
-        mine = make_float2(tile[0], tile[kInner]);
+        mine = make_float2(tile[0] - p_log2, tile[kInner]);
       }
       if (a.bits)
         keep_row = a.bits + b * a.bits_b + ho * a.bits_h + (long long)min(x, a.Lq - 1) * a.bits_q;
@@ -537,16 +547,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       };
       const auto arrived1 = [&](int j) {
         const int st = j % S::kStages1;
-        if (!tc_wait_warp(&y1_full[st], j / S::kStages1 & 1)) return false;
-        if (!KEYS && warp == 8) {
-          // keys that all queries leave out: what they hold must not reach dq, where 0 times NaN
-          // would be added
-          const int key = (t0 + j) * kInner;
-          if (n - key < kInner || key_mask)
-            clear_rows<S::kBoxes, kInner>(sm_y1 + st * S::kInnerBytes, n - key,
-                                  key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
-        }
-        return true;
+        return tc_wait_warp(KEYS ? &y1_full[st] : &y1_clean[st], j / S::kStages1 & 1);
       };
       const auto arrived2 = [&](int j) {
         return tc_wait_warp(&y2_full[j % S::kStages2], j / S::kStages2 & 1);
@@ -573,8 +574,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       } else if (S::kOwnP) {
         for (int j = 0; ok && j < count; ++j) {
-          ok = tc_wait_warp(&y1_full[j % S::kStages1], j / S::kStages1 & 1) &&
-               (!KEYS || arrived2(j)) && when(&ds_ready, j);
+          ok = arrived1(j) && (!KEYS || arrived2(j)) && when(&ds_ready, j);
           if (ok && elect_one()) {
             if (KEYS) sums(j, 1);
             sums(j, 0);
@@ -625,6 +625,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       if (!ok && count > 0) gave_up = 1;
+    } else if (warp == 11 && !KEYS) {
+      // ---- what k holds at keys that no query of the item's key head keeps must not reach dq, where
+      // 0 times NaN would be added: those rows are set to zero before the products may read them
+      for (int j = 0; j < count; ++j) {
+        const int st = j % S::kStages1, key = (t0 + j) * kInner;
+        uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (a.bits) keep = kept_begin(a, b, ho / shared_heads, t0 + j);
+        if (!tc_wait_warp(&y1_full[st], j / S::kStages1 & 1)) { gave_up = 1; break; }
+        if (a.bits) keep = kept_end(keep);
+        if (has_hidden_rows(n - key, keep))
+          clear_rows<S::kBoxes>(sm_y1 + st * S::kInnerBytes, n - key, keep);
+        mbar_arrive_warp(&y1_clean[st]);
+      }
     }
   }
   tc_fence_before();

@@ -6,7 +6,7 @@
 // into tensor memory in 16 bits, and P v is added to the row's accumulator, also there. Four warps
 // serve the first query tile, four the second; two issue their products, on schedulers of their own
 // (one for both held the tensor pipe up: 204 -> 293 us in the first case below), one the copies, one
-// clears v's rows past the keys' end. While one tile's softmax runs, the other tile's products do.
+// clears v's rows past the keys' end and at keys that no query keeps. While one tile's softmax runs, the other tile's products do.
 //
 // What bounds it, at D 64, is the exponentials: 1,024 clocks of the special-function unit for a pair
 // of tiles whose two products take 512 (measured: that unit 69% busy, the tensor pipe 34%); at D 128
@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   } else {
     if (warp == 8) tc_alloc(&tmem_slot, 512);
     // rows that no query is copied to: as good as a query of zeros
-    if (warp == 11 && p.pack > 1) clear_rows<S::kBoxes, kTileQ>(sm_q, queries, nullptr);
+    if (warp == 11 && p.pack > 1)
+      clear_rows<S::kBoxes>(sm_q, queries, make_uint4(~0u, ~0u, ~0u, ~0u));
     tc_fence_before();
     ready_wait<kFwdThreads>();
     tc_fence_after();
@@ -362,16 +363,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           load_v(j);
         }
     } else if (warp == 11) {
-      // ---- what v holds at keys that no query of the CTA keeps must not reach the product, which
-      // would make 0 times NaN of it: those rows are set to zero before the product may read them
-      const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
-      if (key_mask) wait_for_previous();
+      // ---- what v holds at keys that no query of the item's key head keeps must not reach the
+      // product, which would make 0 times NaN of it: those rows are set to zero before the product may
+      // read them
+      if (a.bits) wait_for_previous();
       for (int j = 0; j < count; ++j) {
         const int st = j % S::kStages, key = (t0 + j) * kTileK;
+        uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (a.bits) keep = kept_begin(a, b, hk, t0 + j);
         if (!tc_wait_warp(&v_full[st], j / S::kStages & 1)) { gave_up = 1; break; }
-        if (n - key < kTileK || key_mask)
-          clear_rows<S::kBoxes, kTileK>(sm_v + st * S::kTileBytes, n - key,
-                                key_mask ? a.bits + b * a.bits_b + key / 32 : nullptr);
+        if (a.bits) keep = kept_end(keep);
+        if (has_hidden_rows(n - key, keep))
+          clear_rows<S::kBoxes>(sm_v + st * S::kTileBytes, n - key, keep);
         mbar_arrive_warp(&v_clean[st]);
       }
     } else if (warp == 8 || (warp == 10 && both)) {

@@ -2,7 +2,7 @@
 // (batch item, key head), counting the query heads that share the key head and the queries of each.
 //
 // Bound by HBM: every key and value is read once, for a few rows of work on it. 2 x 65,280 keys, 32
-// query heads on 8 of 128, half: 96 us, 5.6 TB/s; 4 x 3,600 keys of 16 heads of 64: 17.7 us,
+// query heads on 8 of 128, half: 82 us back to back, 6.5 TB/s; 4 x 3,600 keys of 16 heads of 64: 12.5 us,
 // of which the loads' latency is the larger part (five rounds of them a warp). So nothing is
 // staged: each lane loads 16 bytes of a row of k or v straight into the registers in which the
 // warp-wide product (16 x 8 x 16) takes them. The product's contraction index may be numbered
@@ -88,8 +88,9 @@ __device__ __forceinline__ unsigned part(const uint4& v, int u) {
   return u == 0 ? v.x : u == 1 ? v.y : u == 2 ? v.z : v.w;
 }
 
-// DP: head size rounded up to 64 or 128. NT: groups of 8 rows.
-template <typename T, int DP, int NT>
+// DP: head size rounded up to 64 or 128. NT: groups of 8 rows. Calls without a mask have
+// a kernel of their own (2 x 65,280 keys, 8 heads of 128: 94 -> 82 us, 4 x 3,600 of 16 of 64: 14.7 -> 12.5).
+template <typename T, int DP, int NT, bool MASK>
 __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
     attention_single_kernel(const __grid_constant__ SingleParams p) {
   constexpr int MT = 128 / DP;        // blocks of 16 keys in a chunk
@@ -106,8 +107,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
   const int chunks = (n + kChunk - 1) / kChunk;
   const int c0 = (int)((long long)chunks * blockIdx.y / p.splits);
   const int c1 = (int)((long long)chunks * (blockIdx.y + 1) / p.splits);
-  const bool key_mask = a.mask && a.mask_h == 0 && a.mask_q == 0;
-  const unsigned char* mask_b = a.mask ? a.mask + b * a.mask_b : nullptr;
+  const unsigned char* mask_b = a.mask + b * a.mask_b;
 
   const auto head_of = [&](int r) { return hk * shared_heads + r % shared_heads; };
   uint4 q[NT][KL];
@@ -129,9 +129,8 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = min(nt * 8 + 2 * t + e, p.rows - 1);
-      mask_row[nt][e] = mask_b ? mask_b + (long long)head_of(r) * a.mask_h +
-                                     (long long)(r / shared_heads) * a.mask_q
-                               : nullptr;
+      mask_row[nt][e] = mask_b + (long long)head_of(r) * a.mask_h +
+                        (long long)(r / shared_heads) * a.mask_q;
     }
 
   const T* kp = a.k.at<T>(b, 0, hk);
@@ -158,8 +157,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = c * kChunk + m * 16 + 2 * t + (e & 1) + 8 * (e >> 1);
-        // a value that no row keeps is not looked at: 0 times NaN would reach the sum
-        const bool in = c < c1 && j < n && (!key_mask || mask_b[j]);
+        const bool in = c < c1 && j < n;
         const T* row = vp + (long long)j * a.v.l;
 #pragma unroll
         for (int x = 0; x < VB; ++x) {
@@ -194,6 +192,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
       }
     load_k(c + kSingleWarps);
     unsigned pt[NT][MT][2];
+    unsigned kept = 0;  // bit 2 m + e: key g + 8 e of block m, by one of this lane's rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float top[2] = {-INFINITY, -INFINITY};
@@ -203,7 +202,10 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
         for (int e = 0; e < 4; ++e) {  // key g + 8 (e / 2), row 2t + e % 2
           const int j = c * kChunk + m * 16 + g + 8 * (e >> 1);
           float v = s[nt][m][e] * p.scale_log2;
-          if (j >= n || (mask_b && !mask_row[nt][e & 1][j])) v = -INFINITY;
+          if (j >= n || (MASK && !mask_row[nt][e & 1][j]))
+            v = -INFINITY;
+          else if (MASK)
+            kept |= 1u << (2 * m + (e >> 1));
           s[nt][m][e] = v;
           top[e & 1] = fmaxf(top[e & 1], v);
         }
@@ -239,6 +241,19 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
         pt[nt][m][0] = transpose8x8(pack2<T>(s[nt][m][0], s[nt][m][1]));
         pt[nt][m][1] = transpose8x8(pack2<T>(s[nt][m][2], s[nt][m][3]));
       }
+    }
+    if (MASK) {
+      // what v holds at a key that none of the rows keeps must not be multiplied with its weight of 0:
+      // lanes 4 g .. 4 g + 3 know of key g + 8 e, this one holds keys 2 t, 2 t + 1 + 8 e of v
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned all = __ballot_sync(~0u, kept >> (2 * m + (e >> 1)) & 1u);
+          if (!(all >> (4 * (2 * t + (e & 1))) & 0xfu))
+#pragma unroll
+            for (int x = 0; x < VB; ++x) vr[m][x][e] = make_uint4(0u, 0u, 0u, 0u);
+        }
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -381,15 +396,19 @@ size_t attention_single_workspace(const gs_attention_args& a) {
   return splits > kClusterSplits ? (size_t)(splits * rows) * (a.D + 1) * sizeof(float) : 0;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int NT>
 static cudaError_t launch_single(const SingleParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)p.a.B * p.a.Hkv, p.splits), cluster(1, p.cluster ? p.splits : 1);
-  if constexpr (DP == 64)
-    if (p.rows > 8)
-      return launch_overlapped_clusters(attention_single_kernel<T, DP, 2>, grid, cluster,
-                                        kSingleWarps * 32, 0, stream, p);
-  return launch_overlapped_clusters(attention_single_kernel<T, DP, 1>, grid, cluster,
-                                    kSingleWarps * 32, 0, stream, p);
+  return launch_overlapped_clusters(p.a.mask ? attention_single_kernel<T, DP, NT, true>
+                                             : attention_single_kernel<T, DP, NT, false>,
+                                    grid, cluster, kSingleWarps * 32, 0, stream, p);
+}
+
+template <typename T>
+static cudaError_t launch_single(const SingleParams& p, cudaStream_t stream) {
+  return p.a.D > 64   ? launch_single<T, 128, 1>(p, stream)
+         : p.rows > 8 ? launch_single<T, 64, 2>(p, stream)
+                      : launch_single<T, 64, 1>(p, stream);
 }
 
 int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t stream) {
@@ -402,12 +421,8 @@ int attention_single(const gs_attention_args& a, void* workspace, cudaStream_t s
   const long long rows = (long long)a.B * a.Hq * a.Lq;
   p.part_out = static_cast<float*>(workspace);
   p.part_lse = p.part_out + p.splits * rows * a.D;
-  if (a.dtype == GS_FP16)
-    GS_CUDA(a.D <= 64 ? (launch_single<__half, 64>(p, stream))
-                      : (launch_single<__half, 128>(p, stream)));
-  else
-    GS_CUDA(a.D <= 64 ? (launch_single<__nv_bfloat16, 64>(p, stream))
-                      : (launch_single<__nv_bfloat16, 128>(p, stream)));
+  GS_CUDA(a.dtype == GS_FP16 ? launch_single<__half>(p, stream)
+                             : launch_single<__nv_bfloat16>(p, stream));
   count_launches(1u);
   if (p.splits > kClusterSplits) {
     GS_CUDA(attention_combine(a, p.splits, p.part_out, p.part_lse, stream));

@@ -434,8 +434,9 @@ GS_API int gs_rms_norm_backward(int dtype, long long rows, int width, const void
  * lengths[B] (device, or NULL): the keys of each batch item, held to [0, Lk]; what lies past them
  * is not looked at. mask (device bytes, or NULL): 0 leaves a key out for a query; strides for
  * batch item, head and query (0 where they share), keys contiguous. What k and v hold at a key
- * that all queries of a batch item leave out (head and query stride 0) never reaches a result,
- * NaN included; under a mask that differs between queries, v must be finite.
+ * that no query keeps of the batch item and of the heads that share it never reaches a result, NaN
+ * included. At a key that some of them keep and others leave out, v (for the backward also k) must
+ * be finite: the weight 0 is multiplied with it.
  * A query that keeps no key has out = 0, lse = -inf and no gradient.
  * lse[B, Hq, Lq] (or NULL; the backward needs it): log sum exp of the scaled scores.
  * gs_cross_attention_backward: gradients in the layouts of q, k and v, from the same arguments,
