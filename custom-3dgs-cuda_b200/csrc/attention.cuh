@@ -54,18 +54,20 @@ __device__ __forceinline__ unsigned below(int left, int w) {
 
 // The keys of tile `tile` (of 128) that any query of key head hk keeps, in two steps so that the loads can
 // be in flight meanwhile; for a whole warp, whose lanes then all have it. All loads are in flight at
-// once, lanes without a row read the last one (a loop with a trip count of each lane's own takes its
-// odd trips one after another: 306 -> 641 us at 3 x 6,000 x 10,000, 4 heads of 64).
+// once (a loop with a trip count of each lane's own takes its odd trips one after another: 306 -> 641 us
+// at 3 x 6,000 x 10,000, 4 heads of 64).
 constexpr int kKeptMost = 256;  // rows, at most
 __device__ __forceinline__ uint4 kept_begin(const AttentionParams& p, int b, int hk, int tile) {
-  const unsigned* at = p.kept + b * p.kept_b + hk * p.kept_h + (long long)tile * p.kept_tile;
+  const int lane = threadIdx.x % 32;
+  const long long step = 32ll * p.kept_row;
+  const unsigned* at = p.kept + b * p.kept_b + hk * p.kept_h + (long long)tile * p.kept_tile +
+                       (long long)lane * p.kept_row;
   uint4 w[kKeptMost / 32], any = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
   for (int k = 0; k < kKeptMost / 32; ++k) {
     w[k] = make_uint4(0u, 0u, 0u, 0u);
-    if (32 * k < p.kept_rows)
-      w[k] = *reinterpret_cast<const uint4*>(
-          at + (long long)min(32 * k + (int)(threadIdx.x % 32), p.kept_rows - 1) * p.kept_row);
+    if (32 * k + lane < p.kept_rows) w[k] = *reinterpret_cast<const uint4*>(at);
+    at += step;
   }
 #pragma unroll
   for (int k = 0; k < kKeptMost / 32; ++k)

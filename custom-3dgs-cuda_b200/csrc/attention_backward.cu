@@ -37,7 +37,7 @@
 // norms of a row of dO and of a kept row of v the largest dS ends up below 2^15, and those down to
 // 2^-29 of it keep all their bits. (As it is, dS of 999 x 3,600 lies among half's subnormals
 // from a dO of deviation 1e-3 down: 6 times the error of the results' own rounding.) Reading v once more
-// for its norms, and clearing them first, costs 4 us of 111 there, forward included, and 13 of 398 at
+// for its norms, and clearing them first, costs 4 us of 111 there, forward included, and 2 of 395 at
 // 4,096 x 4,096, 16 heads of 64. The power is at least 1: where dO is so large that dS may pass 65,504, the loss is scaled too far up, as with any
 // half gradient.
 #include <algorithm>
@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttentionParams 
   }
 #pragma unroll
   for (int w = 4; w; w >>= 1) delta += __shfl_xor_sync(~0u, delta, w);
+  if (lse == INFINITY) delta = 0.0f;  // keeps no key, whatever dO holds
   if (sub == 0) {
     float* tile = stats + at / kInner * (2 * kInner) + at % kInner;
     tile[0] = lse;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   using PS = ProbabilityScale<T>;
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t x_full, y1_full[S::kStages1], y1_free[S::kStages1], y2_full[S::kStages2],
-      y2_free[S::kStages2], y1_clean[S::kStages1], s_full, s_read, dp_full, p_ready, ds_ready, acc_done, acc_full;
+      y2_free[S::kStages2], y1_clean[S::kStages1], y2_clean[S::kStages2], s_full, s_read, dp_full, p_ready, ds_ready, acc_done, acc_full;
   __shared__ unsigned tmem_slot;
   __shared__ volatile int gave_up;
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int i = 0; i < S::kStages2; ++i) {
       mbar_set(&y2_full[i], 1);
+      mbar_set(&y2_clean[i], 1);
       mbar_set(&y2_free[i], 1);
     }
     for (uint64_t* bar : {&s_full, &dp_full, &acc_done}) mbar_set(bar, 1);
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int outer_rows = KEYS ? a.Lk : a.Lq, outer_heads = KEYS ? a.Hkv : a.Hq;
   const int outer_tiles = (outer_rows + kOuter - 1) / kOuter;
   const int x0 = blockIdx.x % outer_tiles * kOuter, bh = blockIdx.x / outer_tiles;
-  const int b = bh / outer_heads, ho = bh % outer_heads;
+  const int b = bh / outer_heads, ho = bh % outer_heads, hk = KEYS ? ho : ho / shared_heads;
   const int n = warp_uniform(key_count(a, b));
   const int q_tiles = p.lq_pad / kInner;
   const int tiles = KEYS ? (x0 < n ? q_tiles * shared_heads : 0) : (n + kInner - 1) / kInner;
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // dS's scale over P's, and dS's back to 1; dq, which needs P for dS alone, forms P with dS's scale
     float ds_up = 1.0f, ds_back = PS::kAcc, p_log2 = 0.0f;
     if (PS::kOwnDs && count > 0) {
-      const int k = ds_log2(p.norms + 2 * ((long long)b * a.Hkv + (KEYS ? ho : ho / shared_heads)));
+      const int k = ds_log2(p.norms + 2 * ((long long)b * a.Hkv + hk));
       ds_back = __uint_as_float((unsigned)(127 - k) << 23);
       if (KEYS)
         ds_up = PS::kAcc / ds_back;
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         for (int j = 0; j < count; ++j) {
           const int t = t0 + j;
-          const int head = KEYS ? ho * shared_heads + t / q_tiles : ho / shared_heads;
+          const int head = KEYS ? ho * shared_heads + t / q_tiles : hk;
           const int y = (KEYS ? t % q_tiles : t) * kInner;
           const int st1 = j % S::kStages1, st2 = j % S::kStages2;
           if (!tc_wait(&y1_free[st1], (j / S::kStages1 & 1) ^ 1)) { gave_up = 1; break; }
@@ -545,12 +547,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     (second ? tm_p : tm_ds) + (k / 4) * kHalf + (k % 4) * 8, in + k * 128,
                     idesc_acc, j > 0 || k > 0);
       };
+      // with a mask, another warp has looked the tiles over
       const auto arrived1 = [&](int j) {
-        const int st = j % S::kStages1;
-        return tc_wait_warp(KEYS ? &y1_full[st] : &y1_clean[st], j / S::kStages1 & 1);
+        const int st = j % S::kStages1, left = n - (t0 + j) * kInner;
+        if (!tc_wait_warp(a.bits ? &y1_clean[st] : &y1_full[st], j / S::kStages1 & 1)) return false;
+        if (!KEYS && !a.bits && warp == 8 && left < kInner)  // k past the length
+          clear_rows<S::kBoxes>(sm_y1 + st * S::kInnerBytes, left, make_uint4(~0u, ~0u, ~0u, ~0u));
+        return true;
       };
       const auto arrived2 = [&](int j) {
-        return tc_wait_warp(&y2_full[j % S::kStages2], j / S::kStages2 & 1);
+        const int st = j % S::kStages2;
+        return tc_wait_warp(KEYS && a.bits ? &y2_clean[st] : &y2_full[st], j / S::kStages2 & 1);
       };
       const auto when = [&](uint64_t* bar, int j) {
         const bool done = tc_wait_warp(bar, j & 1);
@@ -625,15 +632,37 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       if (!ok && count > 0) gave_up = 1;
-    } else if (warp == 11 && !KEYS) {
+    } else if (warp == 11 && KEYS && a.bits) {
+      // ---- nor must what q and dO hold at queries that keep no key reach dk and dv
+      for (int j = 0; j < count; ++j) {
+        const int st1 = j % S::kStages1, st2 = j % S::kStages2;
+        if (!tc_wait_warp(&y1_full[st1], j / S::kStages1 & 1)) { gave_up = 1; break; }
+        unsigned keep[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {  // the rows past the last query are zero as it is
+          float lse;
+          asm volatile("ld.shared.f32 %0, [%1];"
+                       : "=f"(lse)
+                       : "r"(sm_stats + st1 * S::kStatBytes + (32 * w + lane) * 4));
+          keep[w] = __ballot_sync(~0u, lse != INFINITY) |
+                    ~below(a.Lq - (t0 + j) % q_tiles * kInner, w);
+        }
+        const uint4 rows = make_uint4(keep[0], keep[1], keep[2], keep[3]);
+        const bool some = has_hidden_rows(kInner, rows);
+        if (some) clear_rows<S::kBoxes>(sm_y1 + st1 * S::kInnerBytes, kInner, rows);
+        mbar_arrive_warp(&y1_clean[st1]);
+        if (!tc_wait_warp(&y2_full[st2], j / S::kStages2 & 1)) { gave_up = 1; break; }
+        if (some) clear_rows<S::kBoxes>(sm_y2 + st2 * S::kInnerBytes, kInner, rows);
+        mbar_arrive_warp(&y2_clean[st2]);
+      }
+    } else if (warp == 11 && !KEYS && a.bits) {
       // ---- what k holds at keys that no query of the item's key head keeps must not reach dq, where
       // 0 times NaN would be added: those rows are set to zero before the products may read them
       for (int j = 0; j < count; ++j) {
         const int st = j % S::kStages1, key = (t0 + j) * kInner;
-        uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);
-        if (a.bits) keep = kept_begin(a, b, ho / shared_heads, t0 + j);
+        uint4 keep = kept_begin(a, b, hk, t0 + j);
         if (!tc_wait_warp(&y1_full[st], j / S::kStages1 & 1)) { gave_up = 1; break; }
-        if (a.bits) keep = kept_end(keep);
+        keep = kept_end(keep);
         if (has_hidden_rows(n - key, keep))
           clear_rows<S::kBoxes>(sm_y1 + st * S::kInnerBytes, n - key, keep);
         mbar_arrive_warp(&y1_clean[st]);

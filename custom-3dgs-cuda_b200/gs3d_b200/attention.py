@@ -14,7 +14,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """softmax(scale q k^T) v for q[B, Lq, Hq, D] and k, v[B, Lk, Hkv, D] of float16 or bfloat16,
     D a multiple of 8 up to 128, Hq a multiple of Hkv (neighbouring query heads share a key head).
     `lengths` (int32 [B]): the keys of each batch item; later ones are not looked at. `mask` (bool,
-    [B or 1, Hq or 1, Lq or 1, Lk]): False leaves a key out. A query that keeps no key gives zeros.
+    [B or 1, Hq or 1, Lq or 1, Lk]): False leaves a key out. A query that keeps no key gives zeros and
+    takes no part in the gradients, whatever it holds.
     `scale` is 1 / sqrt(D) unless given. With `return_lse`, (out, lse[B, Hq, Lq] float32): log sum
     exp of the scaled scores, -inf for a query without keys; no gradient flows through it. First
     derivatives backwards only: a tangent (forward mode) is refused.

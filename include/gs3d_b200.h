@@ -437,7 +437,8 @@ GS_API int gs_rms_norm_backward(int dtype, long long rows, int width, const void
  * that no query keeps of the batch item and of the heads that share it never reaches a result, NaN
  * included. At a key that some of them keep and others leave out, v (for the backward also k) must
  * be finite: the weight 0 is multiplied with it.
- * A query that keeps no key has out = 0, lse = -inf and no gradient.
+ * A query that keeps no key has out = 0, lse = -inf and no gradient, and gives none, whatever it and
+ * its dout hold.
  * lse[B, Hq, Lq] (or NULL; the backward needs it): log sum exp of the scaled scores.
  * gs_cross_attention_backward: gradients in the layouts of q, k and v, from the same arguments,
  * the forward's out and lse. Sums run in a fixed order: the same bits on every run.

@@ -75,3 +75,24 @@ def test_one_key_head_leaves_out_what_another_keeps(cuda_device, dtype):
         k2, v2 = k.clone(), v.clone()
         k2[:, 100:200, 0], v2[:, 100:200, 0] = float("nan"), float("inf")
         check(q, k, v, g, mask, None, (q, k2, v2, g))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ("query", "shared", "full"))
+@pytest.mark.parametrize("size", SIZES)
+def test_queries_that_keep_no_key(cuda_device, dtype, kind, size):
+    """They have no gradient and give none, whatever they and their upstream gradients hold."""
+    B, Lq, Lk, Hq, Hkv, D = size
+    q, k, v, g = draw(cuda_device, dtype, *size, seed=45)
+    mask = draw_mask(cuda_device, kind, B, Lq, Lk, Hq, 46)
+    mask[:, :, ::3] = False
+    if kind == "full":
+        mask[:, Hq - 1, -1] = False
+    dead = ~mask.expand(B, Hq, Lq, Lk).any(3).transpose(1, 2)  # [B, Lq, Hq]
+    assert dead.any()
+    q, g = q.masked_fill(dead[..., None], 0.0), g.masked_fill(dead[..., None], 0.0)
+    q2, g2 = q.clone(), g.clone()
+    for i, bad in enumerate((float("nan"), float("inf"), torch.finfo(dtype).min)):
+        at = dead & (torch.arange(Lq, device=cuda_device) // 3 % 3 == i)[None, :, None]
+        q2[at], g2[at] = bad, bad
+    check(q, k, v, g, mask, None, (q2, k, v, g2))
