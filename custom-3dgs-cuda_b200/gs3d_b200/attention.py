@@ -23,6 +23,6 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Tensors whose last axis is contiguous are used in place, whatever the other strides, if address
     and strides are multiples of 16 bytes; others are copied first. What k and v hold at a key that no
     query of its batch item keeps, of none of the heads that share it, never reaches a result, NaN
-    included. Where some of them keep a key and others do not, v must be finite there, for gradients
-    k too."""
+    included. Where some of them keep a key and others do not, v must be finite there; gradients need
+    a finite k at every key that is kept."""
     return native.cross_attention(q, k, v, lengths, mask, scale, return_lse)

@@ -435,8 +435,8 @@ GS_API int gs_rms_norm_backward(int dtype, long long rows, int width, const void
  * is not looked at. mask (device bytes, or NULL): 0 leaves a key out for a query; strides for
  * batch item, head and query (0 where they share), keys contiguous. What k and v hold at a key
  * that no query keeps of the batch item and of the heads that share it never reaches a result, NaN
- * included. At a key that some of them keep and others leave out, v (for the backward also k) must
- * be finite: the weight 0 is multiplied with it.
+ * included. At a key that some of them keep and others leave out, v must be finite: the weight 0 is
+ * multiplied with it. The backward needs a finite k at every key that is kept, for the same reason.
  * A query that keeps no key has out = 0, lse = -inf and no gradient, and gives none, whatever it and
  * its dout hold.
  * lse[B, Hq, Lq] (or NULL; the backward needs it): log sum exp of the scaled scores.
