@@ -5,6 +5,7 @@
 
 #include "device_errors.h"
 #include "overlap.cuh"
+#include "pieces.h"
 #include "token_types.cuh"
 
 namespace gs {

@@ -320,10 +320,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int n = warp_uniform(key_count(a, b));
   const int q_tiles = p.lq_pad / kInner;
   const int tiles = KEYS ? (x0 < n ? q_tiles * shared_heads : 0) : (n + kInner - 1) / kInner;
-  // at most 2^24 tiles times kSms splits fit 32 bits
-  const unsigned splits = (unsigned)p.splits;
-  const int t0 = (int)((unsigned)tiles * blockIdx.y / splits);
-  const int count = (int)((unsigned)tiles * (blockIdx.y + 1) / splits) - t0;
+  // dq's tiles of keys, fewer than 2^24, times at most kSms splits fit 32 bits, which divide faster
+  const auto begin = [&](unsigned piece) {
+    return KEYS ? piece_begin(tiles, piece, p.splits)
+                : (int)((unsigned)tiles * piece / (unsigned)p.splits);
+  };
+  const int t0 = begin(blockIdx.y), count = begin(blockIdx.y + 1) - t0;
   const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
 
   // dk and dv need the rows' statistics and with them the packed mask; the CTAs of dq that start

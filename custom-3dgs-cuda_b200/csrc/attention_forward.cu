@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (!a.bits) wait_for_previous();
   const int n = warp_uniform(key_count(a, b));
   const int tiles = (n + kTileK - 1) / kTileK;
-  // fewer than 2^24 tiles times at most kSms splits fit 32 bits
+  // fewer than 2^24 tiles times at most kSms splits fit 32 bits, which divide faster than 64
   const unsigned splits = (unsigned)p.splits;
   const int t0 = (int)((unsigned)tiles * blockIdx.y / splits);
   const int count = (int)((unsigned)tiles * (blockIdx.y + 1) / splits) - t0;

@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
   const int b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv;
   const int n = key_count(a, b);
   const int chunks = (n + kChunk - 1) / kChunk;
-  const int c0 = (int)((long long)chunks * blockIdx.y / p.splits);
-  const int c1 = (int)((long long)chunks * (blockIdx.y + 1) / p.splits);
+  const int c0 = piece_begin(chunks, blockIdx.y, p.splits);
+  const int c1 = piece_begin(chunks, blockIdx.y + 1, p.splits);
   const unsigned char* mask_b = a.mask + b * a.mask_b;
 
   const auto head_of = [&](int r) { return hk * shared_heads + r % shared_heads; };
