@@ -10,6 +10,10 @@
 
 namespace gs {
 
+// Rows of queries (of all items and query heads) and of keys (items and key heads), at most: indexes of
+// rows are 32-bit, and a tile, or a warp's next chunks, may reach this far past the last row.
+static constexpr long long kMaxRows = (1ll << 31) - 1024;
+
 // The checks that forward and backward share; "" or what is wrong.
 static const char* attention_fault(const gs_attention_args& a) {
   if (a.dtype != GS_FP16 && a.dtype != GS_BF16) return "dtype must be GS_FP16 or GS_BF16";
@@ -17,8 +21,11 @@ static const char* attention_fault(const gs_attention_args& a) {
   if (a.D < 8 || a.D > 128 || a.D % 8) return "the head size must be a multiple of 8 up to 128";
   if (a.Hkv == 0 ? a.Hq != 0 : a.Hq % a.Hkv) return "the key heads must divide the query heads";
   if (!std::isfinite(a.scale)) return "the scale must be finite";
-  if ((long long)a.B * a.Hq * a.Lq >= (1ll << 31) || (long long)a.B * a.Hkv * a.Lk >= (1ll << 31))
-    return "more than 2^31 rows";
+  // two factors fit 64 bits; all three may not
+  const auto many = [&](int heads, int tokens) {
+    return tokens > 0 && (long long)a.B * heads > kMaxRows / tokens;
+  };
+  if (many(a.Hq, a.Lq) || many(a.Hkv, a.Lk)) return "more than 2^31 - 1024 rows";
   return "";
 }
 

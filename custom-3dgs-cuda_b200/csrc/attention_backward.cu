@@ -724,9 +724,9 @@ static BackwardPlan backward_plan(const gs_attention_args& a) {
   };
   plan.lq_pad = tiles(a.Lq, kInner) * kInner;
   if (a.Hkv > 0)
-    plan.key_splits = splits(a.B * a.Hkv * tiles(a.Lk, kOuter),
+    plan.key_splits = splits((long long)a.B * a.Hkv * tiles(a.Lk, kOuter),
                              tiles(a.Lq, kInner) * (a.Hq / a.Hkv));
-  plan.query_splits = splits(a.B * a.Hq * tiles(a.Lq, kOuter), tiles(a.Lk, kInner));
+  plan.query_splits = splits((long long)a.B * a.Hq * tiles(a.Lq, kOuter), tiles(a.Lk, kInner));
   if (plan.key_splits > 1)
     plan.key_floats = (long long)plan.key_splits * a.B * a.Hkv * a.Lk * a.D;
   if (plan.query_splits > 1)
@@ -734,7 +734,7 @@ static BackwardPlan backward_plan(const gs_attention_args& a) {
   if (a.dtype == GS_FP16 && plan.lq_pad && a.Hq > 0)
     plan.norm_floats = ((long long)a.B * a.Hkv * 2 + 3) / 4 * 4;
   // dk, dv and dq in turn use the same parts
-  plan.bytes = (size_t)(a.B * a.Hq * plan.lq_pad * 2 + plan.norm_floats) * sizeof(float) +
+  plan.bytes = (size_t)((long long)a.B * a.Hq * plan.lq_pad * 2 + plan.norm_floats) * sizeof(float) +
                (size_t)std::max(2 * plan.key_floats, plan.query_floats) * sizeof(float);
   return plan;
 }
@@ -784,7 +784,7 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   const size_t mask_bytes = attention_mask_bytes(a);
   float* stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + mask_bytes);
   p.stats = stats;
-  const long long stat_rows = a.B * a.Hq * plan.lq_pad;
+  const long long stat_rows = (long long)a.B * a.Hq * plan.lq_pad;
   float* norms = stats + 2 * stat_rows;
   p.norms = norms;
   float* parts = norms + plan.norm_floats;

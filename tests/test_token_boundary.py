@@ -179,3 +179,29 @@ def test_python_refusals(cuda_device):
             ((q, q, q), dict(lengths=torch.zeros(2, dtype=torch.int32)), "lengths")]:
         with pytest.raises(RuntimeError, match=msg):
             cross_attention(*args, **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(Lk=(1 << 31) - 1, D=8), dict(Lk=(1 << 31) - 1000, D=8),
+                                dict(Lq=(1 << 31) - 1, D=8), dict(B=1 << 30, Hq=1 << 30, Lq=1 << 30),
+                                dict(B=1 << 30, Hkv=1 << 30, Hq=1 << 30, Lq=0, Lk=16)])
+def test_attention_refuses_rows_whose_tiles_would_pass_32_bits(kw):
+    """A tile that reaches past the last row has to have indexes too; the product of three sizes may pass
+    64 bits."""
+    from custom_rasterizer_cuda import _lib
+
+    L, a = _lib.lib, attention_args(lse=A, **kw)
+    p, v = ctypes.addressof(a), ctypes.addressof(a.out)
+    assert L.gs_cross_attention_forward(p, A, 1 << 62, None) == _lib.GS_ERR_INVALID_ARG
+    assert b"rows" in L.gs_last_error()
+    assert L.gs_cross_attention_backward(p, v, v, v, v, A, 1 << 62, None) == _lib.GS_ERR_INVALID_ARG
+    assert b"rows" in L.gs_last_error()
+    assert L.gs_cross_attention_workspace_size(p) == 0
+    assert L.gs_cross_attention_backward_workspace_size(p) == 0
+
+
+def test_attention_workspace_sizes_count_in_64_bits():
+    from custom_rasterizer_cuda import _lib
+
+    # 2^21 queries' statistics of two floats, and their parts; nothing but those without keys
+    a = attention_args(B=1 << 10, Hq=1 << 6, Hkv=1, Lq=1 << 14, Lk=0, D=8)
+    assert _lib.lib.gs_cross_attention_backward_workspace_size(ctypes.addressof(a)) >= 8 << 30
