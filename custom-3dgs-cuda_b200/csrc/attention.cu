@@ -40,6 +40,15 @@ static const char* view_fault(const gs_token_view& v, int tokens, int heads) {
   return "";
 }
 
+// The workspace holds bits, sums and parts that are read 16 bytes at a time.
+static const char* workspace_fault(const void* workspace, size_t bytes, size_t needed) {
+  if (bytes < needed) return "workspace too small";
+  if (needed && !workspace) return "null pointer";
+  if (needed && reinterpret_cast<uintptr_t>(workspace) % 16)
+    return "the workspace must start on a 16-byte boundary";
+  return "";
+}
+
 AttentionParams attention_params(const gs_attention_args& a) {
   AttentionParams p{};
   p.B = a.B, p.Lq = a.Lq, p.Lk = a.Lk, p.Hq = a.Hq, p.Hkv = a.Hkv, p.D = a.D;
@@ -73,9 +82,8 @@ extern "C" int gs_cross_attention_forward(const gs_attention_args* a, void* work
     fault = view_fault(*v, keys ? a->Lk : a->Lq, keys ? a->Hkv : a->Hq);
     GS_REQUIRE(!*fault, fault);
   }
-  const size_t needed = gs_cross_attention_workspace_size(a);
-  GS_REQUIRE(workspace_bytes >= needed, "workspace too small");
-  GS_REQUIRE(workspace || !needed, "null pointer");
+  fault = workspace_fault(workspace, workspace_bytes, gs_cross_attention_workspace_size(a));
+  GS_REQUIRE(!*fault, fault);
   return attention_is_single(*a) ? attention_single(*a, workspace, (cudaStream_t)stream)
                                  : attention_forward(*a, workspace, (cudaStream_t)stream);
   GS_API_END();
@@ -106,9 +114,8 @@ extern "C" int gs_cross_attention_backward(const gs_attention_args* a, const gs_
     GS_REQUIRE(!*fault, fault);
   }
   GS_REQUIRE(no_queries || a->lse, "the backward needs the forward's lse");
-  GS_REQUIRE(workspace_bytes >= gs_cross_attention_backward_workspace_size(a),
-             "workspace too small");
-  GS_REQUIRE(no_queries || workspace, "null pointer");
+  fault = workspace_fault(workspace, workspace_bytes, gs_cross_attention_backward_workspace_size(a));
+  GS_REQUIRE(!*fault, fault);
   return attention_backward(*a, *dout, *dq, *dk, *dv, workspace, (cudaStream_t)stream);
   GS_API_END();
 }

@@ -431,7 +431,7 @@ GS_API int gs_rms_norm_backward(int dtype, long long rows, int width, const void
  * out = softmax(scale q k^T) v for each query head, Hq / Hkv query heads sharing a key head.
  * q, out: [B, Lq, Hq, D]; k, v: [B, Lk, Hkv, D], half or bfloat16, D a multiple of 8 up to 128;
  * every view starts on a 16-byte boundary with strides of multiples of 8 elements. B Hq Lq and
- * B Hkv Lk are at most 2^31 - 1024.
+ * B Hkv Lk are at most 2^31 - 1024. The workspace starts on a 16-byte boundary.
  * lengths[B] (device, or NULL): the keys of each batch item, held to [0, Lk]; what lies past them
  * is not looked at. mask (device bytes, or NULL): 0 leaves a key out for a query; strides for
  * batch item, head and query (0 where they share), keys contiguous. What k and v hold at a key

@@ -205,3 +205,21 @@ def test_attention_workspace_sizes_count_in_64_bits():
     # 2^21 queries' statistics of two floats, and their parts; nothing but those without keys
     a = attention_args(B=1 << 10, Hq=1 << 6, Hkv=1, Lq=1 << 14, Lk=0, D=8)
     assert _lib.lib.gs_cross_attention_backward_workspace_size(ctypes.addressof(a)) >= 8 << 30
+
+
+def test_attention_refuses_a_workspace_it_cannot_read_16_bytes_at_a_time():
+    from custom_rasterizer_cuda import _lib
+
+    L, bad = _lib.lib, _lib.GS_ERR_INVALID_ARG
+    # one with a mask, one whose keys are split; the backward always needs one
+    for kw in (dict(Lq=100, mask=A, mask_query_stride=4), dict(Lk=1 << 20, Lq=40)):
+        a = attention_args(lse=A, **kw)
+        p, v = ctypes.addressof(a), ctypes.addressof(a.out)
+        assert L.gs_cross_attention_workspace_size(p) > 0
+        for off in (4, 8):
+            assert L.gs_cross_attention_forward(p, A + off, 1 << 40, None) == bad
+            assert b"workspace" in L.gs_last_error()
+            assert L.gs_cross_attention_backward(p, v, v, v, v, A + off, 1 << 40, None) == bad
+            assert b"workspace" in L.gs_last_error()
+        assert L.gs_cross_attention_forward(p, None, 1 << 40, None) == bad
+        assert L.gs_cross_attention_backward(p, v, v, v, v, None, 1 << 40, None) == bad
