@@ -75,10 +75,11 @@ __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
   return r;
 }
 
+// Not the read-only path: this kernel may start while the one that makes q, k or v still runs.
 __device__ __forceinline__ uint4 load16(const void* p, bool in) {
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
   if (in)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p));
   return v;

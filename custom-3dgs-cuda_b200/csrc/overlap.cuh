@@ -1,7 +1,8 @@
 // Kernels that overlap at their ends (programmatic dependent launch). A kernel launched so may start
 // before the one in front of it in the stream has ended; it waits for that one's end before it
 // touches memory that the other may write or still read, which hides the launch and its set-up
-// (1 to 2 us between small kernels). A kernel that lets the next one start early only gives up the
+// (1 to 2 us between small kernels). Such a kernel does not read through the read-only path (ld.global.nc,
+// __ldg, const __restrict__), which is for data that nobody writes while the kernel lives. A kernel that lets the next one start early only gives up the
 // room on the SMs: the next one still waits.
 #pragma once
 
