@@ -224,7 +224,7 @@ __device__ __forceinline__ void hide(const unsigned (&keep)[2], bool negative, u
   for (int k = 0; k < 64; ++k)
     if (!(keep[k / 32] >> (k % 32) & 1u)) {
       if (s) s[k] = none;
-      dp[k] = 0u;
+      if (dp) dp[k] = 0u;
     }
 }
 
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
       } else {
         tc_wait_ld();
-        if (hidden) hide(keep, c < 0.0f, pr, dp);
+        if (hidden) hide(keep, c < 0.0f, pr, nullptr);
 #pragma unroll
         for (int h = 0; h < 64; h += 32) {
           probabilities<KEYS>(pr + h, c, stat + h * 4, mine.x);

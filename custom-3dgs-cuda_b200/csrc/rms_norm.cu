@@ -366,15 +366,13 @@ static void with_row_shape(int width, bool packed, F&& f) {
     return;
   }
   const int n = width / V;
-  if (n <= 32)
-    f.template operator()<V, 1, 32>();
-  else if (n <= 64)
-    f.template operator()<V, 2, 32>();
-  else if (n <= 32 * MOST)
-    f.template operator()<V, MOST, 32>();
-  else if (n <= 64 * MOST)
-    f.template operator()<V, MOST, 64>();
-  else if (n <= 128 * MOST)
+  if (n <= 32) return f.template operator()<V, 1, 32>();
+  if (n <= 64) return f.template operator()<V, 2, 32>();
+  if constexpr (MOST > 2)
+    if (n <= 32 * MOST) return f.template operator()<V, MOST, 32>();
+  if constexpr (MOST > 1)
+    if (n <= 64 * MOST) return f.template operator()<V, MOST, 64>();
+  if (n <= 128 * MOST)
     f.template operator()<V, MOST, 128>();
   else if (n <= 256 * MOST)
     f.template operator()<V, MOST, 256>();

@@ -127,10 +127,6 @@ __device__ __forceinline__ void tc_wait_ld() {
 __device__ __forceinline__ void tc_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-// Shared-memory writes of this thread become visible to the copy and matrix engines.
-__device__ __forceinline__ void fence_async_shared() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
 
 // Arrives on `bar` when every matrix product issued by this thread so far has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
