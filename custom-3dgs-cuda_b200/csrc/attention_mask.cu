@@ -180,8 +180,8 @@ size_t attention_mask_bytes(const gs_attention_args& a) {
 
 int attention_pack_mask(const gs_attention_args& a, AttentionParams& p, void* workspace,
                         cudaStream_t stream) {
-  if (!a.mask || a.Lk == 0) return GS_OK;
   const MaskShape m = mask_shape(a);
+  if (!a.mask || a.Lk == 0 || m.b * m.h * m.q == 0) return GS_OK;
   unsigned* bits = static_cast<unsigned*>(workspace);
   p.bits = bits;
   p.bits_q = m.q > 1 ? m.words : 0;

@@ -96,3 +96,25 @@ def test_queries_that_keep_no_key(cuda_device, dtype, kind, size):
         at = dead & (torch.arange(Lq, device=cuda_device) // 3 % 3 == i)[None, :, None]
         q2[at], g2[at] = bad, bad
     check(q, k, v, g, mask, None, (q2, k, v, g2))
+
+
+def test_no_queries_under_a_mask(cuda_device):
+    """At the C entry point, where a mask of queries without queries may be given: dk and dv are 0."""
+    import ctypes
+
+    from custom_rasterizer_cuda import _lib
+
+    k, v, dk, dv = (torch.randn(1, 5, 1, 64, device=cuda_device).half() for _ in range(4))
+    mask = torch.ones(5, dtype=torch.bool, device=cuda_device)
+    view = lambda t: _lib.TokenView(t.data_ptr() if t is not None else None, 320, 64, 64)  # noqa: E731
+    a = _lib.AttentionArgs(_lib.GS_FP16, 1, 0, 5, 1, 1, 64, 0.125, view(None), view(k), view(v),
+                           view(None), None, mask.data_ptr(), 0, 0, 5, None)
+    none, vk, vv = view(None), view(dk), view(dv)
+    p = [ctypes.addressof(x) for x in (a, none, none, vk, vv)]
+    size = _lib.lib.gs_cross_attention_backward_workspace_size(p[0])
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=cuda_device)
+    stream = torch.cuda.current_stream().cuda_stream
+    status = _lib.lib.gs_cross_attention_backward(*p, ws.data_ptr(), size, stream)
+    assert status == _lib.GS_OK, _lib.lib.gs_last_error()
+    torch.cuda.synchronize()
+    assert not dk.any() and not dv.any()
