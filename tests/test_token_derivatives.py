@@ -63,6 +63,9 @@ def test_tangents_are_refused(cuda_device):
     with fw.dual_level():
         for _, call in calls(cuda_device, lambda t: t):
             call()
+    with torch.inference_mode():
+        for _, call in calls(cuda_device, lambda t: t):
+            call()
 
 
 @pytest.mark.gpu
