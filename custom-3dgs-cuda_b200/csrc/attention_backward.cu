@@ -24,10 +24,17 @@
 // room: P takes S's columns and dS dP's, and one warp issues dv, the next S, dk, the next dP, each
 // as its operand arrives, so that S is formed beside the dS of the tile before.
 //
-// Measured, 4,096 queries x 4,096 keys, 16 heads, bfloat16: at D 128 14.5 us for delta, 255 for dk and
-// dv (1,080 TFLOP/s executed, tensor pipe 62% busy) and 178 for dq (1,160, 72%); at D 64 10, 174 and
-// 151. 8,192 x 16,320, 16 heads of 128, forward included: 4.2 ms, 1,290 TFLOP/s executed, near
-// what a library product sustains under the power cap (1,360).
+// Measured, 4,096 queries x 4,096 keys, 16 heads, bfloat16: at D 128 14.5 us for delta, 237 to 255 for dk
+// and dv (1,080 to 1,160 TFLOP/s executed, tensor pipe 62% busy) and 159 to 178 for dq (1,160 to 1,300,
+// 72%); at D 64 10, 163 to 174 and 138 to 151. 8,192 x 16,320, 16 heads of 128, forward included: 4.2 to
+// 4.3 ms, 18 units of executed products of 2.7e11 operations, 1,150 to 1,170 TFLOP/s, 84 to 86% of what a
+// library product sustains under the power cap (1,357).
+//
+// delta is formed from the output as it was written, in 16 bits: an error of 2^-9 (half 2^-12) |dO| |O| of
+// a row, next to which that of dS's own rounding is of the same size, so that a gradient is about 1.4
+// roundings off instead of one. A 32-bit copy of the output, written by the forward and read here, would cost 6
+// bytes a number more (8 us of 560 at 4,096 x 4,096, 16 heads of 128) and twice the output's memory between
+// the two.
 //
 // P and dS are rounded to the products' 16-bit type, a relative error for bfloat16 down to 2^-126,
 // where the exponential's results and the products' operands end. Both are formed 2^32 times

@@ -369,19 +369,19 @@ __global__ void __launch_bounds__(kSingleWarps * 32, single_ctas(NT))
   cluster_wait();
 }
 
-// Against the kernel with tiles of 128 rows, in us with the joining of the splits: up to 8 rows 93
-// against 106 (2 x 65,280 keys, 8 heads of 128) and 18 against 26 (4 x 3,600, 16 of 64), 9 to 16 rows
-// at D up to 64 66 against 76 (2 x 65,280, 8 heads) and 24 against 26 (4 x 3,600, 16 heads); above,
-// where two groups of rows leave 2 CTAs an SM, it loses: 126 against 106, 40 against 35.
+// Against the kernel with tiles of 128 rows, in us with the joining of the splits: up to 8 rows 84
+// against 105 (2 x 65,280 keys, 8 heads of 128) and 15 against 25 (4 x 3,600, 16 of 64), 9 to 16 rows
+// at D up to 64 58 against 81 (2 x 65,280, 8 heads) and 20 against 25 (4 x 3,600, 16 heads); above,
+// where two groups of rows leave 2 CTAs an SM, it lost: 126 against 106, 40 against 35.
 bool attention_is_single(const gs_attention_args& a) {
   return a.Hkv > 0 && (long long)a.Lq * (a.Hq / a.Hkv) <= (a.D <= 64 ? 16 : 8);
 }
 
 // Splits of the keys: one wave of CTAs, each with at least two chunks for every warp. Up to 8 of them
-// are a cluster, which joins its parts through shared memory (4 x 3,600 keys of 16 heads of 64: 17.7 us,
-// 20.0 with a second kernel), so there are 8 rather than a few more, and where a warp has at most
-// 4 chunks with 8 (2 x 3,600, 16 heads of 64: 13.6 us with 8, 15.0 with 13; 3 x 8,160: 24.6 with 8, 26.5
-// with 9; but 2 x 16,320: 34.0 with 8, 31.0 with 13).
+// are a cluster, which joins its parts through shared memory (2 to 3 us less than a second kernel), so
+// there are 8 rather than a few more, and where a warp has at most 4 chunks with 8 (2 x 3,600, 16
+// heads of 64: 11.5 us with 8, 13.1 with 13; 3 x 8,160: 21.0 with 8, 22.5 with 9; but 2 x 16,320 took
+// 3 us more with 8 than with 13).
 static int single_splits(const gs_attention_args& a) {
   const long long pairs = (long long)a.B * a.Hkv;
   const long long chunk = a.D <= 64 ? 32 : 16;

@@ -4,16 +4,23 @@
 // Statistics and products are in 32 bits; h is rounded once when it is written to the residual
 // stream, and y is formed from the unrounded h. With u = h rstd and g = dy w:
 //   dh_total = rstd (g - u mean(g u)) + dh,  dx = dr = dh_total,  dw = sum over rows of dy u.
-// The backward reads the h that the forward wrote and the forward's rstd.
+// The backward reads the h that the forward wrote, rounded to T, and the forward's rstd, which is of the
+// unrounded one: dx is about 1.4 roundings off the exact gradient instead of one. Reading x and r in h's
+// place would cost one more input (134 MB, 20 us of 103, at 65,280 rows of 1,024 bfloat16).
 // 8 bits: for each row, or each group of `group` numbers of it, s = max|y| / 448 and
 // q = e4m3(y / s), so that y ~ q s (448 is e4m3's largest number); s = 0 where y is all zero, else
-// at least 2^-126, whose reciprocal is finite.
+// at least 2^-126, whose reciprocal is finite. y is multiplied by the reciprocal, two roundings in 32
+// bits where a division has one: where y / s lies that near to the middle of two e4m3 numbers, the other may
+// be taken.
 //
 // Bound by HBM: each input is read once and each output written once, the row staying in
 // registers between the sum of squares and the scaling. ROW threads hold one row, up to CHUNKS
 // packs of VEC elements each; the shape that fits the width best takes it (with_row_shape).
 // 65,280 rows of 1,024 bfloat16 with residual: 83 us (6.4 TB/s), with 8-bit rows 81 (5.8 TB/s),
-// gradient 103 (5.2 TB/s).
+// gradient 103 (5.2 TB/s). Where a row does not start on 16 bytes or has an odd end, single elements are
+// read: 16,384 rows of 1,001 bfloat16 take 21 us and 46 for the gradient, and above 1,024 numbers a row,
+// where a CTA of 1,024 threads has 64 registers a thread and spills, 8,192 of 2,001 225 and 782. So does
+// the gradient of more than 8,192 16-bit numbers (4,096 x 16,384: 242 us, 1.7 TB/s).
 // dw is summed by a fixed set of CTAs over their own rows into partial rows, which a second
 // kernel adds in a fixed order: the same bits on every run.
 #include <cuda_fp8.h>
