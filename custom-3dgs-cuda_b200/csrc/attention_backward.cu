@@ -44,8 +44,8 @@
 // norms of a row of dO and of a kept row of v the largest dS ends up below 2^15, and those down to
 // 2^-29 of it keep all their bits. (As it is, dS of 999 x 3,600 lies among half's subnormals
 // from a dO of deviation 1e-3 down: 6 times the error of the results' own rounding.) Reading v once more
-// for its norms, and clearing them first, costs 4 us of 111 there, forward included, and 2 of 395 at
-// 4,096 x 4,096, 16 heads of 64. The power is at least 1: where dO is so large that dS may pass 65,504, the loss is scaled too far up, as with any
+// for its norms takes attention_prepare_kernel from 9 to 16 us at 4,096 x 4,096, 16 heads of 64, of 393 with
+// the forward. The power is at least 1: where dO is so large that dS may pass 65,504, the loss is scaled too far up, as with any
 // half gradient.
 #include <algorithm>
 #include <cmath>
@@ -276,7 +276,9 @@ __device__ __forceinline__ void store_packed(unsigned at, const unsigned* v) {
   tc_st16(at, packed);
 }
 
-template <typename T, int DP, bool KEYS>
+// MASK: with a mask. Without one its code and the barriers of the warp that looks the tiles over for it
+// are not there (dk and dv of 2 x 999 x 3,600, 8 heads of 64: 57 us with them, 47 so).
+template <typename T, int DP, bool KEYS, bool MASK>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attention_backward_kernel(const __grid_constant__ BackwardParams p,
                               const __grid_constant__ CUtensorMap map_x1,
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 : (int)((unsigned)tiles * piece / (unsigned)p.splits);
   };
   const int t0 = begin(blockIdx.y), count = begin(blockIdx.y + 1) - t0;
-  const bool key_mask = a.bits && a.bits_h == 0 && a.bits_q == 0;
+  const bool key_mask = MASK && a.bits_h == 0 && a.bits_q == 0;
 
   // dk and dv need the rows' statistics and with them the packed mask; the CTAs of dq that start
   // beside the last of dk's and dv's then find both, and only end after them
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const float* tile = p.stats + (((long long)b * a.Hq + ho) * p.lq_pad + x0) * 2 + row;
         mine = make_float2(tile[0] - p_log2, tile[kInner]);
       }
-      if (a.bits)
+      if (MASK)
         keep_row = a.bits + b * a.bits_b + ho * a.bits_h + (long long)min(x, a.Lq - 1) * a.bits_q;
     }
     const unsigned my_s = tm_s + lanes + wg * 64, my_dp = tm_dp + lanes + wg * 64,
@@ -391,14 +393,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int j = 0; j < count; ++j) {
       const int st = j % S::kStages1, t = t0 + j;
       const int y0 = (KEYS ? t % q_tiles : t) * kInner + wg * 64;  // first of this thread's columns
-      const bool hidden = a.bits || (KEYS ? x0 + kOuter > n : y0 + 64 > n);
+      const bool hidden = MASK || (KEYS ? x0 + kOuter > n : y0 + 64 > n);
       unsigned keep[2] = {~0u, ~0u};
       if (hidden) {
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           if (KEYS) {
             keep[w] = alive >> lane & 1u ? ~0u : 0u;
-            if (a.bits && !key_mask) {
+            if (MASK && !key_mask) {
               // lane k has the word of query y0 + 32 w + k for the warp's 32 keys; each lane
               // gathers its own key's bit of all 32
               const int head = ho * shared_heads + t / q_tiles;
@@ -559,14 +561,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // with a mask, another warp has looked the tiles over
       const auto arrived1 = [&](int j) {
         const int st = j % S::kStages1, left = n - (t0 + j) * kInner;
-        if (!tc_wait_warp(a.bits ? &y1_clean[st] : &y1_full[st], j / S::kStages1 & 1)) return false;
-        if (!KEYS && !a.bits && warp == 8 && left < kInner)  // k past the length
+        if (!tc_wait_warp(MASK ? &y1_clean[st] : &y1_full[st], j / S::kStages1 & 1)) return false;
+        if (!KEYS && !MASK && warp == 8 && left < kInner)  // k past the length
           clear_rows<S::kBoxes>(sm_y1 + st * S::kInnerBytes, left, make_uint4(~0u, ~0u, ~0u, ~0u));
         return true;
       };
       const auto arrived2 = [&](int j) {
         const int st = j % S::kStages2;
-        return tc_wait_warp(KEYS && a.bits ? &y2_clean[st] : &y2_full[st], j / S::kStages2 & 1);
+        return tc_wait_warp(KEYS && MASK ? &y2_clean[st] : &y2_full[st], j / S::kStages2 & 1);
       };
       const auto when = [&](uint64_t* bar, int j) {
         const bool done = tc_wait_warp(bar, j & 1);
@@ -641,7 +643,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       if (!ok && count > 0) gave_up = 1;
-    } else if (warp == 11 && KEYS && a.bits) {
+    } else if (warp == 11 && KEYS && MASK) {
       // ---- nor must what q and dO hold at queries that keep no key reach dk and dv
       for (int j = 0; j < count; ++j) {
         const int st1 = j % S::kStages1, st2 = j % S::kStages2;
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (some) clear_rows<S::kBoxes>(sm_y2 + st2 * S::kInnerBytes, kInner, rows);
         mbar_arrive_warp(&y2_clean[st2]);
       }
-    } else if (warp == 11 && !KEYS && a.bits) {
+    } else if (warp == 11 && !KEYS && MASK) {
       // ---- what k holds at keys that no query of the item's key head keeps must not reach dq, where
       // 0 times NaN would be added: those rows are set to zero before the products may read them
       for (int j = 0; j < count; ++j) {
@@ -750,12 +752,12 @@ size_t attention_backward_workspace(const gs_attention_args& a) {
   return attention_mask_bytes(a) + backward_plan(a).bytes;
 }
 
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, bool KEYS, bool MASK>
 static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&m)[4],
                                    bool overlapped, cudaStream_t stream) {
-  const auto kernel = attention_backward_kernel<T, DP, KEYS>;
+  const auto kernel = attention_backward_kernel<T, DP, KEYS, MASK>;
   const cudaError_t err =
-      allow_shared<attention_backward_kernel<T, DP, KEYS>>(BackwardShared<DP, KEYS>::kBytes);
+      allow_shared<attention_backward_kernel<T, DP, KEYS, MASK>>(BackwardShared<DP, KEYS>::kBytes);
   if (err != cudaSuccess) return err;
   const int rows = KEYS ? p.a.Lk : p.a.Lq, heads = KEYS ? p.a.Hkv : p.a.Hq;
   const dim3 grid((rows + kOuter - 1) / kOuter * p.a.B * heads, p.splits);
@@ -764,6 +766,16 @@ static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&
                              m[0], m[1], m[2], m[3]);
   kernel<<<grid, kBwdThreads, BackwardShared<DP, KEYS>::kBytes, stream>>>(p, m[0], m[1], m[2], m[3]);
   return cudaGetLastError();
+}
+
+template <typename T, bool KEYS>
+static cudaError_t launch_backward(const BackwardParams& p, const CUtensorMap (&m)[4],
+                                   bool overlapped, cudaStream_t stream) {
+  if (p.a.bits)
+    return p.a.D <= 64 ? launch_backward<T, 64, KEYS, true>(p, m, overlapped, stream)
+                       : launch_backward<T, 128, KEYS, true>(p, m, overlapped, stream);
+  return p.a.D <= 64 ? launch_backward<T, 64, KEYS, false>(p, m, overlapped, stream)
+                     : launch_backward<T, 128, KEYS, false>(p, m, overlapped, stream);
 }
 
 template <typename T>
@@ -827,8 +839,7 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
     p.splits = plan.key_splits;
     p.part1 = parts, p.part2 = parts + plan.key_floats;
     const CUtensorMap m[4] = {map_k, map_v, map_q, map_g};
-    GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, true>(p, m, stat_rows > 0, stream))
-                      : (launch_backward<T, 128, true>(p, m, stat_rows > 0, stream)));
+    GS_CUDA((launch_backward<T, true>(p, m, stat_rows > 0, stream)));
     count_launches(1u);
     if (p.splits > 1) {
       GS_CUDA(launch_add<T>(p.part1, p.splits, p.a.dk, a.Lk, a.Hkv, a.B, a.D, stream));
@@ -844,8 +855,7 @@ static int run_backward(const gs_attention_args& a, const gs_token_view& dout,
   const CUtensorMap m[4] = {map_q, map_g, map_k, map_v};
   // dq starts beside the end of dk and dv, unless both use the parts in turn
   const bool beside = a.Lk > 0 && (plan.key_splits == 1 || plan.query_splits == 1);
-  GS_CUDA(a.D <= 64 ? (launch_backward<T, 64, false>(p, m, beside, stream))
-                    : (launch_backward<T, 128, false>(p, m, beside, stream)));
+  GS_CUDA((launch_backward<T, false>(p, m, beside, stream)));
   count_launches(1u);
   if (p.splits > 1) {
     GS_CUDA(launch_add<T>(p.part1, p.splits, p.a.dq, a.Lq, a.Hq, a.B, a.D, stream));
