@@ -30,11 +30,11 @@
 // 4.3 ms, 18 units of executed products of 2.7e11 operations, 1,150 to 1,170 TFLOP/s, 84 to 86% of what a
 // library product sustains under the power cap (1,357).
 //
-// delta is formed from the output as it was written, in 16 bits: an error of 2^-9 (half 2^-12) |dO| |O| of
-// a row, next to which that of dS's own rounding is of the same size, so that a gradient is about 1.4
-// roundings off instead of one. A 32-bit copy of the output, written by the forward and read here, would cost 6
-// bytes a number more (8 us of 560 at 4,096 x 4,096, 16 heads of 128) and twice the output's memory between
-// the two.
+// The rounding of P and dS makes a gradient about 1.4 roundings off instead of one (in norm, random inputs:
+// 2.33e-3 for bfloat16, 1.66e-3 for the exact gradient rounded once). delta is formed from the output as it was
+// written, in 16 bits, which adds little to that: 2.33e-3 -> 2.37e-3 with 1,200 keys of 64 numbers, 2.45e-3 ->
+// 2.52e-3 with 64 keys of 80. A 32-bit copy of the output, written by the forward and read here, would
+// take twice the output's memory between the two.
 //
 // P and dS are rounded to the products' 16-bit type, a relative error for bfloat16 down to 2^-126,
 // where the exponential's results and the products' operands end. Both are formed 2^32 times
