@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   using PS = ProbabilityScale<T>;
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t x_full, y1_full[S::kStages1], y1_free[S::kStages1], y2_full[S::kStages2],
-      y2_free[S::kStages2], y1_clean[S::kStages1], y2_clean[S::kStages2], s_full, s_read, dp_full, p_ready, ds_ready, acc_done, acc_full;
+      y2_free[S::kStages2], y1_clean[S::kStages1], y2_clean[S::kStages2], s_full, s_read, dp_full,
+      p_ready, ds_ready, acc_done, acc_full;
   __shared__ unsigned tmem_slot;
   __shared__ volatile int gave_up;
   const unsigned base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -307,12 +308,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_set(&acc_full, 1);
     for (int i = 0; i < S::kStages1; ++i) {
       mbar_set(&y1_full[i], 1);
-      mbar_set(&y1_clean[i], 1);
+      if (MASK) mbar_set(&y1_clean[i], 1);
       mbar_set(&y1_free[i], 1);
     }
     for (int i = 0; i < S::kStages2; ++i) {
       mbar_set(&y2_full[i], 1);
-      mbar_set(&y2_clean[i], 1);
+      if (MASK && KEYS) mbar_set(&y2_clean[i], 1);
       mbar_set(&y2_free[i], 1);
     }
     for (uint64_t* bar : {&s_full, &dp_full, &acc_done}) mbar_set(bar, 1);

@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(256) mask_parts_kernel(const unsigned char* ma
   }
   if (writes) {
     const int w = w0 + lane;
-    kept[((long long)group * (m.words / 4) + w / 4) * g.parts * 4 + (slot - group * g.parts) * 4 + w % 4] = any;
+    const long long tile = (long long)group * (m.words / 4) + w / 4;
+    kept[(tile * g.parts + (slot - group * g.parts)) * 4 + w % 4] = any;
   }
 }
 
